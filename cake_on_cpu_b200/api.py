@@ -125,6 +125,23 @@ _SIGNATURES["cakeb200_get_option"] = (_i, [ctypes.c_char_p])
 _SIGNATURES["cakeb200_select_devices"] = (_i, [_pi, _i, _i, _i, _i, _i, _pi])
 _SIGNATURES["cakeb200_sgemm_noalloc"] = (_i, [_vp, _vp, _vp, _i, _i, _i, _vp])
 
+F32, F16, BF16 = 0, 1, 2
+_ll = ctypes.c_longlong
+
+
+class _Q4(ctypes.Structure):
+    """cakeb200_q4."""
+    _fields_ = [("packed", _vp), ("out_features", _i), ("in_features", _i), ("group", _i), ("scale_type", _i), ("has_zeros", _i)]
+
+
+_pq4 = ctypes.POINTER(_Q4)
+_SIGNATURES["cakeb200_q4_packed_bytes"] = (_sz, [_i, _i, _i, _i])
+_SIGNATURES["cakeb200_q4_quantize"] = (_i, [_vp, _ll, _i, _i, _i, _i, _i, _vp, _ll, _vp, _vp, _vp])
+_SIGNATURES["cakeb200_q4_pack"] = (_i, [_vp, _ll, _vp, _vp, _i, _i, _i, _i, _vp, _vp])
+_SIGNATURES["cakeb200_q4_dequantize"] = (_i, [_pq4, _vp, _ll, _i, _vp])
+_SIGNATURES["cakeb200_q4_linear"] = (_i, [_pq4, _vp, _ll, _vp, _vp, _ll, _i, _i, _vp])
+_SIGNATURES["cakeb200_q4_linear_dx"] = (_i, [_pq4, _vp, _ll, _vp, _ll, _i, _i, _vp])
+
 EXPORTED_SYMBOLS = sorted(_SIGNATURES)
 
 
@@ -613,6 +630,203 @@ def cake_sgemm_planes(A, B, C=None, sch=NA, accumulate=False, stream=None):
     _check(lib().cakeb200_sgemm_planes(A._h if pa else None, None if pa else _ptr(A), B._h if pb else None, None if pb else _ptr(B),
                                        _ptr(C), M, N, K, int(bool(accumulate)), sch, _stream_of(C, stream)))
     return C
+
+
+# ------------------------------------------------------- weights held in 4 bits
+
+def _type_code(dtype, what, allowed=(F32, F16, BF16)):
+    """The C ABI's number of a torch element type; raises for one the operator does not take."""
+    import torch
+    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(dtype)
+    if code not in allowed:
+        raise TypeError("%s cannot be %s" % (what, dtype))
+    return code
+
+
+def _rows_of(t, cols, what, device, dtype=None):
+    """Checks a CUDA matrix of `cols` columns given with any leading dimensions, and returns (address, rows, leading
+    dimension) of it as one matrix; raises when its rows are not contiguous or not evenly spaced."""
+    if not (_is_torch(t) and t.is_cuda):
+        raise TypeError("%s must be a CUDA tensor" % what)
+    if t.device != device:
+        raise ValueError("%s is on %s, the weights are on %s" % (what, t.device, device))
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError("%s is %s, expected %s" % (what, t.dtype, dtype))
+    if t.dim() == 0 or t.shape[-1] != cols:
+        raise ValueError("%s has shape %s, expected (..., %d)" % (what, tuple(t.shape), cols))
+    if t.dim() == 2:
+        m = t
+    elif t.dim() == 1:
+        m = t[None]
+    else:
+        try:
+            m = t.view(-1, cols)
+        except RuntimeError:
+            raise TypeError("%s: its leading dimensions cannot be taken as one row dimension; call .contiguous()" % what) from None
+    rows = m.shape[0]
+    if rows and m.stride(1) != 1 and cols > 1:
+        raise TypeError("%s must have contiguous rows" % what)
+    ld = m.stride(0) if rows > 1 else cols
+    if ld < cols:
+        raise TypeError("%s: its rows overlap" % what)
+    return m.data_ptr(), rows, ld
+
+
+class _on_device:
+    """Around a call on a tensor's device: makes the device current, and with an explicit ``stream`` (a raw
+    cudaStream_t or a torch stream) that stream too, so that what the call allocates belongs to the stream it is
+    used on.  Gives the raw stream."""
+
+    def __init__(self, device, stream):
+        import torch
+        self.around = []
+        if stream is not None:
+            raw = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+            if raw != torch.cuda.current_stream(device).cuda_stream:
+                s = torch.cuda.ExternalStream(raw, device=device) if raw else torch.cuda.default_stream(device)
+                self.around = [torch.cuda.stream(s)]
+        else:
+            raw = torch.cuda.current_stream(device).cuda_stream
+        if torch.cuda.current_device() != device.index:
+            self.around.insert(0, torch.cuda.device(device))
+        self.raw = _vp(raw)
+
+    def __enter__(self):
+        for a in self.around:
+            a.__enter__()
+        return self.raw
+
+    def __exit__(self, *exc):
+        for a in reversed(self.around):
+            a.__exit__(*exc)
+
+
+class Q4Weights:
+    """A linear layer's weight in 4 bits, laid out once for the products that read it (cakeb200_q4_pack):
+    w[n, k] = scale[n, k // group] * (code[n, k] - zero[n, k // group]).
+
+    ``codes``: uint8 CUDA tensor (out_features, ceil(in_features / 2)), two codes to a byte, the even input feature in the
+    low half.  ``scales``: float16 or bfloat16, (out_features, ceil(in_features / group)).  ``zeros``: uint8 of the same shape
+    with values 0..15, or None for 8 everywhere.  ``group``: 32, 64 or 128.  ``in_features`` tells an odd number of input
+    features from the even one above it.  ``Q4Weights.quantize(W)`` makes all of them from a matrix."""
+
+    def __init__(self, codes, scales, zeros=None, group=128, in_features=None, stream=None):
+        import torch
+        for t, what in ((codes, "codes"), (scales, "scales")) + (((zeros, "zeros"),) if zeros is not None else ()):
+            if not (_is_torch(t) and t.is_cuda):
+                raise TypeError("%s must be a CUDA tensor" % what)
+            if t.dim() != 2 or not t.is_contiguous():
+                raise TypeError("%s must be a contiguous matrix" % what)
+            if t.device != codes.device:
+                raise ValueError("%s is on %s, the codes are on %s" % (what, t.device, codes.device))
+        if codes.dtype != torch.uint8 or (zeros is not None and zeros.dtype != torch.uint8):
+            raise TypeError("codes and zeros are uint8")
+        self.scale_type = _type_code(scales.dtype, "scales", (F16, BF16))
+        self.out_features = codes.shape[0]
+        self.in_features = 2 * codes.shape[1] if in_features is None else int(in_features)
+        if group not in (32, 64, 128):
+            raise ValueError("group is 32, 64 or 128, not %r" % (group,))
+        if self.out_features < 1 or self.in_features < 1 or (self.in_features + 1) // 2 != codes.shape[1]:
+            raise ValueError("codes have shape %s, which does not hold %d input features" % (tuple(codes.shape), self.in_features))
+        self.group = int(group)
+        groups = -(-self.in_features // self.group)
+        _need_shape(scales, (self.out_features, groups), "scales")
+        if zeros is not None:
+            _need_shape(zeros, (self.out_features, groups), "zeros")
+            if not torch.cuda.is_current_stream_capturing() and int(zeros.max()) > 15:
+                raise ValueError("zero points are 0..15")
+        self.device = codes.device
+        n = lib().cakeb200_q4_packed_bytes(self.out_features, self.in_features, self.group, int(zeros is not None))
+        with _on_device(self.device, stream) as s:
+            self.packed = torch.empty(n, dtype=torch.uint8, device=self.device)
+            self._c = _Q4(self.packed.data_ptr(), self.out_features, self.in_features, self.group, self.scale_type, int(zeros is not None))
+            self._ref = ctypes.byref(self._c)
+            _check(lib().cakeb200_q4_pack(_vp(codes.data_ptr()), codes.stride(0), _vp(scales.data_ptr()),
+                                          _vp(zeros.data_ptr()) if zeros is not None else None, self.out_features, self.in_features,
+                                          self.group, self.scale_type, _vp(self.packed.data_ptr()), s))
+
+    @staticmethod
+    def quantize_codes(W, group=128, symmetric=True, scale_dtype=None, stream=None):
+        """(codes, scales, zeros or None) of a float32, float16 or bfloat16 matrix (cakeb200_q4_quantize)."""
+        import torch
+        scale_dtype = torch.float16 if scale_dtype is None else scale_dtype
+        if not (_is_torch(W) and W.is_cuda):
+            raise TypeError("W must be a CUDA tensor")
+        if W.dim() != 2 or W.shape[0] < 1 or W.shape[1] < 1:
+            raise ValueError("W must be a matrix")
+        if group not in (32, 64, 128):
+            raise ValueError("group is 32, 64 or 128, not %r" % (group,))
+        t = _type_code(W.dtype, "W")
+        st = _type_code(scale_dtype, "scales", (F16, BF16))
+        p, n, ld = _rows_of(W, W.shape[1], "W", W.device)
+        k = W.shape[1]
+        with _on_device(W.device, stream) as s:
+            codes = torch.empty((n, (k + 1) // 2), dtype=torch.uint8, device=W.device)
+            scales = torch.empty((n, -(-k // group)), dtype=scale_dtype, device=W.device)
+            zeros = None if symmetric else torch.empty(scales.shape, dtype=torch.uint8, device=W.device)
+            _check(lib().cakeb200_q4_quantize(_vp(p), ld, t, n, k, group, st, _vp(codes.data_ptr()), codes.stride(0), _vp(scales.data_ptr()),
+                                              _vp(zeros.data_ptr()) if zeros is not None else None, s))
+        return codes, scales, zeros
+
+    @classmethod
+    def quantize(cls, W, group=128, symmetric=True, scale_dtype=None, stream=None):
+        codes, scales, zeros = cls.quantize_codes(W, group, symmetric, scale_dtype, stream)
+        return cls(codes, scales, zeros, group=group, in_features=W.shape[1], stream=stream)  # they were allocated on `stream`
+
+    def dequantize(self, dtype=None, out=None, stream=None):
+        """The matrix (out_features, in_features) the codes stand for."""
+        import torch
+        t = _type_code(out.dtype if out is not None else dtype or torch.float32, "out")
+        with _on_device(self.device, stream) as s:
+            if out is None:
+                out = torch.empty((self.out_features, self.in_features), dtype=dtype or torch.float32, device=self.device)
+            _need_shape(out, (self.out_features, self.in_features), "out")
+            p, _, ld = _rows_of(out, self.in_features, "out", self.device)
+            _check(lib().cakeb200_q4_dequantize(self._ref, p, ld, t, s))
+        return out
+
+
+def _need_q4(W4):
+    if not isinstance(W4, Q4Weights):
+        raise TypeError("the weights must be a Q4Weights object")
+
+
+def _q4_product(dx, what, src, W4, cols_in, cols_out, bias, out, stream):
+    import torch
+    p, rows, ld = _rows_of(src, cols_in, what, W4.device)
+    t = _type_code(src.dtype, what)
+    shape = src.shape[:-1] + (cols_out,)
+    if bias is not None:
+        if bias.dim() != 1:
+            raise ValueError("bias must be a vector")
+        pb = _rows_of(bias, cols_out, "bias", W4.device, src.dtype)[0]
+    else:
+        pb = None
+    if out is not None:
+        _need_shape(out, shape, "out")
+        po, _, ldo = _rows_of(out, cols_out, "out", W4.device, src.dtype)
+    with _on_device(W4.device, stream) as s:
+        if out is None:
+            out = torch.empty(shape, dtype=src.dtype, device=src.device)
+            po, ldo = out.data_ptr(), cols_out
+        if dx:
+            _check(lib().cakeb200_q4_linear_dx(W4._ref, p, ld, po, ldo, rows, t, s))
+        else:
+            _check(lib().cakeb200_q4_linear(W4._ref, p, ld, pb, po, ldo, rows, t, s))
+    return out
+
+
+def cake_q4_linear(x, W4, bias=None, out=None, stream=None):
+    """x @ W.T (+ bias) with W a ``Q4Weights`` (cakeb200_q4_linear), enqueued on the current stream.  x: CUDA tensor
+    (..., in_features) in float32, float16 or bfloat16 with contiguous, evenly spaced rows; bias and result have its type."""
+    _need_q4(W4)
+    return _q4_product(False, "x", x, W4, W4.in_features, W4.out_features, bias, out, stream)
+
+
+def cake_q4_linear_dx(dy, W4, out=None, stream=None):
+    """dy @ W with W a ``Q4Weights`` (cakeb200_q4_linear_dx): the gradient of ``cake_q4_linear`` for its input."""
+    _need_q4(W4)
+    return _q4_product(True, "dy", dy, W4, W4.out_features, W4.in_features, None, out, stream)
 
 
 def tune(A, B, C=None, sch=NA, trials=24, stream=None):

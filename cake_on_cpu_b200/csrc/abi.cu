@@ -39,6 +39,8 @@ const char* const g_option_names[OPT_COUNT] = {"tile_n", "band", "k_pieces", "ch
 }  // namespace
 int option_get(int id) { return (id >= 0 && id < OPT_COUNT) ? g_options[id].load() : 0; }
 
+cakeb200_stats* thread_stats() { return &g_stats; }
+
 void set_error(const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);

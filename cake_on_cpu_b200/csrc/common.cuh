@@ -67,6 +67,11 @@ struct OwnerSlots {
     unsigned* done;  // counter in this GPU's memory: CTAs of the storing kernel that have finished
 };
 
+// the statistics that cakeb200_get_stats returns on the calling thread (abi.cu)
+cakeb200_stats* thread_stats();
+// device (or managed) memory that kernels of the current device may use (q4.cu)
+bool on_current_device(const void* p);
+
 // Per-device state: scratch arena that grows on demand and is reused between calls.
 struct DeviceState {
     int device = -1;

@@ -1,0 +1,773 @@
+// Products with weights held in 4 bits (the packed form is described in q4.cuh):
+//     y[r, n] = sum_k x[r, k] w[n, k] (+ bias[n])        and its gradient for the input
+//     dx[r, k] = sum_n dy[r, n] w[n, k].
+//
+// With few rows both are bound by reading the codes from HBM: half a byte per multiply-add and row.  What stands in
+// the way of that bound is the work of turning codes into numbers.  At 6.4 TB/s an SM receives 46 codes per clock, so a
+// lane may spend 2.8 instructions on one.  Converting a code to FP32 and multiplying takes about four; here a pair of
+// codes becomes a pair of exact 16-bit integers q - z with one LOP3 and one packed subtraction (the code is placed in
+// the mantissa of a power of two, 128 or 1024, which is subtracted again together with z), and mma.m16n8k16 multiplies
+// 16 x 16 of them with up to eight rows of x at once: 1.4 instructions per code, whatever the number of rows up to eight.
+// The products are exact and summed in FP32; a group's sum is multiplied by its scale in FP32 and added to the row's
+// total, so scales are never rounded into the weights.  (tcgen05.mma would take the weights from shared memory: writing
+// converted codes there costs four times the bytes that are read from HBM.)
+//
+// A 32-bit x goes through the 16-bit multiplier as three terms x = x0 + x1 + x2 of 8 mantissa bits each (truncations,
+// so the split is exact and cannot overflow); the three products land in the same FP32 sums.
+#include <algorithm>
+
+#include "q4.cuh"
+
+namespace cakeb200 {
+namespace {
+
+constexpr int WARPS = 8;
+constexpr int THREADS = WARPS * 32;
+constexpr int MAX_CLUSTER = 8;
+
+// ------------------------------------------------------------------ small device helpers
+
+template <typename T> struct Mma;
+template <> struct Mma<__half> {
+    static constexpr uint32_t MAGIC = 0x64006400u;  // 1024 in both halves: its last mantissa bit counts 1
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    static __device__ __forceinline__ void run(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <> struct Mma<__nv_bfloat16> {
+    static constexpr uint32_t MAGIC = 0x43004300u;  // 128 in both halves
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    static __device__ __forceinline__ void run(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+// element type of the MMA and number of terms per element of x
+template <typename T> struct Input { using M = T; static constexpr int TERMS = 1; };
+template <> struct Input<float> { using M = __nv_bfloat16; static constexpr int TERMS = 3; };
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// v = t0 + t1 + ... with every term a bf16 (the upper half of an FP32), by truncation; a pair of values at a time.
+// An infinite value has only its first term (inf - inf would make the sum NaN where the product is infinite).
+template <int TERMS>
+__device__ __forceinline__ void split_pair(float v0, float v1, uint32_t* out) {
+#pragma unroll
+    for (int t = 0; t < TERMS; t++) {
+        out[t] = __byte_perm(__float_as_uint(v0), __float_as_uint(v1), 0x7632);
+        if (t + 1 < TERMS) {
+            const float h0 = __uint_as_float(__float_as_uint(v0) & 0xffff0000u), h1 = __uint_as_float(__float_as_uint(v1) & 0xffff0000u);
+            v0 = (t == 0 && isinf(v0)) ? 0.f : v0 - h0;
+            v1 = (t == 0 && isinf(v1)) ? 0.f : v1 - h1;
+        }
+    }
+}
+
+// Codes of one word -> the four A registers of its MMA, exact integers q - z.  sub_lo / sub_hi: MAGIC + z of rows a / a + 8.
+template <typename M>
+__device__ __forceinline__ void unpack_word(uint32_t w, uint32_t sub_lo, uint32_t sub_hi, uint32_t* a) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | Mma<M>::MAGIC;
+        a[i] = Mma<M>::sub(v, (i & 1) ? sub_hi : sub_lo);
+    }
+}
+// 16-bit pattern of MAGIC + z in both halves (z < 16: exact, and its bits lie below the magic's)
+template <typename M>
+__device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
+    return Mma<M>::MAGIC | (z << 16) | z;
+}
+
+__device__ __forceinline__ uint4 load_codes(const uint4* p) {
+    uint4 v;  // read once: not kept in L1, where x and the scales live
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float load_remote(const float* local, int rank) {
+    uint32_t a = (uint32_t) __cvta_generic_to_shared(local), r;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+    return v;
+}
+
+// Sums `red`[WARPS][E] over the warps of the CTA and then over the CTAs of the cluster, in that fixed order, and hands
+// every element of this CTA's share to `store(e, value)`.
+template <int E, typename F>
+__device__ __forceinline__ void reduce_and_store(float* red, int rank, int cluster, F store) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += THREADS) {
+        float s = red[e];
+#pragma unroll
+        for (int w = 1; w < WARPS; w++) s += red[w * E + e];
+        red[e] = s;
+        if (cluster == 1) store(e, s);
+    }
+    if (cluster == 1) return;
+    cluster_sync();
+    const int per = E / cluster;
+    for (int i = threadIdx.x; i < per; i += THREADS) {
+        const int e = rank * per + i;
+        float s = 0.f;
+        for (int c = 0; c < cluster; c++) s += load_remote(red + e, c);
+        store(e, s);
+    }
+    cluster_sync();  // nobody leaves while its sums are still being read
+}
+
+struct Q4Args {
+    Q4View w;
+    const void* in;      // x (rows x K) or dy (rows x N)
+    void* out;           // y (rows x N) or dx (rows x K)
+    const void* bias;    // N elements of the input's type, or nullptr
+    long long ld_in, ld_out;
+    int rows;
+    int vec;             // 16-byte loads of x allowed
+    int cluster;
+};
+
+// ------------------------------------------------------------------ y = x W^T + b
+
+// B fragments of one 32-feature half of a block for one tile of eight rows: lane (a, t) holds features 8 t .. 8 t + 7 of row a.
+template <typename T>
+__device__ __forceinline__ void load_x(const Q4Args& p, int row, int k, uint32_t (*b)[Input<T>::TERMS]) {
+    constexpr int TERMS = Input<T>::TERMS;
+    if (row >= p.rows || k >= p.w.K) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) b[i][t] = 0u;
+        return;
+    }
+    const T* x = (const T*) p.in + row * p.ld_in + k;
+    if constexpr (sizeof(T) == 2) {
+        if (p.vec && k + 8 <= p.w.K) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(x));
+            b[0][0] = v.x; b[1][0] = v.y; b[2][0] = v.z; b[3][0] = v.w;
+        } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t lo = k + 2 * i < p.w.K ? __ldg(h + 2 * i) : 0, hi = k + 2 * i + 1 < p.w.K ? __ldg(h + 2 * i + 1) : 0;
+                b[i][0] = lo | (hi << 16);
+            }
+        }
+    } else {
+        float v[8];
+        if (p.vec && k + 8 <= p.w.K) {
+            const float4 u0 = __ldg(reinterpret_cast<const float4*>(x)), u1 = __ldg(reinterpret_cast<const float4*>(x) + 1);
+            v[0] = u0.x; v[1] = u0.y; v[2] = u0.z; v[3] = u0.w; v[4] = u1.x; v[5] = u1.y; v[6] = u1.z; v[7] = u1.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = k + i < p.w.K ? __ldg(x + i) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) split_pair<TERMS>(v[2 * i], v[2 * i + 1], b[i]);
+    }
+}
+
+// A CTA computes R block rows (16 R output features) x 8 NT rows of x; its warps share out the k blocks of the CTA, the
+// CTAs of a cluster those of the product.
+template <typename T, int NT, int R>
+__global__ void __launch_bounds__(THREADS)
+q4_linear_kernel(const Q4Args p) {
+    using M = typename Input<T>::M;
+    constexpr int TERMS = Input<T>::TERMS;
+    constexpr int E = R * NT * 128;
+    __shared__ float red[WARPS * E];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, a = lane >> 2, t = lane & 3;
+    const int rank = (int) blockIdx.x % p.cluster, rb = (int) blockIdx.x / p.cluster;
+    const int row0 = (int) blockIdx.y * 8 * NT;
+    const int part = rank * WARPS + warp, parts = p.cluster * WARPS;
+    const int kb0 = (int) ((long long) p.w.k_blocks * part / parts), kb1 = (int) ((long long) p.w.k_blocks * (part + 1) / parts);
+    const bool small_group = p.w.group == 32;
+
+    float total[R][NT][4] = {};
+    const uint4* codes[R];
+    const uint16_t* scales[R];
+    const uint8_t* zeros[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int rt = min(rb * R + r, p.w.row_tiles - 1);  // a block row past the end repeats the last one and is not stored
+        codes[r] = p.w.codes + (long long) rt * p.w.k_blocks * 32 + lane;
+        scales[r] = p.w.scales + (long long) rt * p.w.groups * 16 + a * 2;
+        zeros[r] = p.w.zeros ? p.w.zeros + (long long) rt * p.w.groups * 16 + a * 2 : nullptr;
+    }
+    uint4 next[R];
+    if (kb0 < kb1) {
+#pragma unroll
+        for (int r = 0; r < R; r++) next[r] = load_codes(codes[r] + (long long) kb0 * 32);
+    }
+    for (int kb = kb0; kb < kb1; kb++) {
+        uint4 now[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            now[r] = next[r];
+            if (kb + 1 < kb1) next[r] = load_codes(codes[r] + (long long) (kb + 1) * 32);
+        }
+        uint32_t b[NT][8][TERMS];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) load_x<T>(p, row0 + nt * 8 + a, kb * 64 + h * 32 + t * 8, &b[nt][4 * h]);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float acc[NT][4] = {};
+            const uint32_t words[4] = {now[r].x, now[r].y, now[r].z, now[r].w};
+            uint32_t sub_lo = 0, sub_hi = 0;
+            float s_lo = 0.f, s_hi = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j == 0 || (j == 2 && small_group)) {
+                    if (j == 2) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            total[r][nt][0] += s_lo * acc[nt][0]; total[r][nt][1] += s_lo * acc[nt][1];
+                            total[r][nt][2] += s_hi * acc[nt][2]; total[r][nt][3] += s_hi * acc[nt][3];
+                            acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+                        }
+                    }
+                    const int g = (kb * 64 + j * 16) / p.w.group;
+                    const uint32_t pair = __ldg(reinterpret_cast<const uint32_t*>(scales[r] + (long long) g * 16));
+                    s_lo = q4_scale((uint16_t) (pair & 0xffffu), p.w.scale_bf16);
+                    s_hi = q4_scale((uint16_t) (pair >> 16), p.w.scale_bf16);
+                    uint32_t z = 0x0808u;
+                    if (zeros[r]) z = __ldg(reinterpret_cast<const uint16_t*>(zeros[r] + (long long) g * 16));
+                    sub_lo = zero_pair<M>(z & 15u);
+                    sub_hi = zero_pair<M>((z >> 8) & 15u);
+                }
+                uint32_t w[4];
+                unpack_word<M>(words[j], sub_lo, sub_hi, w);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int u = TERMS - 1; u >= 0; u--) Mma<M>::run(acc[nt], w, b[nt][2 * j][u], b[nt][2 * j + 1][u]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                total[r][nt][0] += s_lo * acc[nt][0]; total[r][nt][1] += s_lo * acc[nt][1];
+                total[r][nt][2] += s_hi * acc[nt][2]; total[r][nt][3] += s_hi * acc[nt][3];
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) red[warp * E + ((r * NT + nt) * 4 + i) * 32 + lane] = total[r][nt][i];
+    T* out = (T*) p.out;
+    const T* bias = (const T*) p.bias;
+    reduce_and_store<E>(red, rank, p.cluster, [&](int e, float v) {
+        const int l = e & 31, i = (e >> 5) & 3, nt = (e >> 7) % NT, r = (e >> 7) / NT;
+        const int n = (rb * R + r) * 16 + (l >> 2) + (i >> 1) * 8, row = row0 + nt * 8 + (l & 3) * 2 + (i & 1);
+        if (n >= p.w.N || row >= p.rows) return;
+        if (bias) v += to_float(bias[n]);
+        out[row * p.ld_out + n] = from_float<T>(v);
+    });
+}
+
+// ------------------------------------------------------------------ dx = dy W
+
+// 8 x 8 matrix of 16-bit elements, transposed across the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t o;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(o) : "r"(v));
+    return o;
+}
+
+// A CTA computes one k block (64 input features) x 8 NT rows; its warps share out the block rows of the CTA, the CTAs
+// of a cluster those of the product.  The reduction runs over output features, whose scales differ, so the scale goes
+// into the other operand: dy[r, n] s[n, g], formed in FP32 and split into TERMS bf16 terms (two for 16-bit types: 2^-16
+// relative, far below their own rounding; three for FP32).  Sums of one block row (16 n) leave the MMA for an FP32 total.
+template <typename T, int NT>
+__global__ void __launch_bounds__(THREADS)
+q4_linear_dx_kernel(const Q4Args p) {
+    using M = __nv_bfloat16;
+    constexpr int TERMS = sizeof(T) == 4 ? 3 : 2;
+    constexpr int E = NT * 512;
+    __shared__ float red[WARPS * E];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, a = lane >> 2, t = lane & 3;
+    const int rank = (int) blockIdx.x % p.cluster, kb = (int) blockIdx.x / p.cluster;
+    const int row0 = (int) blockIdx.y * 8 * NT;
+    const int part = rank * WARPS + warp, parts = p.cluster * WARPS;
+    const int rt0 = (int) ((long long) p.w.row_tiles * part / parts), rt1 = (int) ((long long) p.w.row_tiles * (part + 1) / parts);
+    const bool small_group = p.w.group == 32;
+    const T* dy = (const T*) p.in;
+
+    float total[4][NT][4] = {};
+    const uint4* codes = p.w.codes + (long long) kb * 32 + lane;
+    uint4 next = {};
+    if (rt0 < rt1) next = load_codes(codes + (long long) rt0 * p.w.k_blocks * 32);
+    for (int rt = rt0; rt < rt1; rt++) {
+        const uint4 now = next;
+        if (rt + 1 < rt1) next = load_codes(codes + (long long) (rt + 1) * p.w.k_blocks * 32);
+        const uint32_t words[4] = {now.x, now.y, now.z, now.w};
+        // this lane's four output features: 16 rt + {2 t, 2 t + 1, 2 t + 8, 2 t + 9}
+        float v[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int row = row0 + nt * 8 + a;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int n = rt * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+                v[nt][i] = (row < p.rows && n < p.w.N) ? to_float(dy[row * p.ld_in + n]) : 0.f;
+            }
+        }
+        uint32_t b[NT][2][TERMS];
+        uint32_t sub_lo = 0, sub_hi = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j == 0 || (j == 2 && small_group)) {
+                const long long at = ((long long) rt * p.w.groups + (kb * 64 + j * 16) / p.w.group) * 16;
+                const uint2 s4 = __ldg(reinterpret_cast<const uint2*>(p.w.scales + at + 4 * t));  // rows 2t, 2t+8, 2t+1, 2t+9
+                const float s0 = q4_scale((uint16_t) s4.x, p.w.scale_bf16), s2 = q4_scale((uint16_t) (s4.x >> 16), p.w.scale_bf16);
+                const float s1 = q4_scale((uint16_t) s4.y, p.w.scale_bf16), s3 = q4_scale((uint16_t) (s4.y >> 16), p.w.scale_bf16);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    split_pair<TERMS>(v[nt][0] * s0, v[nt][1] * s1, b[nt][0]);
+                    split_pair<TERMS>(v[nt][2] * s2, v[nt][3] * s3, b[nt][1]);
+                }
+                uint32_t z = 0x0808u;
+                if (p.w.zeros) z = __ldg(reinterpret_cast<const uint16_t*>(p.w.zeros + at + a * 2));
+                sub_lo = zero_pair<M>(z & 15u);
+                sub_hi = zero_pair<M>((z >> 8) & 15u);
+            }
+            uint32_t w[4], wt[4];
+            unpack_word<M>(words[j], sub_lo, sub_hi, w);
+            // registers 0, 1 hold the lower pairs of rows 0-7, 8-15, registers 2, 3 the upper pairs; transposed, the
+            // features are the rows of the A operand and 1 and 2 change places
+            wt[0] = transpose8(w[0]); wt[1] = transpose8(w[2]); wt[2] = transpose8(w[1]); wt[3] = transpose8(w[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float acc[4] = {};
+#pragma unroll
+                for (int u = TERMS - 1; u >= 0; u--) Mma<M>::run(acc, wt, b[nt][0][u], b[nt][1][u]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) total[j][nt][i] += acc[i];
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) red[warp * E + ((j * NT + nt) * 4 + i) * 32 + lane] = total[j][nt][i];
+    T* out = (T*) p.out;
+    reduce_and_store<E>(red, rank, p.cluster, [&](int e, float val) {
+        const int l = e & 31, i = (e >> 5) & 3, nt = (e >> 7) % NT, j = (e >> 7) / NT;
+        // row a of the transposed matrix is the feature of lane group a / 2, element a & 1 of its pair; rows 8..15 are the upper pairs
+        const int ar = l >> 2;
+        const int k = kb * 64 + 32 * (j >> 1) + 8 * (ar >> 1) + 4 * (j & 1) + 2 * (i >> 1) + (ar & 1);
+        const int row = row0 + nt * 8 + (l & 3) * 2 + (i & 1);
+        if (k >= p.w.K || row >= p.rows) return;
+        out[row * p.ld_out + k] = from_float<T>(val);
+    });
+}
+
+// ------------------------------------------------------------------ quantising, packing, unpacking
+
+// One warp per group of one row.  Symmetric: s = max|w| / 7, q = round(w / s) + 8.  With zero points: the range [min(w, 0),
+// max(w, 0)] is cut into 15 steps, z = round(-low / s), q = round(w / s) + z.  The scale is rounded to its 16-bit type first
+// and codes are taken with the rounded scale, so a code is the nearest one to the weight that the stored numbers allow.
+template <typename T>
+__global__ void __launch_bounds__(256)
+q4_quantize_kernel(const T* __restrict__ W, long long ldw, int N, int K, int group, int groups, int scale_bf16, uint8_t* __restrict__ codes,
+                   long long ldq, uint16_t* __restrict__ scales, uint8_t* __restrict__ zeros) {
+    const long long item = ((long long) blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    const int lane = threadIdx.x & 31;
+    if (item >= (long long) N * groups) return;
+    const int n = (int) (item / groups), g = (int) (item % groups);
+    const int k0 = g * group, k1 = min(K, k0 + group);
+    const T* row = W + n * ldw;
+    float low = 0.f, high = 0.f;
+    bool odd = false;  // a weight that is not finite makes the group's scale NaN
+    for (int k = k0 + lane; k < k1; k += 32) {
+        const float v = to_float(row[k]);
+        odd |= !isfinite(v);
+        low = fminf(low, v);
+        high = fmaxf(high, v);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    }
+    odd = __any_sync(0xffffffffu, odd);
+    float s = zeros ? __fdiv_rn(high, 15.f) - __fdiv_rn(low, 15.f) : __fdiv_rn(fmaxf(high, -low), 7.f);
+    uint16_t bits;
+    if (scale_bf16) {
+        bits = __bfloat16_as_ushort(__float2bfloat16_rn(s));
+    } else {
+        bits = __half_as_ushort(__float2half_rn(fminf(s, 65504.f)));
+        if (bits == 0 && s > 0.f) bits = 1;  // the smallest scale there is, not zero
+    }
+    if (odd) bits = 0x7fffu;  // NaN in both types
+    s = q4_scale(bits, scale_bf16);
+    const float zf = zeros && s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(-low, s)), 0.f), 15.f) : (zeros ? 0.f : 8.f);
+    const int z = (int) zf;
+    if (lane == 0) {
+        scales[(long long) n * groups + g] = bits;
+        if (zeros) zeros[(long long) n * groups + g] = (uint8_t) z;
+    }
+    for (int k = k0 + 2 * lane; k < k1; k += 64) {
+        uint32_t two = 0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            int q = z;
+            if (k + i < k1 && s > 0.f) {
+                const float v = rintf(__fdiv_rn(to_float(row[k + i]), s)) + zf;
+                q = (int) fminf(fmaxf(v, 0.f), 15.f);
+            }
+            two |= (uint32_t) q << (4 * i);
+        }
+        codes[n * ldq + k / 2] = (uint8_t) two;  // groups start at even features: a byte belongs to one group
+    }
+}
+
+// One thread per lane of a block: 32 codes gathered from two rows.
+__global__ void __launch_bounds__(256)
+q4_pack_kernel(const uint8_t* __restrict__ codes, long long ldq, int N, int K, int row_tiles, int k_blocks, uint4* __restrict__ out) {
+    const long long i = (long long) blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= (long long) row_tiles * k_blocks * 32) return;
+    const int lane = (int) (i & 31), a = lane >> 2, t = lane & 3;
+    const long long block = i >> 5;
+    const int kb = (int) (block % k_blocks), rt = (int) (block / k_blocks);
+    uint32_t words[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+            const int n = rt * 16 + a + (f & 1) * 8;
+            const int k = kb * 64 + 32 * (j >> 1) + 8 * t + 4 * (j & 1) + 2 * (f >> 1);
+            uint32_t two = 0;
+            if (n < N && k < K) two = codes[n * ldq + k / 2];
+            if (k + 1 >= K) two &= 15u;
+            w |= (two & 15u) << (4 * f) | (two >> 4) << (16 + 4 * f);
+        }
+        words[j] = w;
+    }
+    out[i] = make_uint4(words[0], words[1], words[2], words[3]);
+}
+
+__global__ void __launch_bounds__(256)
+q4_pack_scales_kernel(const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros, int N, int groups_in, int row_tiles, int groups,
+                      uint16_t* __restrict__ out_s, uint8_t* __restrict__ out_z) {
+    const long long i = (long long) blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= (long long) row_tiles * groups * 16) return;
+    const int local = (int) (i & 15);
+    const long long at = i >> 4;
+    const int g = (int) (at % groups), rt = (int) (at / groups), n = rt * 16 + local;
+    const bool in = n < N && g < groups_in;
+    const long long place = at * 16 + q4_scale_place(local);
+    out_s[place] = in ? scales[(long long) n * groups_in + g] : 0;
+    if (out_z) out_z[place] = in ? zeros[(long long) n * groups_in + g] : 0;
+}
+
+// One thread per lane of a block writes the 32 weights it holds.
+template <typename T>
+__global__ void __launch_bounds__(256)
+q4_unpack_kernel(const Q4View w, T* __restrict__ out, long long ldo) {
+    const long long i = (long long) blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= (long long) w.row_tiles * w.k_blocks * 32) return;
+    const int lane = (int) (i & 31), a = lane >> 2, t = lane & 3;
+    const long long block = i >> 5;
+    const int kb = (int) (block % w.k_blocks), rt = (int) (block / w.k_blocks);
+    const uint4 v = w.codes[i];
+    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const long long at = ((long long) rt * w.groups + (kb * 64 + j * 16) / w.group) * 16 + a * 2;
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+            const int n = rt * 16 + a + (f & 1) * 8;
+            const int k = kb * 64 + 32 * (j >> 1) + 8 * t + 4 * (j & 1) + 2 * (f >> 1);
+            const float s = q4_scale(w.scales[at + (f & 1)], w.scale_bf16);
+            const int z = w.zeros ? (w.zeros[at + (f & 1)] & 15) : 8;
+            if (n < w.N && k < w.K) out[n * ldo + k] = from_float<T>(s * (float) ((int) (words[j] >> (4 * f) & 15u) - z));
+            if (n < w.N && k + 1 < w.K) out[n * ldo + k + 1] = from_float<T>(s * (float) ((int) (words[j] >> (16 + 4 * f) & 15u) - z));
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+
+int bad(const char* who, const char* what) {
+    set_error("%s: %s", who, what);
+    return CAKEB200_ERR_ARG;
+}
+
+bool known_type(int type) { return type == CAKEB200_F32 || type == CAKEB200_F16 || type == CAKEB200_BF16; }
+
+int check_geometry(const char* who, int N, int K, int group, int scale_type) {
+    if (N <= 0 || K <= 0) return bad(who, "features must be positive");
+    if (group != 32 && group != 64 && group != 128) return bad(who, "the group is 32, 64 or 128 input features");
+    if (scale_type != CAKEB200_F16 && scale_type != CAKEB200_BF16) return bad(who, "scales are float16 or bfloat16");
+    if (K > (1 << 30) || N > (1 << 30)) {
+        set_error("%s: more than 2^30 features", who);
+        return CAKEB200_ERR_TOO_LARGE;
+    }
+    return CAKEB200_OK;
+}
+
+size_t codes_bytes(int N, int K) { return (size_t) q4_row_tiles(N) * q4_k_blocks(K) * 512; }
+size_t scales_count(int N, int K, int group) { return (size_t) q4_row_tiles(N) * q4_groups(K, group) * 16; }
+
+int blocks_for(const char* who, long long threads, unsigned* out) {
+    const long long b = (threads + 255) / 256;
+    if (b > 0x7fffffffLL) {
+        set_error("%s: the matrix is too large for one launch", who);
+        return CAKEB200_ERR_TOO_LARGE;
+    }
+    *out = (unsigned) b;
+    return CAKEB200_OK;
+}
+
+template <typename K>
+int launch_clustered(K kernel, unsigned x, unsigned y, int cluster, const Q4Args& args, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(x, y);
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned) cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CAKE_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args));
+    return CAKEB200_OK;
+}
+
+// CTAs per product along the reduction: enough of them that the machine holds a few per SM, each warp with at least one
+// block to do; a power of two up to the portable cluster size.
+int pick_cluster(long long ctas, int blocks, int sm_count) {
+    int c = 1;
+    while (c < MAX_CLUSTER && ctas * c < 4LL * sm_count && blocks >= 2 * c * WARPS) c *= 2;
+    return c;
+}
+
+template <typename T>
+int launch_linear(Q4Args& p, int sm_count, cudaStream_t s) {
+    const int tiles = (p.rows + 7) / 8;
+    const bool wide = sizeof(T) == 4 && p.rows <= 8 && p.w.row_tiles >= 8 * sm_count;
+    const int R = wide ? 4 : 2;
+    const int NT = tiles >= 3 ? 4 : tiles;
+    const unsigned rbs = (unsigned) ((p.w.row_tiles + R - 1) / R);
+    const long long chunks = (tiles + NT - 1) / NT;
+    if (chunks > 65535) {
+        set_error("q4_linear: too many rows");
+        return CAKEB200_ERR_TOO_LARGE;
+    }
+    p.cluster = pick_cluster(rbs * chunks, p.w.k_blocks, sm_count);
+    const unsigned x = rbs * (unsigned) p.cluster, y = (unsigned) chunks;
+    if (wide) return launch_clustered(q4_linear_kernel<T, 1, 4>, x, y, p.cluster, p, s);
+    if (NT == 1) return launch_clustered(q4_linear_kernel<T, 1, 2>, x, y, p.cluster, p, s);
+    if (NT == 2) return launch_clustered(q4_linear_kernel<T, 2, 2>, x, y, p.cluster, p, s);
+    return launch_clustered(q4_linear_kernel<T, 4, 2>, x, y, p.cluster, p, s);
+}
+
+template <typename T>
+int launch_dx(Q4Args& p, int sm_count, cudaStream_t s) {
+    const int tiles = (p.rows + 7) / 8, NT = tiles >= 2 ? 2 : 1;
+    const long long chunks = (tiles + NT - 1) / NT;
+    if (chunks > 65535) {
+        set_error("q4_linear_dx: too many rows");
+        return CAKEB200_ERR_TOO_LARGE;
+    }
+    p.cluster = pick_cluster(p.w.k_blocks * chunks, p.w.row_tiles, sm_count);
+    const unsigned x = (unsigned) p.w.k_blocks * (unsigned) p.cluster, y = (unsigned) chunks;
+    if (NT == 1) return launch_clustered(q4_linear_dx_kernel<T, 1>, x, y, p.cluster, p, s);
+    return launch_clustered(q4_linear_dx_kernel<T, 2>, x, y, p.cluster, p, s);
+}
+
+// Common checks of the two products.  in_cols / out_cols: row lengths of the operand and of the result.
+int product(const char* who, const cakeb200_q4* w, const void* in, long long ld_in, const void* bias, void* out, long long ld_out,
+            int rows, int type, bool dx, void* stream) {
+    *thread_stats() = cakeb200_stats();
+    Q4Args p = {};
+    int rc = q4_view(w, who, &p.w);
+    if (rc) return rc;
+    if (!known_type(type)) return bad(who, "the type is float32, float16 or bfloat16");
+    if (rows < 0) return bad(who, "negative number of rows");
+    if (rows == 0) return CAKEB200_OK;
+    if (!in || !out) return bad(who, "null pointer");
+    const int in_cols = dx ? p.w.N : p.w.K, out_cols = dx ? p.w.K : p.w.N;
+    if (rows > 1 && (ld_in < in_cols || ld_out < out_cols)) return bad(who, "a leading dimension is smaller than its row");
+    DeviceState* st = device_state();
+    if (!st) return CAKEB200_ERR_NO_DEVICE;
+    if (!on_current_device(w->packed) || !on_current_device(in) || !on_current_device(out) || (bias && !on_current_device(bias)))
+        return bad(who, "operands must be device pointers of the current device");
+    const size_t size = type == CAKEB200_F32 ? 4 : 2;
+    if ((uintptr_t) in % size || (uintptr_t) out % size || (uintptr_t) bias % size) return bad(who, "a pointer is not aligned to its type");
+    p.in = in; p.out = out; p.bias = bias;
+    p.ld_in = ld_in; p.ld_out = ld_out; p.rows = rows;
+    p.vec = (uintptr_t) in % 16 == 0 && (rows == 1 || (ld_in * (long long) size) % 16 == 0);
+    cudaStream_t s = (cudaStream_t) stream;
+    if (dx)
+        rc = type == CAKEB200_F32 ? launch_dx<float>(p, st->sm_count, s)
+             : type == CAKEB200_F16 ? launch_dx<__half>(p, st->sm_count, s) : launch_dx<__nv_bfloat16>(p, st->sm_count, s);
+    else
+        rc = type == CAKEB200_F32 ? launch_linear<float>(p, st->sm_count, s)
+             : type == CAKEB200_F16 ? launch_linear<__half>(p, st->sm_count, s) : launch_linear<__nv_bfloat16>(p, st->sm_count, s);
+    if (!rc) thread_stats()->launches = 1;
+    return rc;
+}
+
+}  // namespace
+
+bool on_current_device(const void* p) {
+    int dev = -1;
+    cudaPointerAttributes a;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return a.type == cudaMemoryTypeManaged || (a.type == cudaMemoryTypeDevice && a.device == dev);
+}
+
+int q4_view(const cakeb200_q4* w, const char* who, Q4View* out) {
+    if (!w || !w->packed) return bad(who, "null weights");
+    int rc = check_geometry(who, w->out_features, w->in_features, w->group, w->scale_type);
+    if (rc) return rc;
+    if ((uintptr_t) w->packed % 16) return bad(who, "packed weights start on a 16-byte boundary");
+    out->N = w->out_features;
+    out->K = w->in_features;
+    out->group = w->group;
+    out->groups = q4_groups(out->K, out->group);
+    out->row_tiles = q4_row_tiles(out->N);
+    out->k_blocks = q4_k_blocks(out->K);
+    out->scale_bf16 = w->scale_type == CAKEB200_BF16;
+    const char* base = (const char*) w->packed;
+    out->codes = (const uint4*) base;
+    out->scales = (const uint16_t*) (base + codes_bytes(out->N, out->K));
+    out->zeros = w->has_zeros ? (const uint8_t*) (out->scales + scales_count(out->N, out->K, out->group)) : nullptr;
+    return CAKEB200_OK;
+}
+
+}  // namespace cakeb200
+
+using namespace cakeb200;
+
+extern "C" {
+
+size_t cakeb200_q4_packed_bytes(int out_features, int in_features, int group, int has_zeros) {
+    if (check_geometry("cakeb200_q4_packed_bytes", out_features, in_features, group, CAKEB200_F16)) return 0;
+    return codes_bytes(out_features, in_features) + scales_count(out_features, in_features, group) * (has_zeros ? 3 : 2);
+}
+
+int cakeb200_q4_quantize(const void* W, long long ldw, int type, int out_features, int in_features, int group, int scale_type,
+                         void* codes, long long ldq, void* scales, void* zeros, void* stream) {
+    static const char* who = "cakeb200_q4_quantize";
+    *thread_stats() = cakeb200_stats();
+    int rc = check_geometry(who, out_features, in_features, group, scale_type);
+    if (rc) return rc;
+    if (!W || !codes || !scales) return bad(who, "null pointer");
+    if (!known_type(type)) return bad(who, "the type is float32, float16 or bfloat16");
+    if (ldw < in_features || ldq < (in_features + 1) / 2) return bad(who, "a leading dimension is smaller than its row");
+    DeviceState* st = device_state();
+    if (!st) return CAKEB200_ERR_NO_DEVICE;
+    if (!on_current_device(W) || !on_current_device(codes) || !on_current_device(scales) || (zeros && !on_current_device(zeros)))
+        return bad(who, "operands must be device pointers of the current device");
+    const int groups = (in_features + group - 1) / group;
+    unsigned blocks;
+    if ((rc = blocks_for(who, (long long) out_features * groups * 32, &blocks))) return rc;
+    cudaStream_t s = (cudaStream_t) stream;
+    const int bf = scale_type == CAKEB200_BF16;
+    if (type == CAKEB200_F32)
+        q4_quantize_kernel<float><<<blocks, 256, 0, s>>>((const float*) W, ldw, out_features, in_features, group, groups, bf, (uint8_t*) codes, ldq,
+                                                         (uint16_t*) scales, (uint8_t*) zeros);
+    else if (type == CAKEB200_F16)
+        q4_quantize_kernel<__half><<<blocks, 256, 0, s>>>((const __half*) W, ldw, out_features, in_features, group, groups, bf, (uint8_t*) codes, ldq,
+                                                          (uint16_t*) scales, (uint8_t*) zeros);
+    else
+        q4_quantize_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>((const __nv_bfloat16*) W, ldw, out_features, in_features, group, groups, bf,
+                                                                 (uint8_t*) codes, ldq, (uint16_t*) scales, (uint8_t*) zeros);
+    CAKE_CUDA_OK(cudaGetLastError());
+    thread_stats()->launches = 1;
+    return CAKEB200_OK;
+}
+
+int cakeb200_q4_pack(const void* codes, long long ldq, const void* scales, const void* zeros, int out_features, int in_features, int group,
+                     int scale_type, void* packed, void* stream) {
+    static const char* who = "cakeb200_q4_pack";
+    *thread_stats() = cakeb200_stats();
+    int rc = check_geometry(who, out_features, in_features, group, scale_type);
+    if (rc) return rc;
+    if (!codes || !scales || !packed) return bad(who, "null pointer");
+    if (ldq < (in_features + 1) / 2) return bad(who, "a leading dimension is smaller than its row");
+    if ((uintptr_t) packed % 16) return bad(who, "packed weights start on a 16-byte boundary");
+    DeviceState* st = device_state();
+    if (!st) return CAKEB200_ERR_NO_DEVICE;
+    if (!on_current_device(codes) || !on_current_device(scales) || !on_current_device(packed) || (zeros && !on_current_device(zeros)))
+        return bad(who, "operands must be device pointers of the current device");
+    const int rts = q4_row_tiles(out_features), kbs = q4_k_blocks(in_features), groups = q4_groups(in_features, group);
+    unsigned b0, b1;
+    if ((rc = blocks_for(who, (long long) rts * kbs * 32, &b0)) || (rc = blocks_for(who, (long long) rts * groups * 16, &b1))) return rc;
+    cudaStream_t s = (cudaStream_t) stream;
+    uint16_t* out_s = (uint16_t*) ((char*) packed + codes_bytes(out_features, in_features));
+    uint8_t* out_z = zeros ? (uint8_t*) (out_s + scales_count(out_features, in_features, group)) : nullptr;
+    q4_pack_kernel<<<b0, 256, 0, s>>>((const uint8_t*) codes, ldq, out_features, in_features, rts, kbs, (uint4*) packed);
+    CAKE_CUDA_OK(cudaGetLastError());
+    q4_pack_scales_kernel<<<b1, 256, 0, s>>>((const uint16_t*) scales, (const uint8_t*) zeros, out_features,
+                                             (in_features + group - 1) / group, rts, groups, out_s, out_z);
+    CAKE_CUDA_OK(cudaGetLastError());
+    thread_stats()->launches = 2;
+    return CAKEB200_OK;
+}
+
+int cakeb200_q4_dequantize(const cakeb200_q4* w, void* W, long long ldw, int type, void* stream) {
+    static const char* who = "cakeb200_q4_dequantize";
+    *thread_stats() = cakeb200_stats();
+    Q4View v;
+    int rc = q4_view(w, who, &v);
+    if (rc) return rc;
+    if (!W) return bad(who, "null pointer");
+    if (!known_type(type)) return bad(who, "the type is float32, float16 or bfloat16");
+    if (ldw < v.K) return bad(who, "a leading dimension is smaller than its row");
+    DeviceState* st = device_state();
+    if (!st) return CAKEB200_ERR_NO_DEVICE;
+    if (!on_current_device(w->packed) || !on_current_device(W)) return bad(who, "operands must be device pointers of the current device");
+    unsigned blocks;
+    if ((rc = blocks_for(who, (long long) v.row_tiles * v.k_blocks * 32, &blocks))) return rc;
+    cudaStream_t s = (cudaStream_t) stream;
+    if (type == CAKEB200_F32) q4_unpack_kernel<float><<<blocks, 256, 0, s>>>(v, (float*) W, ldw);
+    else if (type == CAKEB200_F16) q4_unpack_kernel<__half><<<blocks, 256, 0, s>>>(v, (__half*) W, ldw);
+    else q4_unpack_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(v, (__nv_bfloat16*) W, ldw);
+    CAKE_CUDA_OK(cudaGetLastError());
+    thread_stats()->launches = 1;
+    return CAKEB200_OK;
+}
+
+int cakeb200_q4_linear(const cakeb200_q4* w, const void* x, long long ldx, const void* bias, void* y, long long ldy, int rows, int type,
+                       void* stream) {
+    return product("cakeb200_q4_linear", w, x, ldx, bias, y, ldy, rows, type, false, stream);
+}
+
+int cakeb200_q4_linear_dx(const cakeb200_q4* w, const void* dy, long long lddy, void* dx, long long lddx, int rows, int type, void* stream) {
+    return product("cakeb200_q4_linear_dx", w, dy, lddy, nullptr, dx, lddx, rows, type, true, stream);
+}
+
+}  // extern "C"

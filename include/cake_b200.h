@@ -1,6 +1,6 @@
 /* cake_b200.h -- the C ABI of the B200 implementation of the CAKE SGEMM path.
  *
- * Plain pointers and sizes only.  Every matrix is FP32, row-major, dense, with
+ * Plain pointers and sizes only.  Unless its entry point says otherwise, every matrix is FP32, row-major, dense, with
  * the leading dimension equal to its column count (A[m*K+k], B[k*N+n],
  * C[m*N+n]) exactly as in vnatesh/CAKE_on_CPU (src/util.cpp:183).  Each data
  * pointer may be a HOST pointer (pageable or pinned) or a DEVICE pointer of the
@@ -41,6 +41,9 @@ enum {
     CAKEB200_KERNEL_TF32X3 = 1, /* tcgen05 tensor cores, FP32 split into two TF32 terms, 3 MMAs */
     CAKEB200_KERNEL_FFMA = 2    /* exact FP32 fused multiply-add on the CUDA cores */
 };
+
+/* Element types of the operators on a linear layer's weight (everything else in this header is FP32). */
+enum { CAKEB200_F32 = 0, CAKEB200_F16 = 1, CAKEB200_BF16 = 2 };
 
 /* Timings of the last call on this thread, milliseconds, from CUDA events. */
 typedef struct cakeb200_stats {
@@ -400,6 +403,47 @@ int cakeb200_unpack_A(float* A, const float* A_p, int M, int K, int p, const cak
                       const cakeb200_cntx* cntx, void* stream);
 int cakeb200_unpack_B(float* B, const float* B_p, int K, int N, int p, const cakeb200_blk_dims* x,
                       const cakeb200_cntx* cntx, void* stream);
+
+/* ---- Weights held in 4 bits.
+ *
+ * The serving form of a linear layer's weight (the reference multiplies the FP32 weight, src/linear.cpp:12-49):
+ *     w[n, k] = s[n, k / group] * (q[n, k] - z[n, k / group]),   q in 0..15,
+ * for N = out_features rows and K = in_features columns; `group` is 32, 64 or 128 consecutive input features of
+ * one row, the scales are float16 or bfloat16, and the zero points (whole numbers 0..15, one byte each) may be left
+ * out: z = 8.
+ *
+ * Codes are exchanged as bytes, two to a byte, the even input feature in the low half: row n starts at codes + n * ldq,
+ * ldq >= (K + 1) / 2.  Scales and zero points are N x ceil(K / group), dense.  _quantize makes them from a matrix:
+ * without zero points s = max|w| / 7 and q = round(w / s) + 8, with them the range of the group and zero is cut into
+ * 15 steps; the scale is rounded to its type first and the codes are taken with the rounded scale.  A group with a weight
+ * that is not finite gets a NaN scale.  Weights that exceed 7 (15) times the largest float16 are clipped.
+ *
+ * The products read a packed form (cf. cakeb200_pack_A: laid out once, passed to every product): _packed_bytes tells its
+ * size, _pack fills it (16-byte aligned device memory of the caller's), _dequantize writes the matrix it stands for.
+ *
+ *     _linear:     y[r, n]  = sum_k x[r, k] w[n, k] (+ bias[n]),   rows r of x at x + r * ldx
+ *     _linear_dx:  dx[r, k] = sum_n dy[r, n] w[n, k],              the gradient of _linear for its input
+ *
+ * x, bias, y, dy and dx share one type, CAKEB200_F32, _F16 or _BF16; leading dimensions are in elements; sums are FP32 and
+ * scales are applied in FP32.  The result must not overlap the operands.  `rows` may be 0.  Device pointers of the
+ * current device only; work is enqueued on `stream` and nothing else is touched, so that calls on several streams,
+ * threads or captured graphs do not disturb one another.  Results do not depend on timing. */
+typedef struct cakeb200_q4 {
+    const void* packed;
+    int out_features, in_features, group;
+    int scale_type; /* CAKEB200_F16 or CAKEB200_BF16 */
+    int has_zeros;
+} cakeb200_q4;
+size_t cakeb200_q4_packed_bytes(int out_features, int in_features, int group, int has_zeros);
+int cakeb200_q4_quantize(const void* W, long long ldw, int type, int out_features, int in_features, int group, int scale_type,
+                         void* codes, long long ldq, void* scales, void* zeros /* NULL: z = 8 */, void* stream);
+int cakeb200_q4_pack(const void* codes, long long ldq, const void* scales, const void* zeros, int out_features, int in_features,
+                     int group, int scale_type, void* packed, void* stream);
+int cakeb200_q4_dequantize(const cakeb200_q4* w, void* W, long long ldw, int type, void* stream);
+int cakeb200_q4_linear(const cakeb200_q4* w, const void* x, long long ldx, const void* bias, void* y, long long ldy, int rows,
+                       int type, void* stream);
+int cakeb200_q4_linear_dx(const cakeb200_q4* w, const void* dy, long long lddy, void* dx, long long lddx, int rows, int type,
+                          void* stream);
 
 /* C = A*B for callers that must not allocate device memory.  This entry point has
  * no counterpart in the reference; it exists for hosts of this library that are
