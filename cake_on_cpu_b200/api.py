@@ -141,6 +141,10 @@ _SIGNATURES["cakeb200_q4_pack"] = (_i, [_vp, _ll, _vp, _vp, _i, _i, _i, _i, _vp,
 _SIGNATURES["cakeb200_q4_dequantize"] = (_i, [_pq4, _vp, _ll, _i, _vp])
 _SIGNATURES["cakeb200_q4_linear"] = (_i, [_pq4, _vp, _ll, _vp, _vp, _ll, _i, _i, _vp])
 _SIGNATURES["cakeb200_q4_linear_dx"] = (_i, [_pq4, _vp, _ll, _vp, _ll, _i, _i, _vp])
+_f, _d = ctypes.c_float, ctypes.c_double
+_SIGNATURES["cakeb200_orthogonalize_workspace"] = (_sz, [_i, _i, _i, _i])
+_SIGNATURES["cakeb200_orthogonalize"] = (_i, [_vp, _ll, _ll, _vp, _ll, _ll] + [_i] * 5 + [_f] * 4 + [_vp, _sz, _vp])
+_SIGNATURES["cakeb200_muon_step"] = (_i, [_vp, _ll, _i, _vp, _ll, _i, _vp, _ll, _i, _i, _d, _d, _i, _d, _d, _i, _f, _f, _f, _f, _vp, _sz, _vp])
 
 EXPORTED_SYMBOLS = sorted(_SIGNATURES)
 
@@ -827,6 +831,96 @@ def cake_q4_linear_dx(dy, W4, out=None, stream=None):
     """dy @ W with W a ``Q4Weights`` (cakeb200_q4_linear_dx): the gradient of ``cake_q4_linear`` for its input."""
     _need_q4(W4)
     return _q4_product(True, "dy", dy, W4, W4.out_features, W4.in_features, None, out, stream)
+
+
+# --------------------------------------------------------- orthogonalised updates
+
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def _matrix_of(t, what, device=None, shape=None):
+    """Checks a CUDA matrix with contiguous rows; returns (address, leading dimension)."""
+    if not (_is_torch(t) and t.is_cuda):
+        raise TypeError("%s must be a CUDA tensor" % what)
+    if device is not None and t.device != device:
+        raise ValueError("%s is on %s, expected %s" % (what, t.device, device))
+    if shape is not None:
+        _need_shape(t, shape, what)
+    rows, cols = t.shape[-2:]
+    if rows < 1 or cols < 1:
+        raise ValueError("%s has an empty side" % what)
+    if cols > 1 and t.stride(-1) != 1:
+        raise TypeError("%s must have contiguous rows" % what)
+    ld = t.stride(-2) if rows > 1 else cols
+    if ld < cols:
+        raise TypeError("%s: its rows overlap" % what)
+    return t.data_ptr(), ld
+
+
+def _ns_workspace(rows, cols, batch, t, device):
+    """(tensor to keep until the call is enqueued, aligned address, bytes) of the products' scratch planes."""
+    import torch
+    need = lib().cakeb200_orthogonalize_workspace(rows, cols, batch, t)
+    if need == 0:
+        _check(-1)
+    buf = torch.empty(need + 1024, dtype=torch.uint8, device=device)
+    p = (buf.data_ptr() + 1023) & ~1023
+    return buf, p, need
+
+
+def cake_orthogonalize(G, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7, stream=None):
+    """The orthogonalisation of a matrix, or of every matrix of a batch, by Newton-Schulz products (cakeb200_orthogonalize),
+    enqueued on the current stream: X = G / (|G|_F + eps), then ``steps`` times X <- a X + b (X X^T) X + c (X X^T)^2 X.
+
+    G: CUDA tensor (rows, cols) or (batch, rows, cols), float32 or bfloat16, rows contiguous.  ``out`` may be G."""
+    import torch
+    if not (_is_torch(G) and G.is_cuda):
+        raise TypeError("G must be a CUDA tensor")
+    if G.dim() not in (2, 3):
+        raise ValueError("G must be a matrix or a batch of matrices")
+    t = _type_code(G.dtype, "G", (F32, BF16))
+    a, b, c = (float(v) for v in coeffs)
+    batch = G.shape[0] if G.dim() == 3 else 1
+    rows, cols = G.shape[-2:]
+    p, ld = _matrix_of(G, "G")
+    if out is not None:
+        po, ldo = _matrix_of(out, "out", G.device, G.shape)
+        if out.dtype != G.dtype:
+            raise TypeError("out is %s, expected %s" % (out.dtype, G.dtype))
+    with _on_device(G.device, stream) as s:
+        if out is None:
+            out = torch.empty(G.shape, dtype=G.dtype, device=G.device)
+            po, ldo = out.data_ptr(), cols
+        if batch == 0:
+            return out
+        stride = lambda m: m.stride(0) if m.dim() == 3 else 0
+        buf, ws, n = _ns_workspace(rows, cols, batch, t, G.device)
+        _check(lib().cakeb200_orthogonalize(p, ld, stride(G), po, ldo, stride(out), rows, cols, batch, t, int(steps), a, b, c, float(eps), ws, n, s))
+    return out
+
+
+def cake_muon_step(W, G, M, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5, coeffs=NS_COEFFS, eps=1e-7, stream=None):
+    """One step of an optimiser with orthogonalised updates on the matrix W, in place (cakeb200_muon_step):
+    M <- momentum M + (1 - momentum) G;  U = momentum M + (1 - momentum) G, or M without ``nesterov``;
+    W <- (1 - lr weight_decay) W - lr scale O(U).  ``scale`` defaults to sqrt(max(1, rows / cols)).
+
+    W and G: float32 or bfloat16 CUDA matrices with contiguous rows, M: the same in float32.  Returns W."""
+    if not (_is_torch(W) and W.is_cuda):
+        raise TypeError("W must be a CUDA tensor")
+    if W.dim() != 2:
+        raise ValueError("W must be a matrix")
+    tw, tg = _type_code(W.dtype, "W", (F32, BF16)), _type_code(G.dtype if _is_torch(G) else None, "G", (F32, BF16))
+    _type_code(M.dtype if _is_torch(M) else None, "M", (F32,))
+    rows, cols = W.shape
+    (pw, ldw), (pg, ldg), (pm, ldm) = _matrix_of(W, "W"), _matrix_of(G, "G", W.device, W.shape), _matrix_of(M, "M", W.device, W.shape)
+    a, b, c = (float(v) for v in coeffs)
+    if scale is None:
+        scale = max(1.0, rows / cols) ** 0.5
+    with _on_device(W.device, stream) as s:
+        buf, ws, n = _ns_workspace(rows, cols, 1, tw, W.device)
+        _check(lib().cakeb200_muon_step(pw, ldw, tw, pg, ldg, tg, pm, ldm, rows, cols, float(lr), float(momentum), int(bool(nesterov)),
+                                        float(weight_decay), float(scale), int(steps), a, b, c, float(eps), ws, n, s))
+    return W
 
 
 def tune(A, B, C=None, sch=NA, trials=24, stream=None):

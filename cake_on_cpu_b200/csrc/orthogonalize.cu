@@ -1,0 +1,527 @@
+// Orthogonalising an update by Newton-Schulz products, alone and inside an optimiser's step.
+//
+//     X_0 = G / (|G|_F + eps);    P = X X^T;    Q = a I + b P + c P P;    X <- Q X;    `steps` times.
+//
+// Every singular value s of X goes to a s + b s^3 + c s^5, the singular vectors stay: with the usual coefficients values
+// anywhere in (0, 1] end up around 1.  X is taken m x n with m <= n (the transpose of a tall G), so that P is the smaller
+// square.  P and Q are symmetric: only the tiles on and below the diagonal are computed, 2 m^2 n + m^3 multiply-adds
+// per step instead of 2 m^2 n + 2 m^3 and an elementwise pass.  The polynomial lives in the second product's epilogue, which
+// adds b P and a I to c P P in FP32.
+//
+// All matrices between the first and the last kernel are bf16 planes (plane_gemm.cuh): three per value for an FP32 result,
+// two for a BF16 one.  Small singular values grow by a factor a = 3.4 per step, 480 in five, and so does the rounding noise
+// of X beside them: single bf16 planes (2^-9) would leave several per cent of noise in the result, two (2^-17) leave a fraction
+// of a BF16 step.  X and its transpose are both kept, as both products want their operands K-major: the epilogue that computes
+// a block writes it both ways.
+#include "plane_gemm.cuh"
+
+namespace cakeb200 {
+
+using plane::Planes;
+using plane::TileAt;
+
+int plane::encode_planes(CUtensorMap* map, const Planes& p, int terms) {
+    const unsigned long long dims[3] = {(unsigned long long) p.cols, (unsigned long long) p.rows, (unsigned long long) terms * p.batches};
+    const unsigned long long strides[2] = {(unsigned long long) p.ld * 2, (unsigned long long) p.ld * 2 * p.rows};
+    const unsigned box[3] = {plane::BK, 128, 1};
+    return encode_tiled_bf16(map, p.base, 3, dims, strides, box, true);
+}
+
+namespace {
+
+constexpr int NORM_BLOCKS = 64;  // partial sums of squares per matrix
+
+// eight consecutive elements; `vec`: all eight exist and the address is 16-byte aligned
+__device__ __forceinline__ void get8(const float* p, int n, bool vec, float* v) {
+    if (vec && n >= 8) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = e < n ? p[e] : 0.f;
+    }
+}
+__device__ __forceinline__ void get8(const __nv_bfloat16* p, int n, bool vec, float* v) {
+    if (vec && n >= 8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[2 * e] = __uint_as_float(u[e] << 16);
+            v[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = e < n ? __bfloat162float(p[e]) : 0.f;
+    }
+}
+__device__ __forceinline__ void put8(float* p, int n, bool vec, const float* v) {
+    if (vec && n >= 8) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < n) p[e] = v[e];
+    }
+}
+__device__ __forceinline__ void put8(__nv_bfloat16* p, int n, bool vec, const float* v) {
+    if (vec && n >= 8) {
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+            u[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < n) p[e] = __float2bfloat16_rn(v[e]);
+    }
+}
+
+// ------------------------------------------------------------------ the input: norm, momentum, planes
+
+// A matrix (or a batch) in the caller's memory; vec: rows start on 16-byte boundaries.
+template <typename T>
+struct Matrix {
+    T* base;
+    long long ld, stride;
+    int vec;
+};
+
+// What is orthogonalised: G itself, or the update U made of G and the momentum M.
+template <typename T>
+struct Source {
+    Matrix<const T> g;
+    float* m;          // nullptr: plain G
+    long long ldm;
+    int vec_m;
+    float mu, rest;    // momentum and 1 - momentum, each rounded once
+    int nesterov;
+    int rows, cols;
+};
+
+// Eight values of row r from column c on.  UPDATE: M <- mu M + (1 - mu) G on the way (else M has it already).
+template <typename T, bool UPDATE>
+__device__ __forceinline__ void source8(const Source<T>& s, int batch, int r, int c, float* v) {
+    const int n = s.cols - c;
+    get8(s.g.base + batch * s.g.stride + r * s.g.ld + c, n, s.g.vec, v);
+    if (s.m == nullptr) return;
+    float m[8];
+    float* at = s.m + r * s.ldm + c;
+    get8(at, n, s.vec_m, m);
+    if (UPDATE) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) m[e] = s.mu * m[e] + s.rest * v[e];
+        put8(at, n, s.vec_m, m);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = s.nesterov ? s.mu * m[e] + s.rest * v[e] : m[e];
+}
+
+// partial[batch][block] = sum of squares, in 64 bits: an FP32 sum of squares overflows and underflows long before G does.
+template <typename T>
+__global__ void __launch_bounds__(256)
+norm_kernel(const Source<T> s, double* __restrict__ partial) {
+    const int batch = blockIdx.y, segments = (s.cols + 7) / 8;
+    const long long total = (long long) s.rows * segments;
+    double sum = 0;
+    for (long long i = (long long) blockIdx.x * 256 + threadIdx.x; i < total; i += (long long) gridDim.x * 256) {
+        const int r = (int) (i / segments), c = (int) (i - (long long) r * segments) * 8;
+        float v[8];
+        source8<T, true>(s, batch, r, c, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (c + e < s.cols) sum += (double) v[e] * v[e];
+    }
+    __shared__ double warps[8];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; w++) sum += warps[w];
+        partial[batch * NORM_BLOCKS + blockIdx.x] = sum;
+    }
+}
+
+// Planes of X_0 and of its transpose; a warp does one 32 x 32 block.
+template <typename T, int TERMS>
+__global__ void __launch_bounds__(256)
+split_kernel(const Source<T> s, const double* __restrict__ partial, int partials, float eps, const Planes direct, const Planes transposed) {
+    __shared__ float patches[8][32 * plane::PATCH_LD];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = blockIdx.z;
+    const int row0 = blockIdx.y * 32, col0 = (blockIdx.x * 8 + warp) * 32;
+    if (col0 >= s.cols) return;
+    double sum = 0;
+    for (int i = lane; i < partials; i += 32) sum += partial[batch * NORM_BLOCKS + i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const double inverse = 1.0 / (sqrt(sum) + (double) eps);
+    float* patch = patches[warp];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int rl = 8 * q + (lane >> 2), cl = 8 * (lane & 3), r = row0 + rl, c = col0 + cl;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = 0.f;
+        if (r < s.rows && c < s.cols) {
+            source8<T, false>(s, batch, r, c, v);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = (float) ((double) v[e] * inverse);
+            if (s.cols - c < 8) {  // the padding columns stay zero whatever the norm (0 times an infinite inverse)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (c + e >= s.cols) v[e] = 0.f;
+            }
+            plane::store8<TERMS>(direct, batch, r, c, v);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) patch[rl * plane::PATCH_LD + cl + e] = v[e];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int r = col0 + 8 * q + (lane >> 2), c = row0 + 8 * (lane & 3);
+        float v[8];
+        plane::read8<true>(patch, lane, q, v);
+        if (r < s.cols && c < s.rows) plane::store8<TERMS>(transposed, batch, r, c, v);
+    }
+}
+
+// ------------------------------------------------------------------ epilogues of the products
+
+template <int T>
+__device__ __forceinline__ void store_block(const Planes& p, int batch, int row, int col, const float* patch, int lane, bool transposed) {
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) {
+        const int r = row + 8 * q + (lane >> 2), c = col + 8 * (lane & 3);
+        float v[8];
+        if (transposed) plane::read8<true>(patch, lane, q, v);
+        else plane::read8<false>(patch, lane, q, v);
+        if (r < p.rows && c < p.cols) plane::store8<T>(p, batch, r, c, v);
+    }
+}
+
+// P = X X^T: planes of the block and of its mirror image
+template <int T>
+struct GramEpilogue {
+    struct Args {
+        Planes out;
+    };
+    static __device__ __forceinline__ void block(const Args& a, const TileAt& at, float* patch, int lane) {
+        store_block<T>(a.out, at.batch, at.row, at.col, patch, lane, false);
+        if (at.mirror) store_block<T>(a.out, at.batch, at.col, at.row, patch, lane, true);
+    }
+};
+
+// Q = a I + b P + c (P P)
+template <int T>
+struct PolynomialEpilogue {
+    struct Args {
+        Planes p, out;
+        float a, b, c;
+    };
+    static __device__ __forceinline__ void block(const Args& g, const TileAt& at, float* patch, int lane) {
+#pragma unroll 1
+        for (int q = 0; q < 4; q++) {
+            const int r = at.row + 8 * q + (lane >> 2), c = at.col + 8 * (lane & 3);
+            if (r >= g.out.rows || c >= g.out.cols) continue;
+            float v[8], old[8];
+            plane::read8<false>(patch, lane, q, v);
+            plane::load8<T>(g.p, at.batch, r, c, old);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[e] = g.c * v[e] + g.b * old[e] + (r == c + e ? g.a : 0.f);
+                patch[(8 * q + (lane >> 2)) * plane::PATCH_LD + 8 * (lane & 3) + e] = v[e];
+            }
+            plane::store8<T>(g.out, at.batch, r, c, v);
+        }
+        if (!at.mirror) return;
+        __syncwarp();
+        store_block<T>(g.out, at.batch, at.col, at.row, patch, lane, true);
+    }
+};
+
+// X = Q X and its transpose
+template <int T>
+struct ApplyEpilogue {
+    struct Args {
+        Planes x, xt;
+    };
+    static __device__ __forceinline__ void block(const Args& a, const TileAt& at, float* patch, int lane) {
+        store_block<T>(a.x, at.batch, at.row, at.col, patch, lane, false);
+        store_block<T>(a.xt, at.batch, at.col, at.row, patch, lane, true);
+    }
+};
+
+// the last X, rounded once to the result's type
+template <typename T>
+struct ResultEpilogue {
+    struct Args {
+        Matrix<T> out;
+        int rows, cols;
+    };
+    static __device__ __forceinline__ void block(const Args& a, const TileAt& at, float* patch, int lane) {
+#pragma unroll 1
+        for (int q = 0; q < 4; q++) {
+            const int r = at.row + 8 * q + (lane >> 2), c = at.col + 8 * (lane & 3);
+            if (r >= a.rows || c >= a.cols) continue;
+            float v[8];
+            plane::read8<false>(patch, lane, q, v);
+            put8(a.out.base + at.batch * a.out.stride + r * a.out.ld + c, a.cols - c, a.out.vec, v);
+        }
+    }
+};
+
+// W <- keep W - step X
+template <typename T>
+struct StepEpilogue {
+    struct Args {
+        Matrix<T> w;
+        int rows, cols;
+        float keep, step;
+    };
+    static __device__ __forceinline__ void block(const Args& a, const TileAt& at, float* patch, int lane) {
+#pragma unroll 1
+        for (int q = 0; q < 4; q++) {
+            const int r = at.row + 8 * q + (lane >> 2), c = at.col + 8 * (lane & 3);
+            if (r >= a.rows || c >= a.cols) continue;
+            float v[8], w[8];
+            T* p = a.w.base + r * a.w.ld + c;
+            plane::read8<false>(patch, lane, q, v);
+            get8(p, a.cols - c, a.w.vec, w);
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = a.keep * w[e] - a.step * v[e];
+            put8(p, a.cols - c, a.w.vec, w);
+        }
+    }
+};
+
+// ------------------------------------------------------------------ host side
+
+int bad(const char* who, const char* what) {
+    set_error("%s: %s", who, what);
+    return CAKEB200_ERR_ARG;
+}
+
+constexpr int MAX_SIDE = 1 << 20, MAX_BATCH = 65535, MAX_STEPS = 64;
+
+struct Layout {
+    Planes x, xt[2], p, q;
+    double* partial;
+    size_t bytes;
+};
+
+// X keeps one set of planes (nothing reads it while the last product of a step writes it), its transpose two.
+Layout lay_out(char* base, int terms, int batch, int m, int n) {
+    Layout l;
+    size_t at = 0;
+    auto planes = [&](int rows, int cols) {
+        Planes p;
+        p.base = (__nv_bfloat16*) (base + at);
+        p.rows = rows; p.cols = cols; p.ld = plane::padded(cols); p.batches = batch;
+        at += plane::plane_bytes(terms, batch, rows, cols);
+        return p;
+    };
+    l.x = planes(m, n);
+    l.xt[0] = planes(n, m);
+    l.xt[1] = planes(n, m);
+    l.p = planes(m, m);
+    l.q = planes(m, m);
+    l.partial = (double*) (base + at);
+    at += ((size_t) batch * NORM_BLOCKS * 8 + 1023) / 1024 * 1024;
+    l.bytes = at;
+    return l;
+}
+
+int terms_for(int type) { return type == CAKEB200_F32 ? 3 : 2; }
+
+int check_shape(const char* who, int rows, int cols, int batch) {
+    if (rows <= 0 || cols <= 0 || batch < 0) return bad(who, "sizes must be positive");
+    if (rows > MAX_SIDE || cols > MAX_SIDE || batch > MAX_BATCH) {
+        set_error("%s: more than 2^20 rows or columns, or 65535 matrices", who);
+        return CAKEB200_ERR_TOO_LARGE;
+    }
+    return CAKEB200_OK;
+}
+
+struct Coefficients {
+    int steps;
+    float a, b, c, eps;
+};
+
+int check_coefficients(const char* who, const Coefficients& k) {
+    if (k.steps < 1 || k.steps > MAX_STEPS) return bad(who, "1 to 64 steps");
+    if (!(k.eps >= 0.f)) return bad(who, "eps is a number that is not negative");
+    return CAKEB200_OK;
+}
+
+template <typename T>
+Matrix<T> matrix(T* base, long long ld, long long stride, int rows, int batch) {
+    Matrix<T> m;
+    m.base = base;
+    m.ld = ld;
+    m.stride = stride;
+    m.vec = (uintptr_t) base % 16 == 0 && (rows == 1 || ld * (long long) sizeof(T) % 16 == 0) && (batch == 1 || stride * (long long) sizeof(T) % 16 == 0);
+    return m;
+}
+
+// From the source to the last X, which goes through `Last`.
+template <typename T, int TERMS, class Last>
+int run(const Source<T>& src, int batch, const Coefficients& k, void* workspace, const typename Last::Args& last, DeviceState* st, cudaStream_t s) {
+    const int rows = src.rows, cols = src.cols;
+    const bool tall = rows > cols;
+    const int m = tall ? cols : rows, n = tall ? rows : cols;
+    Layout l = lay_out((char*) workspace, TERMS, batch, m, n);
+    CUtensorMap map_x, map_xt[2], map_p, map_q;
+    int rc;
+    if ((rc = plane::encode_planes(&map_x, l.x, TERMS)) || (rc = plane::encode_planes(&map_xt[0], l.xt[0], TERMS)) ||
+        (rc = plane::encode_planes(&map_xt[1], l.xt[1], TERMS)) || (rc = plane::encode_planes(&map_p, l.p, TERMS)) ||
+        (rc = plane::encode_planes(&map_q, l.q, TERMS)))
+        return rc;
+    const long long work = (long long) rows * ((cols + 7) / 8);
+    const int partials = (int) std::min<long long>(NORM_BLOCKS, (work + 255) / 256);
+    norm_kernel<T><<<dim3((unsigned) partials, (unsigned) batch), 256, 0, s>>>(src, l.partial);
+    CAKE_CUDA_OK(cudaGetLastError());
+    const dim3 grid((unsigned) ((cols + 255) / 256), (unsigned) ((rows + 31) / 32), (unsigned) batch);
+    split_kernel<T, TERMS><<<grid, 256, 0, s>>>(src, l.partial, partials, k.eps, tall ? l.xt[0] : l.x, tall ? l.x : l.xt[0]);
+    CAKE_CUDA_OK(cudaGetLastError());
+    plane::Problem p = {};
+    p.batch = batch;
+    p.chunk = TERMS == 3 ? 4 : 16;  // 256 of K for an FP32 result, 1024 for a BF16 one
+    p.status_word = st->status_word;
+    for (int i = 0; i < k.steps; i++) {
+        p.rows = p.cols = m;
+        p.symmetric = 1;
+        p.K = n;
+        typename GramEpilogue<TERMS>::Args gram = {l.p};
+        if ((rc = plane::launch<TERMS, TERMS, GramEpilogue<TERMS>>(map_x, map_x, p, gram, st->sm_count, s))) return rc;
+        p.K = m;
+        typename PolynomialEpilogue<TERMS>::Args poly = {l.p, l.q, k.a, k.b, k.c};
+        if ((rc = plane::launch<TERMS, TERMS, PolynomialEpilogue<TERMS>>(map_p, map_p, p, poly, st->sm_count, s))) return rc;
+        p.symmetric = 0;
+        if (i + 1 < k.steps) {
+            p.cols = n;
+            typename ApplyEpilogue<TERMS>::Args apply = {l.x, l.xt[(i + 1) & 1]};
+            if ((rc = plane::launch<TERMS, TERMS, ApplyEpilogue<TERMS>>(map_q, map_xt[i & 1], p, apply, st->sm_count, s))) return rc;
+        } else {
+            // the result as the caller stores it: Q X, or its transpose X^T Q (Q is symmetric)
+            p.rows = rows;
+            p.cols = cols;
+            if ((rc = plane::launch<TERMS, TERMS, Last>(tall ? map_xt[i & 1] : map_q, tall ? map_q : map_xt[i & 1], p, last, st->sm_count, s))) return rc;
+        }
+    }
+    thread_stats()->launches = 2 + 3 * k.steps;
+    return CAKEB200_OK;
+}
+
+bool known(int type) { return type == CAKEB200_F32 || type == CAKEB200_BF16; }
+
+template <typename T, int TERMS>
+int orthogonalize(const void* G, long long ldg, long long stride_g, void* out, long long ldo, long long stride_o, int rows, int cols, int batch,
+                  const Coefficients& k, void* workspace, DeviceState* st, cudaStream_t s) {
+    Source<T> src = {};
+    src.g = matrix((const T*) G, ldg, stride_g, rows, batch);
+    src.rows = rows;
+    src.cols = cols;
+    typename ResultEpilogue<T>::Args last = {matrix((T*) out, ldo, stride_o, rows, batch), rows, cols};
+    return run<T, TERMS, ResultEpilogue<T>>(src, batch, k, workspace, last, st, s);
+}
+
+template <typename TW, int TERMS, typename TG>
+int muon(void* W, long long ldw, const void* G, long long ldg, float* M, long long ldm, int rows, int cols, double lr, double mu, int nesterov,
+         double weight_decay, double scale, const Coefficients& k, void* workspace, DeviceState* st, cudaStream_t s) {
+    Source<TG> src = {};
+    src.g = matrix((const TG*) G, ldg, 0, rows, 1);
+    src.m = M;
+    src.ldm = ldm;
+    src.vec_m = matrix(M, ldm, 0, rows, 1).vec;
+    src.mu = (float) mu;
+    src.rest = (float) (1.0 - mu);
+    src.nesterov = nesterov;
+    src.rows = rows;
+    src.cols = cols;
+    typename StepEpilogue<TW>::Args last = {matrix((TW*) W, ldw, 0, rows, 1), rows, cols, (float) (1.0 - lr * weight_decay), (float) (lr * scale)};
+    return run<TG, TERMS, StepEpilogue<TW>>(src, 1, k, workspace, last, st, s);
+}
+
+}  // namespace
+}  // namespace cakeb200
+
+using namespace cakeb200;
+
+extern "C" {
+
+size_t cakeb200_orthogonalize_workspace(int rows, int cols, int batch, int type) {
+    if (check_shape("cakeb200_orthogonalize_workspace", rows, cols, batch)) return 0;
+    if (!known(type)) {
+        bad("cakeb200_orthogonalize_workspace", "the type is float32 or bfloat16");
+        return 0;
+    }
+    return lay_out(nullptr, terms_for(type), batch, std::min(rows, cols), std::max(rows, cols)).bytes;
+}
+
+int cakeb200_orthogonalize(const void* G, long long ldg, long long stride_g, void* out, long long ldo, long long stride_o, int rows, int cols,
+                           int batch, int type, int steps, float a, float b, float c, float eps, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+    static const char* who = "cakeb200_orthogonalize";
+    *thread_stats() = cakeb200_stats();
+    const Coefficients k = {steps, a, b, c, eps};
+    int rc = check_shape(who, rows, cols, batch);
+    if (rc) return rc;
+    if (!known(type)) return bad(who, "the type is float32 or bfloat16");
+    if ((rc = check_coefficients(who, k))) return rc;
+    if (batch == 0) return CAKEB200_OK;
+    if (!G || !out || !workspace) return bad(who, "null pointer");
+    if (ldg < cols || ldo < cols) return bad(who, "a leading dimension is smaller than its row");
+    if (batch > 1 && stride_o < (long long) (rows - 1) * ldo + cols) return bad(who, "the matrices of the result overlap");
+    if ((uintptr_t) workspace % 1024) return bad(who, "the workspace starts on a 1024-byte boundary");
+    if (workspace_bytes < cakeb200_orthogonalize_workspace(rows, cols, batch, type)) return bad(who, "the workspace is too small");
+    const size_t size = type == CAKEB200_F32 ? 4 : 2;
+    if ((uintptr_t) G % size || (uintptr_t) out % size) return bad(who, "a pointer is not aligned to its type");
+    DeviceState* st = device_state();
+    if (!st) return CAKEB200_ERR_NO_DEVICE;
+    if (!on_current_device(G) || !on_current_device(out) || !on_current_device(workspace))
+        return bad(who, "operands must be device pointers of the current device");
+    cudaStream_t s = (cudaStream_t) stream;
+    if (type == CAKEB200_F32) return orthogonalize<float, 3>(G, ldg, stride_g, out, ldo, stride_o, rows, cols, batch, k, workspace, st, s);
+    return orthogonalize<__nv_bfloat16, 2>(G, ldg, stride_g, out, ldo, stride_o, rows, cols, batch, k, workspace, st, s);
+}
+
+int cakeb200_muon_step(void* W, long long ldw, int type_w, const void* G, long long ldg, int type_g, float* M, long long ldm, int rows, int cols,
+                       double lr, double momentum, int nesterov, double weight_decay, double scale, int steps, float a, float b, float c, float eps,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+    static const char* who = "cakeb200_muon_step";
+    *thread_stats() = cakeb200_stats();
+    const Coefficients k = {steps, a, b, c, eps};
+    int rc = check_shape(who, rows, cols, 1);
+    if (rc) return rc;
+    if (!known(type_w) || !known(type_g)) return bad(who, "the types are float32 or bfloat16");
+    if ((rc = check_coefficients(who, k))) return rc;
+    if (!W || !G || !M || !workspace) return bad(who, "null pointer");
+    if (ldw < cols || ldg < cols || ldm < cols) return bad(who, "a leading dimension is smaller than its row");
+    if ((uintptr_t) workspace % 1024) return bad(who, "the workspace starts on a 1024-byte boundary");
+    if (workspace_bytes < cakeb200_orthogonalize_workspace(rows, cols, 1, type_w)) return bad(who, "the workspace is too small");
+    if ((uintptr_t) W % (type_w == CAKEB200_F32 ? 4 : 2) || (uintptr_t) G % (type_g == CAKEB200_F32 ? 4 : 2) || (uintptr_t) M % 4)
+        return bad(who, "a pointer is not aligned to its type");
+    DeviceState* st = device_state();
+    if (!st) return CAKEB200_ERR_NO_DEVICE;
+    if (!on_current_device(W) || !on_current_device(G) || !on_current_device(M) || !on_current_device(workspace))
+        return bad(who, "operands must be device pointers of the current device");
+    cudaStream_t s = (cudaStream_t) stream;
+    nesterov = nesterov ? 1 : 0;
+#define CAKE_MUON(TW, TERMS, TG) \
+    return muon<TW, TERMS, TG>(W, ldw, G, ldg, M, ldm, rows, cols, lr, momentum, nesterov, weight_decay, scale, k, workspace, st, s)
+    if (type_w == CAKEB200_F32) {
+        if (type_g == CAKEB200_F32) CAKE_MUON(float, 3, float);
+        CAKE_MUON(float, 3, __nv_bfloat16);
+    }
+    if (type_g == CAKEB200_F32) CAKE_MUON(__nv_bfloat16, 2, float);
+    CAKE_MUON(__nv_bfloat16, 2, __nv_bfloat16);
+#undef CAKE_MUON
+}
+
+}  // extern "C"

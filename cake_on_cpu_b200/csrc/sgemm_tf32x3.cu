@@ -938,8 +938,8 @@ encode_fn_t encode_fn() {
 
 }  // namespace
 
-int encode_tiled_f32(CUtensorMap* map, const float* base, int rank, const unsigned long long* dims,
-                     const unsigned long long* strides_bytes, const unsigned* box, bool swizzle128) {
+static int encode_tiled(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const unsigned long long* dims,
+                        const unsigned long long* strides_bytes, const unsigned* box, bool swizzle128) {
     encode_fn_t enc = encode_fn();
     if (!enc) {
         set_error("cuTensorMapEncodeTiled is not available from the driver");
@@ -949,7 +949,7 @@ int encode_tiled_f32(CUtensorMap* map, const float* base, int rank, const unsign
     cuuint32_t b[5], estr[5] = {1, 1, 1, 1, 1};
     for (int i = 0; i < rank; i++) { d[i] = dims[i]; b[i] = box[i]; }
     for (int i = 0; i + 1 < rank; i++) st[i] = strides_bytes[i];
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, (cuuint32_t) rank, (void*) base, d, st, b, estr,
+    CUresult r = enc(map, type, (cuuint32_t) rank, (void*) base, d, st, b, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
@@ -957,6 +957,16 @@ int encode_tiled_f32(CUtensorMap* map, const float* base, int rank, const unsign
         return CAKEB200_ERR_CUDA;
     }
     return CAKEB200_OK;
+}
+
+int encode_tiled_f32(CUtensorMap* map, const float* base, int rank, const unsigned long long* dims,
+                     const unsigned long long* strides_bytes, const unsigned* box, bool swizzle128) {
+    return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rank, dims, strides_bytes, box, swizzle128);
+}
+
+int encode_tiled_bf16(CUtensorMap* map, const void* base, int rank, const unsigned long long* dims,
+                      const unsigned long long* strides_bytes, const unsigned* box, bool swizzle128) {
+    return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rank, dims, strides_bytes, box, swizzle128);
 }
 
 namespace {

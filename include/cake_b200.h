@@ -147,7 +147,8 @@ int cakeb200_sgemm_after(const float* A, const float* B, float* C, int M, int N,
  *               (tcgen05 cta_group::2) wherever the product has more than 128 rows, 2 = always one
  *               CTA per 128-row tile; rule: pairs for 256-wide tiles, unless padding M to a multiple
  *               of 256 instead of 128 adds more than 7 % of rows.  Both forms give the same bits when no tile is
- *               cut along K ("k_pieces" 1).
+ *               cut along K ("k_pieces" 1).  The products inside cakeb200_orthogonalize and cakeb200_muon_step follow it
+ *               too (1 = always pairs; rule: pairs when they need fewer rounds of tiles).
  * They take the place of the block sizes a caller of the reference forces with mcu / kcu / ncu
  * (reference include/cake.h:12-14, src/block_sizing.cpp:363-368) and of update_mr_nr
  * (src/block_sizing.cpp:78-83): on a GPU the blocks a caller may pin are the tile, the walk and
@@ -444,6 +445,38 @@ int cakeb200_q4_linear(const cakeb200_q4* w, const void* x, long long ldx, const
                        int type, void* stream);
 int cakeb200_q4_linear_dx(const cakeb200_q4* w, const void* dy, long long lddy, void* dx, long long lddx, int rows, int type,
                           void* stream);
+
+/* ---- Orthogonalised updates.
+ *
+ * The training form of a linear layer's weight: instead of the gradient the reference's optimisers step along
+ * (python/cake.py computes it, src/linear.cpp:76-84), its orthogonalisation by Newton-Schulz products,
+ *     X = G / (|G|_F + eps);   `steps` times   X <- a X + b (X X^T) X + c (X X^T)^2 X,
+ * taken on the transpose when G has more rows than columns.  With a = 3.4445, b = -4.7750, c = 2.0315 and five steps the
+ * singular values of X end up near 1 whatever those of G were.
+ *
+ * _orthogonalize works on `batch` matrices `stride` elements apart, each rows x cols with leading dimension ld (elements).
+ * G and out have one type, CAKEB200_F32 or CAKEB200_BF16; out may be G itself.  FP32 matrices are multiplied with operands
+ * of 24 bits, BF16 ones with operands of 16, all sums in FP32; the result is rounded once.  A G that is zero gives zero; one
+ * that is not finite gives NaN.
+ *
+ * _muon_step is one optimiser step on one matrix, in place:
+ *     M <- momentum M + (1 - momentum) G
+ *     U  = momentum M + (1 - momentum) G  (nesterov != 0)  or  M
+ *     W <- (1 - lr weight_decay) W - lr scale O(U),    O as above.
+ * W and G are CAKEB200_F32 or CAKEB200_BF16 each, M is FP32; operands of 24 bits when W is FP32.
+ *
+ * `workspace` is device memory of the caller's, 1024-byte aligned and at least _workspace(rows, cols, batch, type of the
+ * result) bytes (1 for the step's batch); its content does not matter before and after the call, but calls that may overlap on the
+ * GPU, captured graphs among them, need one each.  Device pointers of the current device only; work is enqueued on `stream`.  1 to
+ * 64 steps, up to 2^20 rows and columns and 65535 matrices.  Waits inside the kernels are bounded; one that gave up shows in
+ * the status of the next blocking product (cakeb200_sgemm). */
+size_t cakeb200_orthogonalize_workspace(int rows, int cols, int batch, int type);
+int cakeb200_orthogonalize(const void* G, long long ldg, long long stride_g, void* out, long long ldo, long long stride_o, int rows,
+                           int cols, int batch, int type, int steps, float a, float b, float c, float eps, void* workspace,
+                           size_t workspace_bytes, void* stream);
+int cakeb200_muon_step(void* W, long long ldw, int type_w, const void* G, long long ldg, int type_g, float* M, long long ldm, int rows,
+                       int cols, double lr, double momentum, int nesterov, double weight_decay, double scale, int steps, float a, float b,
+                       float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
 
 /* C = A*B for callers that must not allocate device memory.  This entry point has
  * no counterpart in the reference; it exists for hosts of this library that are

@@ -72,3 +72,51 @@ def test_q4_without_a_device(cake):
         pytest.skip("a GPU is present")
     w, p = _q4(), ctypes.c_void_p(0x20000)
     assert cake.lib().cakeb200_q4_linear(ctypes.byref(w), p, 64, None, p, 32, 1, 0, None) == ERR_NO_DEVICE
+
+
+def test_orthogonalize_refusals(cake):
+    L, p = cake.lib(), ctypes.c_void_p(0x100000)
+    ws = L.cakeb200_orthogonalize_workspace(8, 12, 2, 0)
+    # X (8 x 12, rows padded to 16), twice X^T (12 x 8), P and Q (8 x 8): three planes of two matrices each; 64 partial norms each
+    up = lambda n: -(-n // 1024) * 1024
+    assert ws == up(3 * 2 * 8 * 16 * 2) + 2 * up(3 * 2 * 12 * 8 * 2) + 2 * up(3 * 2 * 8 * 8 * 2) + up(2 * 64 * 8)
+    assert L.cakeb200_orthogonalize_workspace(0, 4, 1, 0) == 0 and L.cakeb200_orthogonalize_workspace(4, 4, 1, 1) == 0
+    assert L.cakeb200_orthogonalize_workspace(2 ** 20 + 1, 4, 1, 0) == 0
+
+    def call(**k):
+        d = dict(G=p, ldg=12, sg=96, out=p, ldo=12, so=96, rows=8, cols=12, batch=2, type=0, steps=5, a=1.0, b=0.0, c=0.0, eps=0.0, w=p, n=ws)
+        d.update(k)
+        return L.cakeb200_orthogonalize(*d.values(), None)
+
+    for change, word in [(dict(G=None), "null"), (dict(w=None), "null"), (dict(ldg=11), "leading dimension"), (dict(ldo=11), "leading dimension"),
+                         (dict(so=95), "overlap"), (dict(rows=0), "positive"), (dict(batch=-1), "positive"), (dict(type=1), "type"),
+                         (dict(steps=0), "steps"), (dict(steps=65), "steps"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
+                         (dict(w=ctypes.c_void_p(0x100200)), "1024-byte"), (dict(n=ws - 1), "too small"), (dict(G=ctypes.c_void_p(0x100002)), "aligned")]:
+        assert call(**change) == ERR_ARG and word in _last(cake), (change, _last(cake))
+    assert call(rows=2 ** 20 + 1) == ERR_TOO_LARGE
+    assert call(batch=0) == 0
+
+
+def test_muon_refusals(cake):
+    L, p = cake.lib(), ctypes.c_void_p(0x100000)
+    ws = L.cakeb200_orthogonalize_workspace(8, 12, 1, 2)
+
+    def call(**k):
+        d = dict(W=p, ldw=12, tw=2, G=p, ldg=12, tg=0, M=p, ldm=12, rows=8, cols=12, lr=0.1, mu=0.9, nesterov=1, wd=0.0, scale=1.0, steps=5, a=1.0,
+                 b=0.0, c=0.0, eps=0.0, w=p, n=ws)
+        d.update(k)
+        return L.cakeb200_muon_step(*d.values(), None)
+
+    for change, word in [(dict(W=None), "null"), (dict(M=None), "null"), (dict(tw=1), "types"), (dict(tg=3), "types"), (dict(ldm=11), "leading dimension"),
+                         (dict(n=ws - 1), "too small"), (dict(steps=0), "steps"), (dict(M=ctypes.c_void_p(0x100002)), "aligned"), (dict(cols=0), "positive")]:
+        assert call(**change) == ERR_ARG and word in _last(cake), (change, _last(cake))
+
+
+def test_orthogonalize_python_layer_takes_cuda_tensors_only(cake):
+    import numpy as np
+    import torch
+    for g in (torch.zeros((4, 4)), np.zeros((4, 4), np.float32), None):
+        with pytest.raises(TypeError):
+            cake.cake_orthogonalize(g)
+        with pytest.raises(TypeError):
+            cake.cake_muon_step(g, g, g, 0.1)
