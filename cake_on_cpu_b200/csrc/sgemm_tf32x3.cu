@@ -964,9 +964,9 @@ int encode_tiled_f32(CUtensorMap* map, const float* base, int rank, const unsign
     return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rank, dims, strides_bytes, box, swizzle128);
 }
 
-int encode_tiled_bf16(CUtensorMap* map, const void* base, int rank, const unsigned long long* dims,
-                      const unsigned long long* strides_bytes, const unsigned* box, bool swizzle128) {
-    return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rank, dims, strides_bytes, box, swizzle128);
+int encode_tiled_16(CUtensorMap* map, bool bf16, const void* base, int rank, const unsigned long long* dims,
+                    const unsigned long long* strides_bytes, const unsigned* box, bool swizzle128) {
+    return encode_tiled(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, base, rank, dims, strides_bytes, box, swizzle128);
 }
 
 namespace {

@@ -13,9 +13,9 @@ namespace cakeb200 {
 // out-of-range elements read as zero.  Implemented next to the driver entry-point lookup in sgemm_tf32x3.cu.
 int encode_tiled_f32(CUtensorMap* map, const float* base, int rank, const unsigned long long* dims,
                      const unsigned long long* strides_bytes, const unsigned* box, bool swizzle128);
-// the same for BF16 elements
-int encode_tiled_bf16(CUtensorMap* map, const void* base, int rank, const unsigned long long* dims,
-                      const unsigned long long* strides_bytes, const unsigned* box, bool swizzle128);
+// the same for BF16 or FP16 elements
+int encode_tiled_16(CUtensorMap* map, bool bf16, const void* base, int rank, const unsigned long long* dims,
+                    const unsigned long long* strides_bytes, const unsigned* box, bool swizzle128);
 
 namespace ptx {
 

@@ -80,6 +80,24 @@ def test_one_matrix(cake, shape, dtype, pair):
         cake.set_option("pair", 0)
 
 
+@pytest.mark.parametrize("form", [(1, 1), (1, 2), (1, 4), (2, 1), (2, 2), (2, 4), (2, 8)], ids=str)
+@pytest.mark.parametrize("shape", [(31, 33), (130, 700), (520, 261)], ids=str)
+def test_forms_of_the_product(cake, shape, form):
+    """Every form the products can take (pairs or single SMs, units sharing a tile), several matrices at once."""
+    import torch
+    rng = np.random.default_rng(shape[1])
+    G = np.stack([_gradient(rng, *shape, kind) for kind in ("noise", "tokens")]).astype(np.float32)
+    cake.set_option("pair", form[0])
+    cake.set_option("k_pieces", form[1])
+    try:
+        O = cake.cake_orthogonalize(torch.from_numpy(G).cuda()).double().cpu().numpy()
+    finally:
+        cake.set_option("pair", 0)
+        cake.set_option("k_pieces", 0)
+    for o, g in zip(O, G.astype(np.float64)):
+        _hold(o, _plain(g, np.float64), _plain(g, np.float32).astype(np.float64), "float32")
+
+
 @pytest.mark.parametrize("pair", [1, 2])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_many_tiles(cake, dtype, pair):
