@@ -12,8 +12,9 @@
 // MMAs per product.  Small singular values grow by a factor a = 3.4 per step, 480 in five, and so does the rounding noise
 // of X beside them: a single 16-bit plane (2^-9 or 2^-12) would leave per cents of noise in the result, pairs leave what FP32
 // products leave.  The range of FP16 is no limit: the elements of X are at most 1 (and 1.2 later), X_0 is held 2^k times
-// itself, k near log2 sqrt(m n), which puts its elements around 1 and its resolution at 2^-36 of that.  X and its transpose
-// are both kept, as both products want their operands K-major: the epilogue that computes a block writes it both ways.
+// itself, k near log2 sqrt(m n), which puts its elements around 1 and its resolution at 2^-36 of that.  Nothing is ever
+// transposed or mirrored in memory: Q X reads X, and the upper triangles of P and Q are read, down the columns of what is there
+// (an SM stores 32 bytes a clock, so bytes written are what an epilogue costs).
 #include <cmath>
 
 #include "plane_gemm.cuh"
@@ -130,15 +131,16 @@ norm_kernel(const Source<T> s, double* __restrict__ partial) {
     }
 }
 
-// Planes of `up` X_0 and of its transpose; a warp does one 32 x 32 block.
+// Planes of `up` X_0, which is the transpose of the source where that is `tall`; a warp does one 32 x 32 block.
 template <typename T>
 __global__ void __launch_bounds__(256)
-split_kernel(const Source<T> s, const double* __restrict__ partial, int partials, float eps, double up, const Planes direct, const Planes transposed) {
-    __shared__ float patches[8][32 * plane::PATCH_LD];
+split_kernel(const Source<T> s, const double* __restrict__ partial, int partials, float eps, double up, bool tall, const Planes x, unsigned* arrived) {
+    __shared__ float patches[8][plane::PATCH_FLOATS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = blockIdx.z;
     const int row0 = blockIdx.y * 32, col0 = (blockIdx.x * 8 + warp) * 32;
     if (col0 >= s.cols) return;
     plane::wait_for_previous_kernel();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && batch == 0 && threadIdx.x == 0) *arrived = 0;  // for the barriers of the chain
     double sum = 0;
     for (int i = lane; i < partials; i += 32) sum += partial[batch * NORM_BLOCKS + i];
 #pragma unroll
@@ -155,16 +157,14 @@ split_kernel(const Source<T> s, const double* __restrict__ partial, int partials
             source8<T, false>(s, batch, r, c, v);
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = (float) ((double) v[e] * inverse);
-            if (s.cols - c < 8) {  // the padding columns stay zero whatever the norm (0 times an infinite inverse)
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (c + e >= s.cols) v[e] = 0.f;
-            }
-            plane::store8<Fp16Planes, TERMS>(direct, batch, r, c, v);
+            if (!tall) plane::store8<Fp16Planes, TERMS>(x, batch, r, c, v);
         }
+        if (tall) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) patch[rl * plane::PATCH_LD + cl + e] = v[e];
+            for (int e = 0; e < 8; e++) patch[rl * plane::PATCH_LD + cl + e] = v[e];
+        }
     }
+    if (!tall) return;
     __syncwarp();
 #pragma unroll
     for (int q = 0; q < 4; q++) {
@@ -172,48 +172,11 @@ split_kernel(const Source<T> s, const double* __restrict__ partial, int partials
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = patch[(8 * (lane & 3) + e) * plane::PATCH_LD + 8 * q + (lane >> 2)];
-        if (r < s.cols && c < s.rows) plane::store8<Fp16Planes, TERMS>(transposed, batch, r, c, v);
+        if (r < s.cols && c < s.rows) plane::store8<Fp16Planes, TERMS>(x, batch, r, c, v);
     }
 }
 
-// ------------------------------------------------------------------ epilogues of the products
-
-// P = f X X^T: planes of the block and of its mirror image
-struct GramEpilogue {
-    struct Args {
-        Planes out;
-        float f;
-    };
-    static __device__ __forceinline__ void block(const Args& a, const TileAt& at, const float* v, uint32_t* patch, int lane) {
-        plane::store_block<Fp16Planes>(v, a.f, a.out, at.batch, at.row, at.col, a.out, at.col, at.row, at.mirror, patch, lane);
-    }
-};
-
-// Q = a I + b P + c (P P)
-struct PolynomialEpilogue {
-    struct Args {
-        Planes p, out;
-        float a, b, c;
-    };
-    static __device__ __forceinline__ void block(const Args& g, const TileAt& at, const float* v, uint32_t* patch, int lane) {
-        float w[32];
-        plane::load_block<Fp16Planes>(g.p, at.batch, at.row, at.col, lane, w);
-#pragma unroll
-        for (int j = 0; j < 32; j++) w[j] = g.c * v[j] + g.b * w[j] + (at.row + lane == at.col + j ? g.a : 0.f);
-        plane::store_block<Fp16Planes>(w, 1.f, g.out, at.batch, at.row, at.col, g.out, at.col, at.row, at.mirror, patch, lane);
-    }
-};
-
-// X = f Q X and its transpose
-struct ApplyEpilogue {
-    struct Args {
-        Planes x, xt;
-        float f;
-    };
-    static __device__ __forceinline__ void block(const Args& a, const TileAt& at, const float* v, uint32_t* patch, int lane) {
-        plane::store_block<Fp16Planes>(v, a.f, a.x, at.batch, at.row, at.col, a.xt, at.col, at.row, true, patch, lane);
-    }
-};
+// ------------------------------------------------------------------ what becomes of the last X
 
 __device__ __forceinline__ float get(const float* p) { return *p; }
 __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -254,6 +217,227 @@ struct StepEpilogue {
     }
 };
 
+// ------------------------------------------------------------------ the chain of products
+
+// One kernel runs all products of all steps (a launch each cost 4 us and more beside its 5 to 40 us of work, and ran its
+// epilogue from a cold instruction cache).  CTAs meet at a grid-wide barrier between products: the drain warps of a CTA
+// count it in when their stores are done, the TMA thread and the drain warps wait for the count.  The launch is
+// cooperative, so that all CTAs are resident; waits are bounded.
+//
+// A product's tiles are dealt to the units (CTAs or pairs) in turn; the tiles of the last round, fewer than there are
+// units, may be cut along K into `splits` parts of one unit each.  Parts go to memory as FP32, and after one more barrier
+// all drain warps of the machine add them up, part by part in order, 32 x 32 blocks dealt out evenly: this also spreads the
+// epilogue, which takes a CTA several microseconds on its own tile (and pays for that alone: splits may be 1).
+enum { X_ROWS, X_COLUMNS, P_SYM, Q_SYM };  // what an operand is: X, its transpose, P, Q
+struct Product {
+    int a, b;
+    int rows, cols, K;
+    int symmetric;
+    int tiles_m, tiles_n, tiles; // tiles: of one matrix
+    int whole;                   // tiles of all matrices that a unit finishes by itself, dealt out in turn
+    int cut, splits;             // how many others there are, and into how many parts each is cut (cut * splits <= units)
+};
+
+struct Chain {
+    Planes x[2], p, q;           // step s reads x[s % 2] and writes the other
+    Product gram, poly, apply, last;
+    int batch, steps, chunk;
+    float f0;                    // X_0 is held 1 / f0 times itself
+    float ka, kb, kc;
+    float* parts;                // of cut tiles: [slot][32 x 32 block][1024]
+    unsigned* arrived;           // CTAs that have come to the barriers so far
+    int* status_word;
+};
+
+struct Maps {
+    plane::OperandMaps x[2], p, q;
+};
+
+struct Item {
+    int tile, kb0, kb1, slot;    // slot < 0: whole K, straight to the epilogue
+};
+__device__ __forceinline__ bool item_at(const Product& g, int i, int unit, int units, Item& w) {
+    const int blocks = (g.K + plane::BK - 1) / plane::BK;
+    const int mine = (g.whole - unit + units - 1) / units;  // whole tiles of this unit
+    if (i < mine) {
+        w.tile = unit + i * units; w.kb0 = 0; w.kb1 = blocks; w.slot = -1;
+        return true;
+    }
+    if (i > mine || unit >= g.cut * g.splits) return false;
+    const int part = unit / g.cut;   // units next to one another read the same range of K
+    w.tile = g.whole + unit % g.cut;
+    w.kb0 = blocks * part / g.splits;
+    w.kb1 = blocks * (part + 1) / g.splits;
+    w.slot = unit;
+    return true;
+}
+__device__ __forceinline__ void place(const Product& g, int id, int& batch, int& tm, int& tn) {
+    batch = id / g.tiles;
+    const int t = id - batch * g.tiles;
+    if (g.symmetric) plane::triangle(t, tm, tn);
+    else tile_coords(t, g.tiles_m, g.tiles_n, CAKEB200_SCHED_MKN, 8, tm, tn);
+}
+
+// Stores of this thread become visible to loads of other SMs, TMA among them, once the CTA has been counted in.
+__device__ __forceinline__ void publish() { asm volatile("fence.proxy.async.global;\n\tfence.acq_rel.gpu;" ::: "memory"); }
+__device__ __forceinline__ void count_in(unsigned* counter) { asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory"); }
+// Waits until `target` CTAs have been counted in (bounded, as the waits of plane_gemm.cuh).
+__device__ __forceinline__ bool wait_for_count(const unsigned* counter, unsigned target, volatile int* abort_flag, int* status_word) {
+    const unsigned long long t0 = ptx::global_ns();
+    for (int spins = 1;; spins++) {
+        unsigned v;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
+        if ((int) (v - target) >= 0) break;
+        if ((spins & 255) == 0) {
+            if (*abort_flag) return false;
+            if ((long long) (ptx::global_ns() - t0) > ptx::WAIT_LIMIT_NS) {
+                *abort_flag = 1;
+                if (atomicCAS(status_word, 0, 1) == 0) {
+                    status_word[1] = 550;
+                    status_word[2] = (int) blockIdx.x;
+                }
+                return false;
+            }
+        }
+    }
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+    return true;
+}
+
+template <bool PAIR, class Last>
+__global__ void __launch_bounds__(plane::THREADS, 1)
+newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Chain c, const __grid_constant__ typename Last::Args last) {
+    using C = plane::Cfg<TERMS, TERMS, PAIR>;
+    extern __shared__ uint8_t smem_raw[];
+    plane::Engine<Fp16Planes, TERMS, TERMS, PAIR> e;
+    e.open(smem_raw, c.status_word);
+    const int unit = (int) blockIdx.x / (PAIR ? 2 : 1), units = (int) gridDim.x / (PAIR ? 2 : 1);
+    const int products = 3 * c.steps;
+    Item w;
+    int batch, tm, tn;
+    unsigned barriers = 0;  // passed so far
+    auto product = [&](int i) -> const Product& { return i % 3 == 0 ? c.gram : i % 3 == 1 ? c.poly : i + 1 < products ? c.apply : c.last; };
+    // P and Q have the tiles on and below the diagonal: rows of tile t turn down the columns after it
+    auto turn = [&](int which, int t) {
+        return which == X_ROWS ? plane::ALONG : which == X_COLUMNS ? plane::DOWN : (t + 1) * (C::TILE_M / plane::BK);
+    };
+    auto map_of = [&](int which, int i) { return which == P_SYM ? maps.p.m : which == Q_SYM ? maps.q.m : maps.x[i / 3 & 1].m; };
+
+    if (e.warp < 4) {
+        plane::few_registers();
+        if (e.warp == 0 && e.lane == 0) {
+            bool ok = true;
+            for (int i = 0; ok && i < products; i++) {
+                const Product& g = product(i);
+                ok = barriers == 0 || wait_for_count(c.arrived, barriers * gridDim.x, e.abort_flag, c.status_word);
+                for (int k = 0; ok && item_at(g, k, unit, units, w); k++) {
+                    place(g, w.tile, batch, tm, tn);
+                    const plane::Operand a = {map_of(g.a, i), tm * C::TILE_M + (int) e.rank * 128, turn(g.a, tm)};
+                    const plane::Operand b = {map_of(g.b, i), tn * C::BN + (int) e.rank * 128, turn(g.b, tn)};
+                    ok = e.load(a, b, batch, c.batch, w.kb0, w.kb1);
+                }
+                barriers += g.cut ? 2 : 1;
+            }
+            if (!ok) e.drain_loads();
+        } else if (e.warp == 1 && e.lane == 0 && e.rank == 0) {
+            bool ok = true;
+            for (int i = 0; ok && i < products; i++) {
+                const Product& g = product(i);
+                for (int k = 0; ok && item_at(g, k, unit, units, w); k++) {
+                    place(g, w.tile, batch, tm, tn);
+                    ok = e.multiply(turn(g.a, tm), turn(g.b, tn), w.kb0, w.kb1, c.chunk);
+                }
+            }
+        }
+    } else {
+        plane::many_registers();
+        const bool leader = threadIdx.x == 128;
+        // Once a wait has given up a warp does no more work, but comes to every barrier, so that nobody waits for it.
+        bool ok = true;
+        // all drain warps: wait until all CTAs have come to `barriers` barriers
+        auto meet = [&]() {
+            if (leader) wait_for_count(c.arrived, barriers * gridDim.x, e.abort_flag, c.status_word);
+            ptx::named_barrier_sync(1, 256);
+            ok = __all_sync(0xffffffffu, ok && *e.abort_flag == 0);
+        };
+        auto arrive = [&]() {
+            publish();
+            ptx::named_barrier_sync(1, 256);
+            if (leader) count_in(c.arrived);
+            barriers++;
+        };
+        float sum[C::COLS];
+        for (int i = 0; i < products; i++) {
+            const Product& g = product(i);
+            const int kind = i + 1 == products ? 3 : i % 3;
+            if (barriers) meet();
+            constexpr int WIDE = C::BN / 32, PER_TILE = (C::TILE_M / 32) * WIDE;  // 32 x 32 blocks of a tile, row by row
+            const Planes& out = kind == 0 ? c.p : kind == 1 ? c.q : c.x[(i / 3 + 1) & 1];
+            const float f = kind == 1 ? c.kc : i == 0 ? c.f0 * c.f0 : i == 2 ? c.f0 : 1.f;
+            // one body for all products, so that its code is fetched once
+            auto finish = [&](const TileAt& at, const float* v) {
+                if (at.row >= g.rows || at.col >= g.cols) return;
+                if (kind == 3) {
+                    Last::block(last, at, v, (uint32_t*) e.patch, e.lane);
+                    return;
+                }
+                plane::by_eights(v, (uint32_t*) e.patch, e.lane, [&](int r, int col, float* u) {
+                    r += at.row;
+                    col += at.col;
+                    if (r >= out.rows || col >= out.cols) return;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) u[j] *= f;
+                    if (kind == 1) {  // Q = a I + b P + c (P P)
+                        float old[8];
+                        plane::load8<Fp16Planes>(c.p, at.batch, r, col, old);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) u[j] += c.kb * old[j] + (r == col + j ? c.ka : 0.f);
+                    }
+                    plane::store8<Fp16Planes, TERMS>(out, at.batch, r, col, u);
+                });
+            };
+            for (int k = 0; ok && item_at(g, k, unit, units, w); k++) {
+                ok = e.collect(w.kb0, w.kb1, c.chunk, sum);
+                if (!ok) break;
+                TileAt at;
+                place(g, w.tile, at.batch, tm, tn);
+                const int row = (int) e.rank * plane::BM + e.quarter() * 32;
+                at.row = tm * C::TILE_M + row;
+                e.blocks(sum, [&](int column, const float* v) {
+                    const int b = row / 32 * WIDE + column / 32;
+                    at.col = tn * C::BN + column;
+                    if (w.slot < 0) finish(at, v);
+                    else plane::store_values(c.parts + ((long long) w.slot * PER_TILE + b) * 1024, v, e.lane);
+                });
+            }
+            if (g.cut) {
+                arrive();
+                meet();
+                const int total = g.cut * PER_TILE;
+                for (int b = (int) blockIdx.x * plane::DRAIN_WARPS + e.warp - 4; ok && b < total; b += (int) gridDim.x * plane::DRAIN_WARPS) {
+                    TileAt at;
+                    place(g, g.whole + b / PER_TILE, at.batch, tm, tn);
+                        at.row = tm * C::TILE_M + b % PER_TILE / WIDE * 32;
+                    at.col = tn * C::BN + b % WIDE * 32;
+                    if (at.row >= g.rows || at.col >= g.cols) continue;
+                    float v[32];
+                    plane::load_values(c.parts + (long long) b * 1024, v, e.lane);
+                    for (int s = 1; s < g.splits; s++) {
+                        float u[32];
+                        plane::load_values(c.parts + ((long long) s * total + b) * 1024, u, e.lane);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[j] += u[j];
+                    }
+                    finish(at, v);
+                    __syncwarp();
+                }
+            }
+            if (i + 1 < products) arrive();
+        }
+    }
+    e.close();
+}
+
 // ------------------------------------------------------------------ host side
 
 int bad(const char* who, const char* what) {
@@ -264,12 +448,68 @@ int bad(const char* who, const char* what) {
 constexpr int MAX_SIDE = 1 << 20, MAX_BATCH = 65535, MAX_STEPS = 64;
 
 struct Layout {
-    Planes x, xt[2], p, q;
+    Planes x[2], p, q;
     double* partial;
+    unsigned* arrived;
+    float* parts;
     size_t bytes;
 };
 
-// X keeps one set of planes (nothing reads it while the last product of a step writes it), its transpose two.
+// One product's share of a plan, for `units` units of one form, and its time in microseconds by a model with measured constants
+// (globaltimer stamps): 0.93 (pair) or 0.75 (single SM) per K block, 2 from a barrier to the first MMA, 0.7 to read the sums out,
+// 2.0 and 1.0 per 32 x 32 block of a warp, four of a pair's tile and two of a single one's; where parts are stored 1.0 and 0.7
+// instead, then per block dealt out 2.4 and 0.15 per part; 1.2 to be counted in and 1.0 to be let go at a barrier.
+double plan_product(Product* g, int rows, int cols, int K, int symmetric, int batch, bool pair, int units) {
+    const int side = pair ? 256 : 128, blocks = (K + plane::BK - 1) / plane::BK;
+    g->rows = rows; g->cols = cols; g->K = K; g->symmetric = symmetric;
+    g->tiles_m = (rows + side - 1) / side;
+    g->tiles_n = (cols + side - 1) / side;
+    g->tiles = symmetric ? g->tiles_m * (g->tiles_m + 1) / 2 : g->tiles_m * g->tiles_n;
+    const int total = g->tiles * batch, left = total % units, rounds = total / units;
+    const double block_time = pair ? 0.93 : 0.75, round_time = blocks * block_time + 0.7, barrier = 2.2;
+    g->whole = total; g->cut = 0; g->splits = 1;
+    double best = (rounds + (left ? 1 : 0)) * round_time + 2 + (pair ? 8 : 2) + barrier;
+    const int forced = option_get(OPT_K_PIECES);
+    if (left == 0 || forced == 1) return best;
+    for (int splits = 1; splits <= std::min(units / left, blocks); splits++) {
+        const int done = (left * (side / 32) * (side / 32) + units * (pair ? 16 : 8) - 1) / (units * (pair ? 16 : 8));
+        const double time = rounds * round_time + (blocks + splits - 1) / splits * block_time + 0.7 + 2 + (pair ? 4 : 1.4) + barrier + done * (2.4 + 0.15 * splits) + barrier;
+        if (forced ? splits <= forced : time < best) {
+            g->whole = total - left; g->cut = left; g->splits = splits;
+            best = time;
+        }
+    }
+    return best;
+}
+
+// The products of one matrix size for one form.  Returns the time of a step.
+double plan(Product* gram, Product* poly, Product* apply, Product* last, int m, int n, bool tall, int batch, bool pair, int units) {
+    gram->a = gram->b = X_ROWS;
+    poly->a = poly->b = P_SYM;
+    apply->a = Q_SYM; apply->b = X_COLUMNS;
+    // the result as the caller stores it: Q X, or its transpose X^T Q (Q is symmetric)
+    last->a = tall ? X_COLUMNS : Q_SYM; last->b = tall ? Q_SYM : X_COLUMNS;
+    const double t = plan_product(gram, m, m, n, 1, batch, pair, units) + plan_product(poly, m, m, m, 1, batch, pair, units) +
+                     plan_product(apply, m, n, m, 0, batch, pair, units);
+    plan_product(last, tall ? n : m, tall ? m : n, m, 0, batch, pair, units);
+    return t;
+}
+
+constexpr int MAX_UNITS = 160;  // single SMs; half as many pairs
+
+// Room for the parts of cut tiles, whatever the device's number of SMs and the form: at most MAX_UNITS parts of 128 x 128 or half as
+// many of 256 x 256 values, and no more than there are K blocks of all tiles.
+size_t parts_bytes(int m, int n, int batch) {
+    size_t most = 0;
+    for (int pair = 0; pair < 2; pair++) {
+        const long long side = pair ? 256 : 128, tm = (m + side - 1) / side, tn = (n + side - 1) / side;
+        const long long bm = (m + plane::BK - 1) / plane::BK, bn = (n + plane::BK - 1) / plane::BK;
+        const long long pieces = std::max<long long>(tm * (tm + 1) / 2 * std::max(bm, bn), tm * tn * bm) * batch;
+        most = std::max(most, (size_t) std::min<long long>(pieces, pair ? MAX_UNITS / 2 : MAX_UNITS) * (size_t) (side * side * 4));
+    }
+    return most;
+}
+
 Layout lay_out(char* base, int batch, int m, int n) {
     Layout l;
     size_t at = 0;
@@ -280,13 +520,16 @@ Layout lay_out(char* base, int batch, int m, int n) {
         at += plane::plane_bytes(TERMS, batch, rows, cols);
         return p;
     };
-    l.x = planes(m, n);
-    l.xt[0] = planes(n, m);
-    l.xt[1] = planes(n, m);
+    l.x[0] = planes(m, n);
+    l.x[1] = planes(m, n);
     l.p = planes(m, m);
     l.q = planes(m, m);
     l.partial = (double*) (base + at);
     at += ((size_t) batch * NORM_BLOCKS * 8 + 1023) / 1024 * 1024;
+    l.arrived = (unsigned*) (base + at);
+    at += 1024;
+    l.parts = (float*) (base + at);
+    at += parts_bytes(m, n, batch);
     l.bytes = at;
     return l;
 }
@@ -337,59 +580,116 @@ int launch_after(void (*kernel)(P...), dim3 grid, cudaStream_t s, const A&... ar
     return CAKEB200_OK;
 }
 
+// Units of one form that are resident together on the current device (asked once per device and kernel).
+template <bool PAIR, class Last>
+int resident_units(int* out) {
+    using C = plane::Cfg<TERMS, TERMS, PAIR>;
+    auto kernel = newton_schulz_kernel<PAIR, Last>;
+    static std::atomic<int> known[64];
+    int dev = 0;
+    CAKE_CUDA_OK(cudaGetDevice(&dev));
+    if (dev < 64 && (*out = known[dev].load()) > 0) return CAKEB200_OK;
+    CAKE_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    int n = 0;
+    if (PAIR) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2);
+        cfg.blockDim = dim3(plane::THREADS);
+        cfg.dynamicSmemBytes = C::SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        CAKE_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    } else {
+        int per_sm = 0, sms = 0;
+        CAKE_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, plane::THREADS, C::SMEM));
+        CAKE_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+        n = per_sm * sms;
+    }
+    n = std::min(n, PAIR ? MAX_UNITS / 2 : MAX_UNITS);
+    if (n < 1) {
+        set_error("the orthogonalisation kernel does not fit the device");
+        return CAKEB200_ERR_CUDA;
+    }
+    if (dev < 64) known[dev] = n;
+    *out = n;
+    return CAKEB200_OK;
+}
+
+template <bool PAIR, class Last>
+int launch_chain(const Maps& maps, const Chain& c, const typename Last::Args& last, int units, cudaStream_t s) {
+    using C = plane::Cfg<TERMS, TERMS, PAIR>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) (PAIR ? 2 * units : units));
+    cfg.blockDim = dim3(plane::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    CAKE_CUDA_OK(cudaLaunchKernelEx(&cfg, newton_schulz_kernel<PAIR, Last>, maps, c, last));
+    return CAKEB200_OK;
+}
+
 // From the source to the last X, which goes through `Last`.  chunk: K blocks of 64 between folds of the main accumulator.
 template <typename T, class Last>
 int run(const Source<T>& src, int batch, const Coefficients& k, int chunk, void* workspace, typename Last::Args last, DeviceState* st, cudaStream_t s) {
     const int rows = src.rows, cols = src.cols;
     const bool tall = rows > cols;
     const int m = tall ? cols : rows, n = tall ? rows : cols;
-    Layout l = lay_out((char*) workspace, batch, m, n);
-    CUtensorMap map_x, map_xt[2], map_p, map_q;
-    int rc;
-    if ((rc = plane::encode_planes<Fp16Planes>(&map_x, l.x, TERMS)) || (rc = plane::encode_planes<Fp16Planes>(&map_xt[0], l.xt[0], TERMS)) ||
-        (rc = plane::encode_planes<Fp16Planes>(&map_xt[1], l.xt[1], TERMS)) || (rc = plane::encode_planes<Fp16Planes>(&map_p, l.p, TERMS)) ||
-        (rc = plane::encode_planes<Fp16Planes>(&map_q, l.q, TERMS)))
+    const Layout l = lay_out((char*) workspace, batch, m, n);
+    int rc, units_single = 0, units_pair = 0;
+    if ((rc = resident_units<false, Last>(&units_single)) || (rc = resident_units<true, Last>(&units_pair))) return rc;
+    const long long tiles = plane::count_tiles(m, n, batch, false, 128);
+    if (tiles > (1LL << 27)) {
+        set_error("the matrices have too many tiles");
+        return CAKEB200_ERR_TOO_LARGE;
+    }
+    Maps maps;
+    if ((rc = plane::encode_planes<Fp16Planes>(maps.x[0].m, l.x[0], TERMS)) || (rc = plane::encode_planes<Fp16Planes>(maps.x[1].m, l.x[1], TERMS)) ||
+        (rc = plane::encode_planes<Fp16Planes>(maps.p.m, l.p, TERMS)) || (rc = plane::encode_planes<Fp16Planes>(maps.q.m, l.q, TERMS)))
         return rc;
+
     // X_0 is held 2^up times itself: around sqrt(m n), below the 2^16 at which its largest possible element would overflow
     const int up = std::min(15, (int) (0.5 * std::log2((double) m * n)));
-    const float down = std::ldexp(1.f, -up);
+    Chain c = {};
+    c.x[0] = l.x[0]; c.x[1] = l.x[1]; c.p = l.p; c.q = l.q;
+    c.batch = batch; c.steps = k.steps; c.chunk = chunk;
+    c.f0 = std::ldexp(1.f, -up);
+    c.ka = k.a; c.kb = k.b; c.kc = k.c;
+    c.parts = l.parts;
+    c.arrived = l.arrived;
+    c.status_word = st->status_word;
+    last.f = k.steps == 1 ? c.f0 : 1.f;
+    const int forced = option_get(OPT_PAIR);  // 1: pairs, 2: single SMs, 0: the faster by the model
+    Chain other = c;
+    const double t_single = plan(&c.gram, &c.poly, &c.apply, &c.last, m, n, tall, batch, false, units_single);
+    const double t_pair = plan(&other.gram, &other.poly, &other.apply, &other.last, m, n, tall, batch, true, units_pair);
+    const bool pair = forced ? forced == 1 : t_pair < t_single;
+    if (pair) c = other;
+    // no more units than any product gives work to
+    int units = 1;
+    for (const Product* g : {&c.gram, &c.poly, &c.apply, &c.last}) units = std::max(units, std::max(g->whole, g->cut * g->splits));
+    units = std::min(units, pair ? units_pair : units_single);
+
     const long long work = (long long) rows * ((cols + 7) / 8);
     const int partials = (int) std::max<long long>(1, std::min<long long>(NORM_BLOCKS, work / 512));
     norm_kernel<T><<<dim3((unsigned) partials, (unsigned) batch), 256, 0, s>>>(src, l.partial);
     CAKE_CUDA_OK(cudaGetLastError());
     const dim3 grid((unsigned) ((cols + 255) / 256), (unsigned) ((rows + 31) / 32), (unsigned) batch);
-    if ((rc = launch_after(split_kernel<T>, grid, s, src, l.partial, partials, k.eps, std::ldexp(1.0, up), tall ? l.xt[0] : l.x, tall ? l.x : l.xt[0])))
+    if ((rc = launch_after(split_kernel<T>, grid, s, src, l.partial, partials, k.eps, std::ldexp(1.0, up), tall, l.x[0], l.arrived)))
         return rc;
-    plane::Problem p = {};
-    p.batch = batch;
-    p.chunk = chunk;
-    p.status_word = st->status_word;
-    for (int i = 0; i < k.steps; i++) {
-        const float f = i == 0 ? down : 1.f;
-        p.rows = p.cols = m;
-        p.symmetric = 1;
-        p.K = n;
-        const GramEpilogue::Args gram = {l.p, f * f};
-        if ((rc = plane::launch<Fp16Planes, TERMS, TERMS, GramEpilogue>(map_x, map_x, p, gram, st->sm_count, s))) return rc;
-        p.K = m;
-        const PolynomialEpilogue::Args poly = {l.p, l.q, k.a, k.b, k.c};
-        if ((rc = plane::launch<Fp16Planes, TERMS, TERMS, PolynomialEpilogue>(map_p, map_p, p, poly, st->sm_count, s))) return rc;
-        p.symmetric = 0;
-        if (i + 1 < k.steps) {
-            p.cols = n;
-            const ApplyEpilogue::Args apply = {l.x, l.xt[(i + 1) & 1], f};
-            if ((rc = plane::launch<Fp16Planes, TERMS, TERMS, ApplyEpilogue>(map_q, map_xt[i & 1], p, apply, st->sm_count, s))) return rc;
-        } else {
-            // the result as the caller stores it: Q X, or its transpose X^T Q (Q is symmetric)
-            p.rows = rows;
-            p.cols = cols;
-            last.f = f;
-            if ((rc = plane::launch<Fp16Planes, TERMS, TERMS, Last>(tall ? map_xt[i & 1] : map_q, tall ? map_q : map_xt[i & 1], p, last, st->sm_count, s)))
-                return rc;
-        }
-    }
-    thread_stats()->launches = 2 + 3 * k.steps;
-    return CAKEB200_OK;
+    rc = pair ? launch_chain<true, Last>(maps, c, last, units, s) : launch_chain<false, Last>(maps, c, last, units, s);
+    if (!rc) thread_stats()->launches = 3;
+    return rc;
 }
 
 // An FP32 result is folded every 128 of K, a BF16 one every 1024.  Errors of 4096 x 4096 FP32 against 64 bits with folds every

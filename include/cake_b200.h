@@ -148,8 +148,8 @@ int cakeb200_sgemm_after(const float* A, const float* B, float* C, int M, int N,
  *               CTA per 128-row tile; rule: pairs for 256-wide tiles, unless padding M to a multiple
  *               of 256 instead of 128 adds more than 7 % of rows.  Both forms give the same bits when no tile is
  *               cut along K ("k_pieces" 1).  The products inside cakeb200_orthogonalize and cakeb200_muon_step follow it
- *               too (1 = always pairs; rule: a model of their time), and "k_pieces" forces the number of units that share
- *               a tile there (rounded down to 1, 2, 4 or, on single SMs, 8).
+ *               too (1 = always pairs; rule: a model of their time), and "k_pieces" gives the number of parts the tiles of a
+ *               last round are cut into there (1 = never cut).
  * They take the place of the block sizes a caller of the reference forces with mcu / kcu / ncu
  * (reference include/cake.h:12-14, src/block_sizing.cpp:363-368) and of update_mr_nr
  * (src/block_sizing.cpp:78-83): on a GPU the blocks a caller may pin are the tile, the walk and

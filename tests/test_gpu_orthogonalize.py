@@ -80,7 +80,7 @@ def test_one_matrix(cake, shape, dtype, pair):
         cake.set_option("pair", 0)
 
 
-@pytest.mark.parametrize("form", [(1, 1), (1, 2), (1, 4), (2, 1), (2, 2), (2, 4), (2, 8)], ids=str)
+@pytest.mark.parametrize("form", [(1, 0), (1, 1), (1, 2), (1, 4), (2, 0), (2, 1), (2, 2), (2, 5), (2, 8)], ids=str)
 @pytest.mark.parametrize("shape", [(31, 33), (130, 700), (520, 261)], ids=str)
 def test_forms_of_the_product(cake, shape, form):
     """Every form the products can take (pairs or single SMs, units sharing a tile), several matrices at once."""

@@ -77,9 +77,10 @@ def test_q4_without_a_device(cake):
 def test_orthogonalize_refusals(cake):
     L, p = cake.lib(), ctypes.c_void_p(0x100000)
     ws = L.cakeb200_orthogonalize_workspace(8, 12, 2, 0)
-    # X (8 x 12), twice X^T (12 x 8), P and Q (8 x 8), all rows padded to 16: two planes of two matrices each; 512 partial norms each
+    # X twice (8 x 12, rows padded to 16), P and Q (8 x 8): two planes of two matrices each; 512 partial norms each;
+    # a counter; and the parts of cut tiles: two products of one 256 x 256 tile and one K block each
     up = lambda n: -(-n // 1024) * 1024
-    assert ws == up(2 * 2 * 8 * 16 * 2) + 2 * up(2 * 2 * 12 * 16 * 2) + 2 * up(2 * 2 * 8 * 16 * 2) + up(2 * 512 * 8)
+    assert ws == 2 * up(2 * 2 * 8 * 16 * 2) + 2 * up(2 * 2 * 8 * 8 * 2) + up(2 * 512 * 8) + 1024 + 2 * 256 * 256 * 4
     assert L.cakeb200_orthogonalize_workspace(0, 4, 1, 0) == 0 and L.cakeb200_orthogonalize_workspace(4, 4, 1, 1) == 0
     assert L.cakeb200_orthogonalize_workspace(2 ** 20 + 1, 4, 1, 0) == 0
 
