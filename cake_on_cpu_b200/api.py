@@ -139,8 +139,9 @@ _SIGNATURES["cakeb200_q4_packed_bytes"] = (_sz, [_i, _i, _i, _i])
 _SIGNATURES["cakeb200_q4_quantize"] = (_i, [_vp, _ll, _i, _i, _i, _i, _i, _vp, _ll, _vp, _vp, _vp])
 _SIGNATURES["cakeb200_q4_pack"] = (_i, [_vp, _ll, _vp, _vp, _i, _i, _i, _i, _vp, _vp])
 _SIGNATURES["cakeb200_q4_dequantize"] = (_i, [_pq4, _vp, _ll, _i, _vp])
-_SIGNATURES["cakeb200_q4_linear"] = (_i, [_pq4, _vp, _ll, _vp, _vp, _ll, _i, _i, _vp])
-_SIGNATURES["cakeb200_q4_linear_dx"] = (_i, [_pq4, _vp, _ll, _vp, _ll, _i, _i, _vp])
+_SIGNATURES["cakeb200_q4_workspace"] = (_sz, [_pq4, _i, _i, _i])
+_SIGNATURES["cakeb200_q4_linear"] = (_i, [_pq4, _vp, _ll, _vp, _vp, _ll, _i, _i, _vp, _sz, _vp])
+_SIGNATURES["cakeb200_q4_linear_dx"] = (_i, [_pq4, _vp, _ll, _vp, _ll, _i, _i, _vp, _sz, _vp])
 _f, _d = ctypes.c_float, ctypes.c_double
 _SIGNATURES["cakeb200_orthogonalize_workspace"] = (_sz, [_i, _i, _i, _i])
 _SIGNATURES["cakeb200_orthogonalize"] = (_i, [_vp, _ll, _ll, _vp, _ll, _ll] + [_i] * 5 + [_f] * 4 + [_vp, _sz, _vp])
@@ -676,6 +677,14 @@ def _rows_of(t, cols, what, device, dtype=None):
     return m.data_ptr(), rows, ld
 
 
+def _workspace(need, device):
+    """(tensor to keep until the call is enqueued, its first 1024-byte aligned address) of `need` bytes of scratch.  It comes
+    from torch's allocator: every call and every captured graph has its own."""
+    import torch
+    buf = torch.empty(need + 1024, dtype=torch.uint8, device=device)
+    return buf, (buf.data_ptr() + 1023) & ~1023
+
+
 class _on_device:
     """Around a call on a tensor's device: makes the device current, and with an explicit ``stream`` (a raw
     cudaStream_t or a torch stream) that stream too, so that what the call allocates belongs to the stream it is
@@ -745,6 +754,7 @@ class Q4Weights:
             self.packed = torch.empty(n, dtype=torch.uint8, device=self.device)
             self._c = _Q4(self.packed.data_ptr(), self.out_features, self.in_features, self.group, self.scale_type, int(zeros is not None))
             self._ref = ctypes.byref(self._c)
+            self._workspace = {}  # bytes needed by (rows, type, gradient)
             _check(lib().cakeb200_q4_pack(_vp(codes.data_ptr()), codes.stride(0), _vp(scales.data_ptr()),
                                           _vp(zeros.data_ptr()) if zeros is not None else None, self.out_features, self.in_features,
                                           self.group, self.scale_type, _vp(self.packed.data_ptr()), s))
@@ -813,10 +823,15 @@ def _q4_product(dx, what, src, W4, cols_in, cols_out, bias, out, stream):
         if out is None:
             out = torch.empty(shape, dtype=src.dtype, device=src.device)
             po, ldo = out.data_ptr(), cols_out
+        key = (rows, t, dx)
+        need = W4._workspace.get(key)
+        if need is None:
+            need = W4._workspace[key] = lib().cakeb200_q4_workspace(W4._ref, rows, t, int(dx))
+        buf, ws = _workspace(need, W4.device) if need else (None, None)
         if dx:
-            _check(lib().cakeb200_q4_linear_dx(W4._ref, p, ld, po, ldo, rows, t, s))
+            _check(lib().cakeb200_q4_linear_dx(W4._ref, p, ld, po, ldo, rows, t, ws, need, s))
         else:
-            _check(lib().cakeb200_q4_linear(W4._ref, p, ld, pb, po, ldo, rows, t, s))
+            _check(lib().cakeb200_q4_linear(W4._ref, p, ld, pb, po, ldo, rows, t, ws, need, s))
     return out
 
 
@@ -859,13 +874,10 @@ def _matrix_of(t, what, device=None, shape=None):
 
 def _ns_workspace(rows, cols, batch, t, device):
     """(tensor to keep until the call is enqueued, aligned address, bytes) of the products' scratch planes."""
-    import torch
     need = lib().cakeb200_orthogonalize_workspace(rows, cols, batch, t)
     if need == 0:
         _check(-1)
-    buf = torch.empty(need + 1024, dtype=torch.uint8, device=device)
-    p = (buf.data_ptr() + 1023) & ~1023
-    return buf, p, need
+    return _workspace(need, device) + (need,)
 
 
 def cake_orthogonalize(G, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7, stream=None):

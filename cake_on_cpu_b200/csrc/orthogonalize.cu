@@ -224,18 +224,9 @@ struct StepEpilogue {
 // count it in when their stores are done, the TMA thread and the drain warps wait for the count.  The launch is
 // cooperative, so that all CTAs are resident; waits are bounded.
 //
-// A product's tiles are dealt to the units (CTAs or pairs) in turn; the tiles of the last round, fewer than there are
-// units, may be cut along K into `splits` parts of one unit each.  Parts go to memory as FP32, and after one more barrier
-// all drain warps of the machine add them up, part by part in order, 32 x 32 blocks dealt out evenly: this also spreads the
-// epilogue, which takes a CTA several microseconds on its own tile (and pays for that alone: splits may be 1).
 enum { X_ROWS, X_COLUMNS, P_SYM, Q_SYM };  // what an operand is: X, its transpose, P, Q
-struct Product {
+struct Product : plane::Tiling {
     int a, b;
-    int rows, cols, K;
-    int symmetric;
-    int tiles_m, tiles_n, tiles; // tiles: of one matrix
-    int whole;                   // tiles of all matrices that a unit finishes by itself, dealt out in turn
-    int cut, splits;             // how many others there are, and into how many parts each is cut (cut * splits <= units)
 };
 
 struct Chain {
@@ -253,30 +244,9 @@ struct Maps {
     plane::OperandMaps x[2], p, q;
 };
 
-struct Item {
-    int tile, kb0, kb1, slot;    // slot < 0: whole K, straight to the epilogue
-};
-__device__ __forceinline__ bool item_at(const Product& g, int i, int unit, int units, Item& w) {
-    const int blocks = (g.K + plane::BK - 1) / plane::BK;
-    const int mine = (g.whole - unit + units - 1) / units;  // whole tiles of this unit
-    if (i < mine) {
-        w.tile = unit + i * units; w.kb0 = 0; w.kb1 = blocks; w.slot = -1;
-        return true;
-    }
-    if (i > mine || unit >= g.cut * g.splits) return false;
-    const int part = unit / g.cut;   // units next to one another read the same range of K
-    w.tile = g.whole + unit % g.cut;
-    w.kb0 = blocks * part / g.splits;
-    w.kb1 = blocks * (part + 1) / g.splits;
-    w.slot = unit;
-    return true;
-}
-__device__ __forceinline__ void place(const Product& g, int id, int& batch, int& tm, int& tn) {
-    batch = id / g.tiles;
-    const int t = id - batch * g.tiles;
-    if (g.symmetric) plane::triangle(t, tm, tn);
-    else tile_coords(t, g.tiles_m, g.tiles_n, CAKEB200_SCHED_MKN, 8, tm, tn);
-}
+using plane::Item;
+using plane::item_at;
+using plane::place;
 
 // Stores of this thread become visible to loads of other SMs, TMA among them, once the CTA has been counted in.
 __device__ __forceinline__ void publish() { asm volatile("fence.proxy.async.global;\n\tfence.acq_rel.gpu;" ::: "memory"); }
@@ -421,13 +391,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                     at.col = tn * C::BN + b % WIDE * 32;
                     if (at.row >= g.rows || at.col >= g.cols) continue;
                     float v[32];
-                    plane::load_values(c.parts + (long long) b * 1024, v, e.lane);
-                    for (int s = 1; s < g.splits; s++) {
-                        float u[32];
-                        plane::load_values(c.parts + ((long long) s * total + b) * 1024, u, e.lane);
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] += u[j];
-                    }
+                    plane::join_parts(c.parts, b, total, g.splits, v, e.lane);
                     finish(at, v);
                     __syncwarp();
                 }
@@ -455,33 +419,6 @@ struct Layout {
     size_t bytes;
 };
 
-// One product's share of a plan, for `units` units of one form, and its time in microseconds by a model with measured constants
-// (globaltimer stamps): 0.93 (pair) or 0.75 (single SM) per K block, 2 from a barrier to the first MMA, 0.7 to read the sums out,
-// 2.0 and 1.0 per 32 x 32 block of a warp, four of a pair's tile and two of a single one's; where parts are stored 1.0 and 0.7
-// instead, then per block dealt out 2.4 and 0.15 per part; 1.2 to be counted in and 1.0 to be let go at a barrier.
-double plan_product(Product* g, int rows, int cols, int K, int symmetric, int batch, bool pair, int units) {
-    const int side = pair ? 256 : 128, blocks = (K + plane::BK - 1) / plane::BK;
-    g->rows = rows; g->cols = cols; g->K = K; g->symmetric = symmetric;
-    g->tiles_m = (rows + side - 1) / side;
-    g->tiles_n = (cols + side - 1) / side;
-    g->tiles = symmetric ? g->tiles_m * (g->tiles_m + 1) / 2 : g->tiles_m * g->tiles_n;
-    const int total = g->tiles * batch, left = total % units, rounds = total / units;
-    const double block_time = pair ? 0.93 : 0.75, round_time = blocks * block_time + 0.7, barrier = 2.2;
-    g->whole = total; g->cut = 0; g->splits = 1;
-    double best = (rounds + (left ? 1 : 0)) * round_time + 2 + (pair ? 8 : 2) + barrier;
-    const int forced = option_get(OPT_K_PIECES);
-    if (left == 0 || forced == 1) return best;
-    for (int splits = 1; splits <= std::min(units / left, blocks); splits++) {
-        const int done = (left * (side / 32) * (side / 32) + units * (pair ? 16 : 8) - 1) / (units * (pair ? 16 : 8));
-        const double time = rounds * round_time + (blocks + splits - 1) / splits * block_time + 0.7 + 2 + (pair ? 4 : 1.4) + barrier + done * (2.4 + 0.15 * splits) + barrier;
-        if (forced ? splits <= forced : time < best) {
-            g->whole = total - left; g->cut = left; g->splits = splits;
-            best = time;
-        }
-    }
-    return best;
-}
-
 // The products of one matrix size for one form.  Returns the time of a step.
 double plan(Product* gram, Product* poly, Product* apply, Product* last, int m, int n, bool tall, int batch, bool pair, int units) {
     gram->a = gram->b = X_ROWS;
@@ -489,27 +426,24 @@ double plan(Product* gram, Product* poly, Product* apply, Product* last, int m, 
     apply->a = Q_SYM; apply->b = X_COLUMNS;
     // the result as the caller stores it: Q X, or its transpose X^T Q (Q is symmetric)
     last->a = tall ? X_COLUMNS : Q_SYM; last->b = tall ? Q_SYM : X_COLUMNS;
-    const double t = plan_product(gram, m, m, n, 1, batch, pair, units) + plan_product(poly, m, m, m, 1, batch, pair, units) +
-                     plan_product(apply, m, n, m, 0, batch, pair, units);
-    plan_product(last, tall ? n : m, tall ? m : n, m, 0, batch, pair, units);
+    const plane::Costs costs = plane::costs_of(TERMS, TERMS, 3, 2.2);
+    const double t = plane::plan(gram, m, m, n, 1, batch, pair, units, costs) + plane::plan(poly, m, m, m, 1, batch, pair, units, costs) +
+                     plane::plan(apply, m, n, m, 0, batch, pair, units, costs);
+    plane::plan(last, tall ? n : m, tall ? m : n, m, 0, batch, pair, units, costs);
     return t;
 }
 
-constexpr int MAX_UNITS = 160;  // single SMs; half as many pairs
-
-// Room for the parts of cut tiles, whatever the device's number of SMs and the form: at most MAX_UNITS parts of 128 x 128 or half as
-// many of 256 x 256 values, and no more than there are K blocks of all tiles.
+// Room for the parts of cut tiles of any product, in either form.
 size_t parts_bytes(int m, int n, int batch) {
     size_t most = 0;
     for (int pair = 0; pair < 2; pair++) {
-        const long long side = pair ? 256 : 128, tm = (m + side - 1) / side, tn = (n + side - 1) / side;
+        const int side = pair ? 256 : 128;
         const long long bm = (m + plane::BK - 1) / plane::BK, bn = (n + plane::BK - 1) / plane::BK;
-        const long long pieces = std::max<long long>(tm * (tm + 1) / 2 * std::max(bm, bn), tm * tn * bm) * batch;
-        most = std::max(most, (size_t) std::min<long long>(pieces, pair ? MAX_UNITS / 2 : MAX_UNITS) * (size_t) (side * side * 4));
+        const long long pieces = std::max(plane::count_tiles(m, m, batch, true, side) * std::max(bm, bn), plane::count_tiles(m, n, batch, false, side) * bm);
+        most = std::max(most, plane::parts_bytes(pieces, pair != 0));
     }
     return most;
 }
-
 Layout lay_out(char* base, int batch, int m, int n) {
     Layout l;
     size_t at = 0;
@@ -609,7 +543,7 @@ int resident_units(int* out) {
         CAKE_CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
         n = per_sm * sms;
     }
-    n = std::min(n, PAIR ? MAX_UNITS / 2 : MAX_UNITS);
+    n = std::min(n, PAIR ? plane::MAX_UNITS / 2 : plane::MAX_UNITS);
     if (n < 1) {
         set_error("the orthogonalisation kernel does not fit the device");
         return CAKEB200_ERR_CUDA;

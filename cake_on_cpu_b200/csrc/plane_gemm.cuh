@@ -109,15 +109,34 @@ struct TileAt {
     int row, col;     // of its upper left element
 };
 
-struct Problem {
-    int rows, cols, K;   // of one product
-    int a_turn, b_turn;  // ALONG or DOWN
-    int batch;
-    int tiles_m, tiles_n, tiles;  // tiles: of one product
-    int chunk;           // K blocks between folds of `main`
-    int* status_word;
+// How a product (or `batch` products of one shape) is dealt to units, a unit being a CTA or a pair.  Tiles go to the units in
+// turn; the tiles of a ragged last round, fewer than there are units, may be cut along K into `splits` parts of one unit
+// each, which go to memory as FP32 and are joined afterwards, 32 x 32 blocks dealt out to all warps of the machine.
+struct Tiling {
+    int rows, cols, K;
+    int symmetric;               // rows == cols and D = D^T: only tiles on and below the diagonal are computed
+    int tiles_m, tiles_n, tiles; // tiles: of one product
+    int whole;                   // tiles of all products that a unit finishes by itself
+    int cut, splits;             // how many others there are, and into how many parts each is cut (cut * splits <= units)
 };
-
+struct Item {
+    int tile, kb0, kb1, slot;    // slot < 0: whole K, straight to the epilogue
+};
+__device__ __forceinline__ bool item_at(const Tiling& g, int i, int unit, int units, Item& w) {
+    const int blocks = (g.K + BK - 1) / BK;
+    const int mine = (g.whole - unit + units - 1) / units;  // whole tiles of this unit
+    if (i < mine) {
+        w.tile = unit + i * units; w.kb0 = 0; w.kb1 = blocks; w.slot = -1;
+        return true;
+    }
+    if (i > mine || unit >= g.cut * g.splits) return false;
+    const int part = unit / g.cut;   // units next to one another read the same range of K
+    w.tile = g.whole + unit % g.cut;
+    w.kb0 = (int) ((long long) blocks * part / g.splits);
+    w.kb1 = (int) ((long long) blocks * (part + 1) / g.splits);
+    w.slot = unit;
+    return true;
+}
 // tile `id` of a symmetric product's lower triangle, row by row
 __device__ __forceinline__ void triangle(int id, int& tm, int& tn) {
     tm = (int) ((sqrtf(8.f * (float) id + 1.f) - 1.f) * 0.5f);
@@ -125,11 +144,21 @@ __device__ __forceinline__ void triangle(int id, int& tm, int& tn) {
     while (tm * (tm + 1) / 2 > id) tm--;
     tn = id - tm * (tm + 1) / 2;
 }
-
-__device__ __forceinline__ void tile_at(const Problem& p, int id, int& batch, int& tm, int& tn) {
-    batch = id / p.tiles;
-    tile_coords(id - batch * p.tiles, p.tiles_m, p.tiles_n, CAKEB200_SCHED_MKN, 8, tm, tn);
+__device__ __forceinline__ void place(const Tiling& g, int id, int& batch, int& tm, int& tn) {
+    batch = id / g.tiles;
+    const int t = id - batch * g.tiles;
+    if (g.symmetric) triangle(t, tm, tn);
+    else tile_coords(t, g.tiles_m, g.tiles_n, CAKEB200_SCHED_MKN, 8, tm, tn);
 }
+
+struct Problem {
+    Tiling t;
+    int batch;
+    int a_turn, b_turn;  // ALONG or DOWN
+    int chunk;           // K blocks between folds of `main`
+    float* parts;        // of cut tiles: [slot][32 x 32 block][1024]
+    int* status_word;
+};
 
 // D = F32, A and B of one 16-bit format, both K-major (bits 15 and 16 make A and B MN-major)
 __host__ __device__ constexpr uint32_t idesc_16(uint32_t format, int m, int n) {
@@ -179,6 +208,31 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
                      : "memory");
     else
         tma_load_3d(dst, map, x, y, z, bar);
+}
+
+// A block as 4 KB of FP32 in memory, row by row per lane and 16 bytes of every lane next to one another: whole lines both ways.
+__device__ __forceinline__ void store_values(float* at, const float* v, int lane) {
+#pragma unroll
+    for (int q = 0; q < 8; q++) *reinterpret_cast<float4*>(at + q * 128 + lane * 4) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+}
+// from L2: another SM may have written it in this kernel
+__device__ __forceinline__ void load_values(const float* at, float* v, int lane) {
+#pragma unroll
+    for (int q = 0; q < 8; q++) {
+        const float4 u = __ldcg(reinterpret_cast<const float4*>(at + q * 128 + lane * 4));
+        v[4 * q] = u.x; v[4 * q + 1] = u.y; v[4 * q + 2] = u.z; v[4 * q + 3] = u.w;
+    }
+}
+
+// The sum of a block's parts, in part order: block b of `total` cut blocks.
+__device__ __forceinline__ void join_parts(const float* parts, int b, int total, int splits, float* v, int lane) {
+    load_values(parts + (long long) b * 1024, v, lane);
+    for (int s = 1; s < splits; s++) {
+        float u[32];
+        load_values(parts + ((long long) s * total + b) * 1024, u, lane);
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] += u[j];
+    }
 }
 
 // What a CTA's roles share.  Every role walks the same sequence of (tile, K range) items and keeps its own place in it.
@@ -401,37 +455,61 @@ plane_gemm_kernel(const __grid_constant__ OperandMaps map_a, const __grid_consta
     e.open(smem_raw, p.status_word);
     wait_for_previous_kernel();
     const int unit = (int) blockIdx.x / (PAIR ? 2 : 1), units = (int) gridDim.x / (PAIR ? 2 : 1);
-    const int all_tiles = p.tiles * p.batch, kblocks = (p.K + BK - 1) / BK;
+    constexpr int WIDE = C::BN / 32, PER_TILE = (C::TILE_M / 32) * WIDE;  // 32 x 32 blocks of a tile, row by row
+    Item w;
     int batch, tm, tn;
     if (e.warp < 4) {
         few_registers();
         if (e.warp == 0 && e.lane == 0) {
             bool ok = true;
-            for (int id = unit; ok && id < all_tiles; id += units) {
-                tile_at(p, id, batch, tm, tn);
+            for (int k = 0; ok && item_at(p.t, k, unit, units, w); k++) {
+                place(p.t, w.tile, batch, tm, tn);
                 const Operand a = {map_a.m, tm * C::TILE_M + (int) e.rank * 128, p.a_turn}, b = {map_b.m, tn * C::BN + (int) e.rank * 128, p.b_turn};
-                ok = e.load(a, b, batch, p.batch, 0, kblocks);
+                ok = e.load(a, b, batch, p.batch, w.kb0, w.kb1);
             }
             if (!ok) e.drain_loads();
         } else if (e.warp == 1 && e.lane == 0 && e.rank == 0) {
-            for (int id = unit; id < all_tiles; id += units)
-                if (!e.multiply(p.a_turn, p.b_turn, 0, kblocks, p.chunk)) break;
+            for (int k = 0; item_at(p.t, k, unit, units, w); k++)
+                if (!e.multiply(p.a_turn, p.b_turn, w.kb0, w.kb1, p.chunk)) break;
         }
     } else {
         many_registers();
         float sum[C::COLS];
-        for (int id = unit; id < all_tiles; id += units) {
-            if (!e.collect(0, kblocks, p.chunk, sum)) break;
+        for (int k = 0; item_at(p.t, k, unit, units, w); k++) {
+            if (!e.collect(w.kb0, w.kb1, p.chunk, sum)) break;
             TileAt at;
-            tile_at(p, id, at.batch, tm, tn);
-            at.row = tm * C::TILE_M + (int) e.rank * BM + e.quarter() * 32;
+            place(p.t, w.tile, at.batch, tm, tn);
+            const int row = (int) e.rank * BM + e.quarter() * 32;
+            at.row = tm * C::TILE_M + row;
             e.blocks(sum, [&](int column, const float* v) {
                 at.col = tn * C::BN + column;
-                if (at.row < p.rows && at.col < p.cols) Epilogue::block(ep, at, v, (uint32_t*) e.patch, e.lane);
+                if (w.slot >= 0) store_values(p.parts + ((long long) w.slot * PER_TILE + row / 32 * WIDE + column / 32) * 1024, v, e.lane);
+                else if (at.row < p.t.rows && at.col < p.t.cols) Epilogue::block(ep, at, v, (uint32_t*) e.patch, e.lane);
             });
         }
     }
     e.close();
+}
+
+// The epilogue of the cut tiles of a plane_gemm_kernel of that form: a warp per 32 x 32 block.
+template <bool PAIR, class Epilogue>
+__global__ void __launch_bounds__(256)
+join_kernel(const __grid_constant__ Problem p, const __grid_constant__ typename Epilogue::Args ep) {
+    constexpr int SIDE = PAIR ? 256 : 128, WIDE = SIDE / 32, PER_TILE = WIDE * WIDE;
+    __shared__ uint32_t patches[8][PATCH_FLOATS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int total = p.t.cut * PER_TILE, b = (int) blockIdx.x * 8 + warp;
+    wait_for_previous_kernel();
+    if (b >= total) return;
+    TileAt at;
+    int tm, tn;
+    place(p.t, p.t.whole + b / PER_TILE, at.batch, tm, tn);
+    at.row = tm * SIDE + b % PER_TILE / WIDE * 32;
+    at.col = tn * SIDE + b % WIDE * 32;
+    if (at.row >= p.t.rows || at.col >= p.t.cols) return;
+    float v[32];
+    join_parts(p.parts, b, total, p.t.splits, v, lane);
+    Epilogue::block(ep, at, v, patches[warp], lane);
 }
 
 // ------------------------------------------------------------------ epilogue helpers
@@ -489,20 +567,6 @@ __device__ __forceinline__ void by_eights(const float* v, uint32_t* patch, int l
     }
 }
 
-// A block as 4 KB of FP32 in memory, row by row per lane and 16 bytes of every lane next to one another: whole lines both ways.
-__device__ __forceinline__ void store_values(float* at, const float* v, int lane) {
-#pragma unroll
-    for (int q = 0; q < 8; q++) *reinterpret_cast<float4*>(at + q * 128 + lane * 4) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-}
-// from L2: another SM may have written it in this kernel
-__device__ __forceinline__ void load_values(const float* at, float* v, int lane) {
-#pragma unroll
-    for (int q = 0; q < 8; q++) {
-        const float4 u = __ldcg(reinterpret_cast<const float4*>(at + q * 128 + lane * 4));
-        v[4 * q] = u.x; v[4 * q + 1] = u.y; v[4 * q + 2] = u.z; v[4 * q + 3] = u.w;
-    }
-}
-
 // A block through the patch to a lane per column: f(r, value) for every row r of the block, whole rows at a time.
 template <typename F>
 __device__ __forceinline__ void by_rows(const float* v, uint32_t* patch, int lane, F f) {
@@ -534,20 +598,78 @@ inline long long count_tiles(int rows, int cols, int batch, bool symmetric, int 
     return batch * (symmetric ? m * (m + 1) / 2 : m * n);
 }
 
-// Pairs or single SMs: the shorter by a model of the time in clocks.  A K block of two planes takes 1280 clocks on a single SM
-// and 1536 on a pair (see above); the epilogue after the last tile was measured at 6000 clocks for a 128 x 128 tile and 13000
-// for a CTA's half of a 256 x 256 one.
-inline bool use_pairs(int rows, int cols, int K, int batch, int sm_count) {
-    const int forced = option_get(OPT_PAIR);  // 1: pairs, 2: single SMs, 0: this rule
-    if (forced) return forced == 1;
-    const double blocks = (K + BK - 1) / BK;
-    const double single = (double) ((count_tiles(rows, cols, batch, false, 128) + sm_count - 1) / sm_count) * (blocks * 1280 + 1500) + 6000;
-    const double pair = (double) ((count_tiles(rows, cols, batch, false, 256) + sm_count / 2 - 1) / (sm_count / 2)) * (blocks * 1536 + 1500) + 13000;
-    return pair < single;
+// What the model below knows about a kernel, in microseconds: measured with globaltimer stamps.
+struct Costs {
+    double block[2];   // a K block, [0] on a single SM, [1] on a pair
+    double between;    // from the last store of a part to the first load of a part, and likewise to what follows the product
+};
+// A K block: the MMAs (64 and 128 clocks each) or the shared-memory traffic (16 KB per plane written, 8 KB per MMA read, 128 bytes
+// a clock), whichever is longer, at 1.85 GHz and with the 10 % that both lose in practice (three products of two planes:
+// 0.75 and 0.93 measured).
+inline Costs costs_of(int ta, int tb, int products, double between) {
+    const double smem = ((ta + tb) * 16384.0 + products * 4 * 8192.0) / 128.0;
+    Costs c;
+    c.block[0] = std::max(smem, products * 4 * 64.0) * 1.1 / 1850;
+    c.block[1] = std::max(smem, products * 4 * 128.0) * 1.1 / 1850;
+    c.between = between;
+    return c;
+}
+
+// Deals a product to `units` units of one form and returns its time by the model: 2 to the first MMA, 0.7 to read a tile's sums
+// out, 2.0 and 1.0 per 32 x 32 block of a warp, four of a pair's tile and two of a single one's; where parts are stored 1.0
+// and 0.7 instead, then 2.4 and 0.15 per part for each block that a warp joins.
+inline double plan(Tiling* g, int rows, int cols, int K, int symmetric, int batch, bool pair, int units, const Costs& costs) {
+    const int side = pair ? 256 : 128, blocks = (K + BK - 1) / BK;
+    g->rows = rows; g->cols = cols; g->K = K; g->symmetric = symmetric;
+    g->tiles_m = (rows + side - 1) / side;
+    g->tiles_n = (cols + side - 1) / side;
+    g->tiles = symmetric ? g->tiles_m * (g->tiles_m + 1) / 2 : g->tiles_m * g->tiles_n;
+    const int total = g->tiles * batch, left = total % units, rounds = total / units;
+    const double block_time = costs.block[pair ? 1 : 0], round_time = blocks * block_time + 0.7;
+    g->whole = total; g->cut = 0; g->splits = 1;
+    double best = (rounds + (left ? 1 : 0)) * round_time + 2 + (pair ? 8 : 2) + costs.between;
+    const int forced = option_get(OPT_K_PIECES);
+    if (left == 0 || forced == 1) return best;
+    for (int splits = 1; splits <= std::min(units / left, blocks); splits++) {
+        const int warps = units * (pair ? 2 : 1) * DRAIN_WARPS, per_warp = (left * (side / 32) * (side / 32) + warps - 1) / warps;
+        const double time = rounds * round_time + (blocks + splits - 1) / splits * block_time + 0.7 + 2 + (pair ? 4 : 1.4) + costs.between +
+                            per_warp * (2.4 + 0.15 * splits) + costs.between;
+        if (forced ? splits <= forced : time < best) {
+            g->whole = total - left; g->cut = left; g->splits = splits;
+            best = time;
+        }
+    }
+    return best;
+}
+
+constexpr int MAX_UNITS = 160;  // single SMs; half as many pairs
+inline int units_of(bool pair, int sm_count) { return std::min(pair ? sm_count / 2 : sm_count, pair ? MAX_UNITS / 2 : MAX_UNITS); }
+// Room for the parts of `pieces` pieces (K blocks of all tiles) at most, whatever the number of SMs: a part is a tile of one form.
+inline size_t parts_bytes(long long pieces, bool pair) {
+    return (size_t) std::min<long long>(pieces, pair ? MAX_UNITS / 2 : MAX_UNITS) * (pair ? 256 * 256 * 4 : 128 * 128 * 4);
+}
+
+template <typename... P>
+int launch_kernel(void (*kernel)(P...), unsigned grid, unsigned threads, unsigned cluster, size_t smem, cudaStream_t s, P... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    CAKE_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return CAKEB200_OK;
 }
 
 template <class Format, int TA, int TB, bool PAIR, class Epilogue>
-int launch_form(const OperandMaps& a, const OperandMaps& b, Problem p, const typename Epilogue::Args& ep, int sm_count, cudaStream_t s) {
+int launch_form(const OperandMaps& a, const OperandMaps& b, const Problem& p, const typename Epilogue::Args& ep, int units, cudaStream_t s) {
     using C = Cfg<TA, TB, PAIR>;
     auto kernel = plane_gemm_kernel<Format, TA, TB, PAIR, Epilogue>;
     static std::atomic<unsigned long long> opted{0};  // devices whose shared-memory limit has been raised for this kernel
@@ -557,37 +679,31 @@ int launch_form(const OperandMaps& a, const OperandMaps& b, Problem p, const typ
         CAKE_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         if (dev < 64) opted |= 1ull << dev;
     }
-    p.tiles_m = (p.rows + C::TILE_M - 1) / C::TILE_M;
-    p.tiles_n = (p.cols + C::BN - 1) / C::BN;
-    const long long tiles = (long long) p.tiles_m * p.tiles_n;
-    if (tiles * p.batch > (1LL << 27)) {
+    units = std::min(units, std::max(p.t.whole, p.t.cut * p.t.splits));
+    int rc = launch_kernel(kernel, (unsigned) (PAIR ? 2 * units : units), THREADS, PAIR ? 2u : 1u, C::SMEM, s, a, b, p, ep);
+    if (rc || p.t.cut == 0) return rc;
+    const unsigned blocks = (unsigned) (p.t.cut * (PAIR ? 64 : 16) + 7) / 8;
+    return launch_kernel(join_kernel<PAIR, Epilogue>, blocks, 256u, 1u, 0, s, p, ep);
+}
+
+// One product (or p.batch of them).  `parts` of the problem holds parts_bytes(K blocks of all tiles) of the larger form.
+template <class Format, int TA, int TB, int PRODUCTS, class Epilogue>
+int launch(const OperandMaps& a, const OperandMaps& b, Problem p, int rows, int cols, int K, const typename Epilogue::Args& ep, int sm_count,
+           cudaStream_t s, int* launches) {
+    if (count_tiles(rows, cols, p.batch, false, 128) > (1LL << 27)) {
         set_error("the product has too many tiles");
         return CAKEB200_ERR_TOO_LARGE;
     }
-    p.tiles = (int) tiles;
-    const int per_tile = PAIR ? 2 : 1;
-    const int units = (int) std::min<long long>(tiles * p.batch, sm_count / per_tile);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) (units * per_tile));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned) per_tile;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    CAKE_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a, b, p, ep));
-    return CAKEB200_OK;
-}
-
-template <class Format, int TA, int TB, class Epilogue>
-int launch(const OperandMaps& a, const OperandMaps& b, const Problem& p, const typename Epilogue::Args& ep, int sm_count, cudaStream_t s) {
-    if (use_pairs(p.rows, p.cols, p.K, p.batch, sm_count)) return launch_form<Format, TA, TB, true, Epilogue>(a, b, p, ep, sm_count, s);
-    return launch_form<Format, TA, TB, false, Epilogue>(a, b, p, ep, sm_count, s);
+    const Costs costs = costs_of(TA, TB, PRODUCTS, 3.0);
+    const int forced = option_get(OPT_PAIR);  // 1: pairs, 2: single SMs, 0: the faster by the model
+    Tiling single, pair;
+    const double t_single = plan(&single, rows, cols, K, 0, p.batch, false, units_of(false, sm_count), costs);
+    const double t_pair = plan(&pair, rows, cols, K, 0, p.batch, true, units_of(true, sm_count), costs);
+    const bool paired = forced ? forced == 1 : t_pair < t_single;
+    p.t = paired ? pair : single;
+    if (launches) *launches += p.t.cut ? 2 : 1;
+    if (paired) return launch_form<Format, TA, TB, true, Epilogue>(a, b, p, ep, units_of(true, sm_count), s);
+    return launch_form<Format, TA, TB, false, Epilogue>(a, b, p, ep, units_of(false, sm_count), s);
 }
 
 }  // namespace plane

@@ -56,29 +56,6 @@ template <> struct Mma<__nv_bfloat16> {
 template <typename T> struct Input { using M = T; static constexpr int TERMS = 1; };
 template <> struct Input<float> { using M = __nv_bfloat16; static constexpr int TERMS = 3; };
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// v = t0 + t1 + ... with every term a bf16 (the upper half of an FP32), by truncation; a pair of values at a time.
-// An infinite value has only its first term (inf - inf would make the sum NaN where the product is infinite).
-template <int TERMS>
-__device__ __forceinline__ void split_pair(float v0, float v1, uint32_t* out) {
-#pragma unroll
-    for (int t = 0; t < TERMS; t++) {
-        out[t] = __byte_perm(__float_as_uint(v0), __float_as_uint(v1), 0x7632);
-        if (t + 1 < TERMS) {
-            const float h0 = __uint_as_float(__float_as_uint(v0) & 0xffff0000u), h1 = __uint_as_float(__float_as_uint(v1) & 0xffff0000u);
-            v0 = (t == 0 && isinf(v0)) ? 0.f : v0 - h0;
-            v1 = (t == 0 && isinf(v1)) ? 0.f : v1 - h1;
-        }
-    }
-}
-
 // Codes of one word -> the four A registers of its MMA, exact integers q - z.  sub_lo / sub_hi: MAGIC + z of rows a / a + 8.
 template <typename M>
 __device__ __forceinline__ void unpack_word(uint32_t w, uint32_t sub_lo, uint32_t sub_hi, uint32_t* a) {
@@ -134,6 +111,9 @@ __device__ __forceinline__ void reduce_and_store(float* red, int rank, int clust
     }
     cluster_sync();  // nobody leaves while its sums are still being read
 }
+
+// From this many rows on the weights are expanded and multiplied on tcgen05 (q4_gemm.cu).
+constexpr int MANY_ROWS = 65;
 
 struct Q4Args {
     Q4View w;
@@ -605,7 +585,7 @@ int launch_dx(Q4Args& p, int sm_count, cudaStream_t s) {
 
 // Common checks of the two products.  in_cols / out_cols: row lengths of the operand and of the result.
 int product(const char* who, const cakeb200_q4* w, const void* in, long long ld_in, const void* bias, void* out, long long ld_out,
-            int rows, int type, bool dx, void* stream) {
+            int rows, int type, bool dx, void* workspace, size_t workspace_bytes, void* stream) {
     *thread_stats() = cakeb200_stats();
     Q4Args p = {};
     int rc = q4_view(w, who, &p.w);
@@ -626,6 +606,12 @@ int product(const char* who, const cakeb200_q4* w, const void* in, long long ld_
     p.ld_in = ld_in; p.ld_out = ld_out; p.rows = rows;
     p.vec = (uintptr_t) in % 16 == 0 && (rows == 1 || (ld_in * (long long) size) % 16 == 0);
     cudaStream_t s = (cudaStream_t) stream;
+    if (rows >= MANY_ROWS) {
+        if (!workspace || (uintptr_t) workspace % 1024) return bad(who, "this many rows need a workspace on a 1024-byte boundary");
+        if (workspace_bytes < q4_gemm_workspace(p.w, rows, type, dx)) return bad(who, "the workspace is too small");
+        if (!on_current_device(workspace)) return bad(who, "operands must be device pointers of the current device");
+        return launch_q4_gemm(p.w, in, ld_in, bias, out, ld_out, rows, type, dx, workspace, st, s);
+    }
     if (dx)
         rc = type == CAKEB200_F32 ? launch_dx<float>(p, st->sm_count, s)
              : type == CAKEB200_F16 ? launch_dx<__half>(p, st->sm_count, s) : launch_dx<__nv_bfloat16>(p, st->sm_count, s);
@@ -761,13 +747,20 @@ int cakeb200_q4_dequantize(const cakeb200_q4* w, void* W, long long ldw, int typ
     return CAKEB200_OK;
 }
 
-int cakeb200_q4_linear(const cakeb200_q4* w, const void* x, long long ldx, const void* bias, void* y, long long ldy, int rows, int type,
-                       void* stream) {
-    return product("cakeb200_q4_linear", w, x, ldx, bias, y, ldy, rows, type, false, stream);
+size_t cakeb200_q4_workspace(const cakeb200_q4* w, int rows, int type, int dx) {
+    Q4View v;
+    if (q4_view(w, "cakeb200_q4_workspace", &v) || !known_type(type) || rows < MANY_ROWS) return 0;
+    return q4_gemm_workspace(v, rows, type, dx != 0);
 }
 
-int cakeb200_q4_linear_dx(const cakeb200_q4* w, const void* dy, long long lddy, void* dx, long long lddx, int rows, int type, void* stream) {
-    return product("cakeb200_q4_linear_dx", w, dy, lddy, nullptr, dx, lddx, rows, type, true, stream);
+int cakeb200_q4_linear(const cakeb200_q4* w, const void* x, long long ldx, const void* bias, void* y, long long ldy, int rows, int type,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+    return product("cakeb200_q4_linear", w, x, ldx, bias, y, ldy, rows, type, false, workspace, workspace_bytes, stream);
+}
+
+int cakeb200_q4_linear_dx(const cakeb200_q4* w, const void* dy, long long lddy, void* dx, long long lddx, int rows, int type, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+    return product("cakeb200_q4_linear_dx", w, dy, lddy, nullptr, dx, lddx, rows, type, true, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

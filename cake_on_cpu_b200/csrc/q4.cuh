@@ -42,7 +42,35 @@ inline __host__ __device__ int q4_scale_place(int i) { return (i & 7) * 2 + (i >
 // Checks the descriptor (no device access) and fills the view.
 int q4_view(const cakeb200_q4* w, const char* who, Q4View* out);
 
+// Products with many rows (q4_gemm.cu); type: CAKEB200_F32, _F16 or _BF16.
+size_t q4_gemm_workspace(const Q4View& w, int rows, int type, bool dx);
+int launch_q4_gemm(const Q4View& w, const void* in, long long ld_in, const void* bias, void* out, long long ld_out, int rows, int type, bool dx,
+                   void* workspace, DeviceState* st, cudaStream_t s);
+
 #ifdef __CUDACC__
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// v = t0 + t1 + ... with every term a bf16 (the upper half of an FP32), by truncation; a pair of values at a time.
+// An infinite value has only its first term (inf - inf would make the sum NaN where the product is infinite).
+template <int TERMS>
+__device__ __forceinline__ void split_pair(float v0, float v1, uint32_t* out) {
+#pragma unroll
+    for (int t = 0; t < TERMS; t++) {
+        out[t] = __byte_perm(__float_as_uint(v0), __float_as_uint(v1), 0x7632);
+        if (t + 1 < TERMS) {
+            const float h0 = __uint_as_float(__float_as_uint(v0) & 0xffff0000u), h1 = __uint_as_float(__float_as_uint(v1) & 0xffff0000u);
+            v0 = (t == 0 && isinf(v0)) ? 0.f : v0 - h0;
+            v1 = (t == 0 && isinf(v1)) ? 0.f : v1 - h1;
+        }
+    }
+}
+
 __device__ __forceinline__ float q4_scale(uint16_t bits, int is_bf16) {
     return is_bf16 ? __uint_as_float((uint32_t) bits << 16) : __half2float(__ushort_as_half(bits));
 }

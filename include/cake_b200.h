@@ -426,10 +426,13 @@ int cakeb200_unpack_B(float* B, const float* B_p, int K, int N, int p, const cak
  *     _linear:     y[r, n]  = sum_k x[r, k] w[n, k] (+ bias[n]),   rows r of x at x + r * ldx
  *     _linear_dx:  dx[r, k] = sum_n dy[r, n] w[n, k],              the gradient of _linear for its input
  *
- * x, bias, y, dy and dx share one type, CAKEB200_F32, _F16 or _BF16; leading dimensions are in elements; sums are FP32 and
- * scales are applied in FP32.  The result must not overlap the operands.  `rows` may be 0.  Device pointers of the
- * current device only; work is enqueued on `stream` and nothing else is touched, so that calls on several streams,
- * threads or captured graphs do not disturb one another.  Results do not depend on timing. */
+ * x, bias, y, dy and dx share one type, CAKEB200_F32, _F16 or _BF16; leading dimensions are in elements; sums are FP32.  Few rows
+ * are multiplied with the weights as they are, the scales applied in FP32; for many rows the weights are expanded first, a
+ * slab at a time: exactly for FP32, to 17 bits for FP16, rounded once to BF16 for BF16.  _workspace tells how many bytes
+ * of device memory, on a 1024-byte boundary, the call needs for that (0 for few rows: workspace may then be NULL); two
+ * calls that may overlap on the GPU need one each.  The result must not overlap the operands.  `rows` may be 0.  Device
+ * pointers of the current device only; work is enqueued on `stream`.  Results do not depend on timing.  Waits inside the
+ * kernels are bounded; one that gave up shows in the status of the next blocking product (cakeb200_sgemm). */
 typedef struct cakeb200_q4 {
     const void* packed;
     int out_features, in_features, group;
@@ -442,10 +445,11 @@ int cakeb200_q4_quantize(const void* W, long long ldw, int type, int out_feature
 int cakeb200_q4_pack(const void* codes, long long ldq, const void* scales, const void* zeros, int out_features, int in_features,
                      int group, int scale_type, void* packed, void* stream);
 int cakeb200_q4_dequantize(const cakeb200_q4* w, void* W, long long ldw, int type, void* stream);
+size_t cakeb200_q4_workspace(const cakeb200_q4* w, int rows, int type, int dx);
 int cakeb200_q4_linear(const cakeb200_q4* w, const void* x, long long ldx, const void* bias, void* y, long long ldy, int rows,
-                       int type, void* stream);
+                       int type, void* workspace, size_t workspace_bytes, void* stream);
 int cakeb200_q4_linear_dx(const cakeb200_q4* w, const void* dy, long long lddy, void* dx, long long lddx, int rows, int type,
-                          void* stream);
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- Orthogonalised updates.
  *

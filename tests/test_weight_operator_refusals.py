@@ -31,8 +31,8 @@ def test_q4_sizes(cake):
 def test_q4_products_refuse_bad_weights(cake, change, word):
     w = _q4(**change)
     p = ctypes.c_void_p(0x20000)
-    for rc in (cake.lib().cakeb200_q4_linear(ctypes.byref(w), p, 64, None, p, 64, 1, 0, None),
-               cake.lib().cakeb200_q4_linear_dx(ctypes.byref(w), p, 64, p, 64, 1, 0, None),
+    for rc in (cake.lib().cakeb200_q4_linear(ctypes.byref(w), p, 64, None, p, 64, 1, 0, None, 0, None),
+               cake.lib().cakeb200_q4_linear_dx(ctypes.byref(w), p, 64, p, 64, 1, 0, None, 0, None),
                cake.lib().cakeb200_q4_dequantize(ctypes.byref(w), p, 64, 0, None)):
         assert rc == ERR_ARG and word in _last(cake)
 
@@ -44,13 +44,26 @@ def test_q4_products_refuse_bad_operands(cake):
                        ((ref, None, 64, None, p, 32, 1, 0, None), "null"), ((ref, p, 64, None, None, 32, 1, 0, None), "null"),
                        ((ref, p, 63, None, p, 32, 2, 0, None), "leading dimension"), ((ref, p, 64, None, p, 31, 2, 0, None), "leading dimension"),
                        ((None, p, 64, None, p, 32, 1, 0, None), "null weights")]:
-        assert L.cakeb200_q4_linear(*args) == ERR_ARG and word in _last(cake), (args, _last(cake))
-    assert L.cakeb200_q4_linear_dx(ref, p, 31, p, 64, 2, 0, None) == ERR_ARG and "leading dimension" in _last(cake)
-    assert L.cakeb200_q4_linear(ref, None, 0, None, None, 0, 0, 0, None) == 0  # no rows: nothing to do
+        assert L.cakeb200_q4_linear(*args[:-1], None, 0, None) == ERR_ARG and word in _last(cake), (args, _last(cake))
+    assert L.cakeb200_q4_linear_dx(ref, p, 31, p, 64, 2, 0, None, 0, None) == ERR_ARG and "leading dimension" in _last(cake)
+    assert L.cakeb200_q4_linear(ref, None, 0, None, None, 0, 0, 0, None, 0, None) == 0  # no rows: nothing to do
     assert L.cakeb200_q4_pack(p, 31, p, None, 32, 64, 64, 1, p, None) == ERR_ARG and "leading dimension" in _last(cake)
     assert L.cakeb200_q4_pack(p, 32, p, None, 32, 64, 64, 1, ctypes.c_void_p(0x20001), None) == ERR_ARG and "16-byte" in _last(cake)
     assert L.cakeb200_q4_quantize(p, 63, 0, 32, 64, 64, 1, p, 32, p, None, None) == ERR_ARG and "leading dimension" in _last(cake)
     assert L.cakeb200_q4_quantize(p, 64, 0, 32, 64, 64, 0, p, 32, p, None, None) == ERR_ARG and "scales" in _last(cake)
+
+
+def test_q4_workspace(cake):
+    L = cake.lib()
+    w = _q4(n=300, k=500, group=128)
+    ref = ctypes.byref(w)
+    assert all(L.cakeb200_q4_workspace(ref, rows, t, dx) == 0 for rows in (0, 1, 64) for t in (0, 1, 2) for dx in (0, 1))
+    assert L.cakeb200_q4_workspace(ref, 65, 7, 0) == 0
+    up = lambda n: -(-n // 1024) * 1024
+    # planes of x (65 x 500, rows of 504) and of W (300 x 500), and 6 tiles of 8 K blocks of 128 x 128 or 2 of 256 x 256
+    parts = max(min(160, 3 * 8) * 65536, min(80, 2 * 8) * 262144)
+    for t, tx, tw in ((0, 3, 2), (1, 2, 2), (2, 1, 1)):
+        assert L.cakeb200_q4_workspace(ref, 65, t, 0) == up(tx * 65 * 504 * 2) + up(tw * 300 * 504 * 2) + parts
 
 
 def test_q4_python_layer_takes_cuda_tensors_only(cake):
@@ -71,7 +84,7 @@ def test_q4_without_a_device(cake):
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
     w, p = _q4(), ctypes.c_void_p(0x20000)
-    assert cake.lib().cakeb200_q4_linear(ctypes.byref(w), p, 64, None, p, 32, 1, 0, None) == ERR_NO_DEVICE
+    assert cake.lib().cakeb200_q4_linear(ctypes.byref(w), p, 64, None, p, 32, 1, 0, None, 0, None) == ERR_NO_DEVICE
 
 
 def test_orthogonalize_refusals(cake):
