@@ -166,9 +166,46 @@ __device__ __forceinline__ void load_x(const Q4Args& p, int row, int k, uint32_t
     }
 }
 
-// A CTA computes R block rows (16 R output features) x 8 NT rows of x; its warps share out the k blocks of the CTA, the
-// CTAs of a cluster those of the product.
-template <typename T, int NT, int R>
+// What a warp holds of one block row and step: codes of two blocks, scales and zero points of rows a and a + 8.
+template <int GROUPS>
+struct Step {
+    uint4 codes[2];
+    uint32_t scales[GROUPS];   // two to a word
+    uint32_t zeros[(GROUPS + 1) / 2];
+};
+template <int GROUPS>
+__device__ __forceinline__ void load_step(const Q4View& w, int rt, int step, int lane, Step<GROUPS>& s) {
+    const uint4* c = w.codes + ((long long) rt * w.steps + step) * 64 + lane;
+    s.codes[0] = load_codes(c);
+    s.codes[1] = load_codes(c + 32);
+    const long long at = ((long long) rt * w.steps + step) * (16 * GROUPS) + (lane >> 2) * (2 * GROUPS);
+    const uint16_t* p = w.scales + at;
+    if constexpr (GROUPS == 1) {
+        s.scales[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else if constexpr (GROUPS == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        s.scales[0] = v.x; s.scales[1] = v.y;
+    } else {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+        s.scales[0] = v.x; s.scales[1] = v.y; s.scales[2] = v.z; s.scales[3] = v.w;
+    }
+    if (w.zeros) {
+        const uint8_t* z = w.zeros + at;
+        if constexpr (GROUPS == 1) s.zeros[0] = __ldg(reinterpret_cast<const uint16_t*>(z));
+        else if constexpr (GROUPS == 2) s.zeros[0] = __ldg(reinterpret_cast<const uint32_t*>(z));
+        else {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(z));
+            s.zeros[0] = v.x; s.zeros[1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < (GROUPS + 1) / 2; i++) s.zeros[i] = 0x08080808u;
+    }
+}
+
+// A CTA computes R block rows (16 R output features) x 8 NT rows of x; its warps share out the steps of the CTA, the CTAs of a
+// cluster those of the product.  The next step's codes, scales and zero points are on their way while a step is multiplied.
+template <typename T, int NT, int R, int GROUPS>
 __global__ void __launch_bounds__(THREADS)
 q4_linear_kernel(const Q4Args p) {
     using M = typename Input<T>::M;
@@ -179,47 +216,45 @@ q4_linear_kernel(const Q4Args p) {
     const int rank = (int) blockIdx.x % p.cluster, rb = (int) blockIdx.x / p.cluster;
     const int row0 = (int) blockIdx.y * 8 * NT;
     const int part = rank * WARPS + warp, parts = p.cluster * WARPS;
-    const int kb0 = (int) ((long long) p.w.k_blocks * part / parts), kb1 = (int) ((long long) p.w.k_blocks * (part + 1) / parts);
-    const bool small_group = p.w.group == 32;
+    const int s0 = (int) ((long long) p.w.steps * part / parts), s1 = (int) ((long long) p.w.steps * (part + 1) / parts);
 
     float total[R][NT][4] = {};
-    const uint4* codes[R];
-    const uint16_t* scales[R];
-    const uint8_t* zeros[R];
+    Step<GROUPS> next[R];
+    if (s0 < s1) {
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int rt = min(rb * R + r, p.w.row_tiles - 1);  // a block row past the end repeats the last one and is not stored
-        codes[r] = p.w.codes + (long long) rt * p.w.k_blocks * 32 + lane;
-        scales[r] = p.w.scales + (long long) rt * p.w.groups * 16 + a * 2;
-        zeros[r] = p.w.zeros ? p.w.zeros + (long long) rt * p.w.groups * 16 + a * 2 : nullptr;
+        for (int r = 0; r < R; r++) load_step(p.w, min(rb * R + r, p.w.row_tiles - 1), s0, lane, next[r]);  // a block row past the end repeats the last one
     }
-    uint4 next[R];
-    if (kb0 < kb1) {
-#pragma unroll
-        for (int r = 0; r < R; r++) next[r] = load_codes(codes[r] + (long long) kb0 * 32);
-    }
-    for (int kb = kb0; kb < kb1; kb++) {
-        uint4 now[R];
+    for (int step = s0; step < s1; step++) {
+        Step<GROUPS> now[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
             now[r] = next[r];
-            if (kb + 1 < kb1) next[r] = load_codes(codes[r] + (long long) (kb + 1) * 32);
+            if (step + 1 < s1) load_step(p.w, min(rb * R + r, p.w.row_tiles - 1), step + 1, lane, next[r]);
         }
-        uint32_t b[NT][8][TERMS];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int half = 0; half < 2; half++) {  // a block of 64 features
+            uint32_t b[NT][8][TERMS];
 #pragma unroll
-            for (int h = 0; h < 2; h++) load_x<T>(p, row0 + nt * 8 + a, kb * 64 + h * 32 + t * 8, &b[nt][4 * h]);
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            float acc[NT][4] = {};
-            const uint32_t words[4] = {now[r].x, now[r].y, now[r].z, now[r].w};
-            uint32_t sub_lo = 0, sub_hi = 0;
-            float s_lo = 0.f, s_hi = 0.f;
+                for (int h = 0; h < 2; h++) load_x<T>(p, row0 + nt * 8 + a, step * 128 + half * 64 + h * 32 + t * 8, &b[nt][4 * h]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (j == 0 || (j == 2 && small_group)) {
-                    if (j == 2) {
+            for (int r = 0; r < R; r++) {
+                const uint4 c = now[r].codes[half];
+                const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+                float acc[NT][4] = {};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int g = (half * 4 + j) * GROUPS / 8;  // of the step
+                    const uint32_t z = now[r].zeros[g / 2] >> (16 * (g & 1));
+                    uint32_t w[4];
+                    unpack_word<M>(words[j], zero_pair<M>(z & 15u), zero_pair<M>((z >> 8) & 15u), w);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int u = TERMS - 1; u >= 0; u--) Mma<M>::run(acc[nt], w, b[nt][2 * j][u], b[nt][2 * j + 1][u]);
+                    if (j == 3 || (j == 1 && GROUPS == 4)) {  // the group (or its half in this block) is complete
+                        const float s_lo = q4_scale((uint16_t) now[r].scales[g], p.w.scale_bf16), s_hi = q4_scale((uint16_t) (now[r].scales[g] >> 16), p.w.scale_bf16);
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             total[r][nt][0] += s_lo * acc[nt][0]; total[r][nt][1] += s_lo * acc[nt][1];
@@ -227,26 +262,7 @@ q4_linear_kernel(const Q4Args p) {
                             acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
                         }
                     }
-                    const int g = (kb * 64 + j * 16) / p.w.group;
-                    const uint32_t pair = __ldg(reinterpret_cast<const uint32_t*>(scales[r] + (long long) g * 16));
-                    s_lo = q4_scale((uint16_t) (pair & 0xffffu), p.w.scale_bf16);
-                    s_hi = q4_scale((uint16_t) (pair >> 16), p.w.scale_bf16);
-                    uint32_t z = 0x0808u;
-                    if (zeros[r]) z = __ldg(reinterpret_cast<const uint16_t*>(zeros[r] + (long long) g * 16));
-                    sub_lo = zero_pair<M>(z & 15u);
-                    sub_hi = zero_pair<M>((z >> 8) & 15u);
                 }
-                uint32_t w[4];
-                unpack_word<M>(words[j], sub_lo, sub_hi, w);
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int u = TERMS - 1; u >= 0; u--) Mma<M>::run(acc[nt], w, b[nt][2 * j][u], b[nt][2 * j + 1][u]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                total[r][nt][0] += s_lo * acc[nt][0]; total[r][nt][1] += s_lo * acc[nt][1];
-                total[r][nt][2] += s_hi * acc[nt][2]; total[r][nt][3] += s_hi * acc[nt][3];
             }
         }
     }
@@ -280,7 +296,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 // of a cluster those of the product.  The reduction runs over output features, whose scales differ, so the scale goes
 // into the other operand: dy[r, n] s[n, g], formed in FP32 and split into TERMS bf16 terms (two for 16-bit types: 2^-16
 // relative, far below their own rounding; three for FP32).  Sums of one block row (16 n) leave the MMA for an FP32 total.
-template <typename T, int NT>
+template <typename T, int NT, int GROUPS>
 __global__ void __launch_bounds__(THREADS)
 q4_linear_dx_kernel(const Q4Args p) {
     using M = __nv_bfloat16;
@@ -288,21 +304,37 @@ q4_linear_dx_kernel(const Q4Args p) {
     constexpr int E = NT * 512;
     __shared__ float red[WARPS * E];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, a = lane >> 2, t = lane & 3;
-    const int rank = (int) blockIdx.x % p.cluster, kb = (int) blockIdx.x / p.cluster;
+    const int rank = (int) blockIdx.x % p.cluster, kb = (int) blockIdx.x / p.cluster;  // block of 64 features
     const int row0 = (int) blockIdx.y * 8 * NT;
     const int part = rank * WARPS + warp, parts = p.cluster * WARPS;
     const int rt0 = (int) ((long long) p.w.row_tiles * part / parts), rt1 = (int) ((long long) p.w.row_tiles * (part + 1) / parts);
-    const bool small_group = p.w.group == 32;
     const T* dy = (const T*) p.in;
 
+    // what a warp holds of one block row: a block's codes and, for its one or two groups, zero points of rows a and a + 8 and
+    // scales of rows 2 t, 2 t + 8 and 2 t + 1, 2 t + 9
+    constexpr int MINE = GROUPS == 4 ? 2 : 1;
+    struct Row {
+        uint4 codes;
+        uint32_t zeros[MINE], scales[MINE][2];
+    };
+    const int first = (kb & 1) * GROUPS / 2;  // the block's first group in its step
+    auto load = [&](int rt, Row& r) {
+        const long long at = ((long long) rt * p.w.steps + (kb >> 1)) * (16 * GROUPS);
+        r.codes = load_codes(p.w.codes + ((long long) rt * p.w.steps * 2 + kb) * 32 + lane);
+#pragma unroll
+        for (int m = 0; m < MINE; m++) {
+            r.zeros[m] = p.w.zeros ? __ldg(reinterpret_cast<const uint16_t*>(p.w.zeros + at + (a * GROUPS + first + m) * 2)) : 0x0808u;
+            r.scales[m][0] = __ldg(reinterpret_cast<const uint32_t*>(p.w.scales + at + (2 * t * GROUPS + first + m) * 2));
+            r.scales[m][1] = __ldg(reinterpret_cast<const uint32_t*>(p.w.scales + at + ((2 * t + 1) * GROUPS + first + m) * 2));
+        }
+    };
     float total[4][NT][4] = {};
-    const uint4* codes = p.w.codes + (long long) kb * 32 + lane;
-    uint4 next = {};
-    if (rt0 < rt1) next = load_codes(codes + (long long) rt0 * p.w.k_blocks * 32);
+    Row next = {};
+    if (rt0 < rt1) load(rt0, next);
     for (int rt = rt0; rt < rt1; rt++) {
-        const uint4 now = next;
-        if (rt + 1 < rt1) next = load_codes(codes + (long long) (rt + 1) * p.w.k_blocks * 32);
-        const uint32_t words[4] = {now.x, now.y, now.z, now.w};
+        const Row now = next;
+        if (rt + 1 < rt1) load(rt + 1, next);
+        const uint32_t words[4] = {now.codes.x, now.codes.y, now.codes.z, now.codes.w};
         // this lane's four output features: 16 rt + {2 t, 2 t + 1, 2 t + 8, 2 t + 9}
         float v[NT][4];
 #pragma unroll
@@ -314,37 +346,33 @@ q4_linear_dx_kernel(const Q4Args p) {
                 v[nt][i] = (row < p.rows && n < p.w.N) ? to_float(dy[row * p.ld_in + n]) : 0.f;
             }
         }
-        uint32_t b[NT][2][TERMS];
-        uint32_t sub_lo = 0, sub_hi = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j == 0 || (j == 2 && small_group)) {
-                const long long at = ((long long) rt * p.w.groups + (kb * 64 + j * 16) / p.w.group) * 16;
-                const uint2 s4 = __ldg(reinterpret_cast<const uint2*>(p.w.scales + at + 4 * t));  // rows 2t, 2t+8, 2t+1, 2t+9
-                const float s0 = q4_scale((uint16_t) s4.x, p.w.scale_bf16), s2 = q4_scale((uint16_t) (s4.x >> 16), p.w.scale_bf16);
-                const float s1 = q4_scale((uint16_t) s4.y, p.w.scale_bf16), s3 = q4_scale((uint16_t) (s4.y >> 16), p.w.scale_bf16);
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    split_pair<TERMS>(v[nt][0] * s0, v[nt][1] * s1, b[nt][0]);
-                    split_pair<TERMS>(v[nt][2] * s2, v[nt][3] * s3, b[nt][1]);
-                }
-                uint32_t z = 0x0808u;
-                if (p.w.zeros) z = __ldg(reinterpret_cast<const uint16_t*>(p.w.zeros + at + a * 2));
-                sub_lo = zero_pair<M>(z & 15u);
-                sub_hi = zero_pair<M>((z >> 8) & 15u);
-            }
-            uint32_t w[4], wt[4];
-            unpack_word<M>(words[j], sub_lo, sub_hi, w);
-            // registers 0, 1 hold the lower pairs of rows 0-7, 8-15, registers 2, 3 the upper pairs; transposed, the
-            // features are the rows of the A operand and 1 and 2 change places
-            wt[0] = transpose8(w[0]); wt[1] = transpose8(w[2]); wt[2] = transpose8(w[1]); wt[3] = transpose8(w[3]);
+        for (int m = 0; m < MINE; m++) {
+            const uint32_t s0 = now.scales[m][0], s1 = now.scales[m][1];
+            const float s[4] = {q4_scale((uint16_t) s0, p.w.scale_bf16), q4_scale((uint16_t) s1, p.w.scale_bf16),
+                                q4_scale((uint16_t) (s0 >> 16), p.w.scale_bf16), q4_scale((uint16_t) (s1 >> 16), p.w.scale_bf16)};
+            uint32_t b[NT][2][TERMS];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                float acc[4] = {};
+                split_pair<TERMS>(v[nt][0] * s[0], v[nt][1] * s[1], b[nt][0]);
+                split_pair<TERMS>(v[nt][2] * s[2], v[nt][3] * s[3], b[nt][1]);
+            }
+            const uint32_t sub_lo = zero_pair<M>(now.zeros[m] & 15u), sub_hi = zero_pair<M>((now.zeros[m] >> 8) & 15u);
 #pragma unroll
-                for (int u = TERMS - 1; u >= 0; u--) Mma<M>::run(acc, wt, b[nt][0][u], b[nt][1][u]);
+            for (int j = m * 4 / MINE; j < (m + 1) * 4 / MINE; j++) {
+                uint32_t w[4], wt[4];
+                unpack_word<M>(words[j], sub_lo, sub_hi, w);
+                // registers 0, 1 hold the lower pairs of rows 0-7, 8-15, registers 2, 3 the upper pairs; transposed, the
+                // features are the rows of the A operand and 1 and 2 change places
+                wt[0] = transpose8(w[0]); wt[1] = transpose8(w[2]); wt[2] = transpose8(w[1]); wt[3] = transpose8(w[3]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) total[j][nt][i] += acc[i];
+                for (int nt = 0; nt < NT; nt++) {
+                    float acc[4] = {};
+#pragma unroll
+                    for (int u = TERMS - 1; u >= 0; u--) Mma<M>::run(acc, wt, b[nt][0][u], b[nt][1][u]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) total[j][nt][i] += acc[i];
+                }
             }
         }
     }
@@ -428,12 +456,12 @@ q4_quantize_kernel(const T* __restrict__ W, long long ldw, int N, int K, int gro
 
 // One thread per lane of a block: 32 codes gathered from two rows.
 __global__ void __launch_bounds__(256)
-q4_pack_kernel(const uint8_t* __restrict__ codes, long long ldq, int N, int K, int row_tiles, int k_blocks, uint4* __restrict__ out) {
+q4_pack_kernel(const uint8_t* __restrict__ codes, long long ldq, int N, int K, int row_tiles, int blocks, uint4* __restrict__ out) {
     const long long i = (long long) blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (long long) row_tiles * k_blocks * 32) return;
+    if (i >= (long long) row_tiles * blocks * 32) return;
     const int lane = (int) (i & 31), a = lane >> 2, t = lane & 3;
     const long long block = i >> 5;
-    const int kb = (int) (block % k_blocks), rt = (int) (block / k_blocks);
+    const int kb = (int) (block % blocks), rt = (int) (block / blocks);
     uint32_t words[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -453,15 +481,16 @@ q4_pack_kernel(const uint8_t* __restrict__ codes, long long ldq, int N, int K, i
 }
 
 __global__ void __launch_bounds__(256)
-q4_pack_scales_kernel(const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros, int N, int groups_in, int row_tiles, int groups,
-                      uint16_t* __restrict__ out_s, uint8_t* __restrict__ out_z) {
+q4_pack_scales_kernel(const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros, int groups_in, const Q4View w, uint16_t* __restrict__ out_s,
+                      uint8_t* __restrict__ out_z) {
+    const int per_step = 1 << (7 - w.group_shift);  // groups
     const long long i = (long long) blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (long long) row_tiles * groups * 16) return;
+    if (i >= (long long) w.row_tiles * w.steps * per_step * 16) return;
     const int local = (int) (i & 15);
     const long long at = i >> 4;
-    const int g = (int) (at % groups), rt = (int) (at / groups), n = rt * 16 + local;
-    const bool in = n < N && g < groups_in;
-    const long long place = at * 16 + q4_scale_place(local);
+    const int g = (int) (at % ((long long) w.steps * per_step)), rt = (int) (at / ((long long) w.steps * per_step)), n = rt * 16 + local;
+    const bool in = n < w.N && g < groups_in;
+    const long long place = q4_scale_at(w, rt, g / per_step) + q4_scale_place(local, (g % per_step) << w.group_shift, w.group_shift);
     out_s[place] = in ? scales[(long long) n * groups_in + g] : 0;
     if (out_z) out_z[place] = in ? zeros[(long long) n * groups_in + g] : 0;
 }
@@ -471,15 +500,16 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 q4_unpack_kernel(const Q4View w, T* __restrict__ out, long long ldo) {
     const long long i = (long long) blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (long long) w.row_tiles * w.k_blocks * 32) return;
+    const int blocks = 2 * w.steps;
+    if (i >= (long long) w.row_tiles * blocks * 32) return;
     const int lane = (int) (i & 31), a = lane >> 2, t = lane & 3;
     const long long block = i >> 5;
-    const int kb = (int) (block % w.k_blocks), rt = (int) (block / w.k_blocks);
+    const int kb = (int) (block % blocks), rt = (int) (block / blocks);
     const uint4 v = w.codes[i];
     const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const long long at = ((long long) rt * w.groups + (kb * 64 + j * 16) / w.group) * 16 + a * 2;
+        const long long at = q4_scale_at(w, rt, kb >> 1) + q4_scale_place(a, (kb & 1) * 64 + j * 16, w.group_shift);
 #pragma unroll
         for (int f = 0; f < 4; f++) {
             const int n = rt * 16 + a + (f & 1) * 8;
@@ -512,8 +542,9 @@ int check_geometry(const char* who, int N, int K, int group, int scale_type) {
     return CAKEB200_OK;
 }
 
-size_t codes_bytes(int N, int K) { return (size_t) q4_row_tiles(N) * q4_k_blocks(K) * 512; }
-size_t scales_count(int N, int K, int group) { return (size_t) q4_row_tiles(N) * q4_groups(K, group) * 16; }
+size_t codes_bytes(int N, int K) { return (size_t) q4_row_tiles(N) * q4_steps(K) * 1024; }
+size_t scales_count(int N, int K, int group) { return (size_t) q4_row_tiles(N) * q4_steps(K) * (128 / group) * 16; }
+int shift_of(int group) { return group == 32 ? 5 : group == 64 ? 6 : 7; }
 
 int blocks_for(const char* who, long long threads, unsigned* out) {
     const long long b = (threads + 255) / 256;
@@ -549,38 +580,35 @@ int pick_cluster(long long ctas, int blocks, int sm_count) {
     return c;
 }
 
+template <typename T, int NT, int R>
+int launch_linear_form(Q4Args& p, int sm_count, cudaStream_t s) {
+    const unsigned rbs = (unsigned) ((p.w.row_tiles + R - 1) / R), chunks = (unsigned) ((p.rows + 8 * NT - 1) / (8 * NT));
+    p.cluster = pick_cluster((long long) rbs * chunks, p.w.steps, sm_count);
+    const unsigned x = rbs * (unsigned) p.cluster;
+    if (p.w.group_shift == 7) return launch_clustered(q4_linear_kernel<T, NT, R, 1>, x, chunks, p.cluster, p, s);
+    if (p.w.group_shift == 6) return launch_clustered(q4_linear_kernel<T, NT, R, 2>, x, chunks, p.cluster, p, s);
+    return launch_clustered(q4_linear_kernel<T, NT, R, 4>, x, chunks, p.cluster, p, s);
+}
 template <typename T>
 int launch_linear(Q4Args& p, int sm_count, cudaStream_t s) {
-    const int tiles = (p.rows + 7) / 8;
-    const bool wide = sizeof(T) == 4 && p.rows <= 8 && p.w.row_tiles >= 8 * sm_count;
-    const int R = wide ? 4 : 2;
-    const int NT = tiles >= 3 ? 4 : tiles;
-    const unsigned rbs = (unsigned) ((p.w.row_tiles + R - 1) / R);
-    const long long chunks = (tiles + NT - 1) / NT;
-    if (chunks > 65535) {
-        set_error("q4_linear: too many rows");
-        return CAKEB200_ERR_TOO_LARGE;
-    }
-    p.cluster = pick_cluster(rbs * chunks, p.w.k_blocks, sm_count);
-    const unsigned x = rbs * (unsigned) p.cluster, y = (unsigned) chunks;
-    if (wide) return launch_clustered(q4_linear_kernel<T, 1, 4>, x, y, p.cluster, p, s);
-    if (NT == 1) return launch_clustered(q4_linear_kernel<T, 1, 2>, x, y, p.cluster, p, s);
-    if (NT == 2) return launch_clustered(q4_linear_kernel<T, 2, 2>, x, y, p.cluster, p, s);
-    return launch_clustered(q4_linear_kernel<T, 4, 2>, x, y, p.cluster, p, s);
+    if (p.rows <= 8) return launch_linear_form<T, 1, 2>(p, sm_count, s);
+    if (p.rows <= 16) return launch_linear_form<T, 2, 2>(p, sm_count, s);
+    return launch_linear_form<T, 4, 2>(p, sm_count, s);
 }
 
+template <typename T, int NT>
+int launch_dx_form(Q4Args& p, int sm_count, cudaStream_t s) {
+    const unsigned blocks = 2u * (unsigned) p.w.steps, chunks = (unsigned) ((p.rows + 8 * NT - 1) / (8 * NT));
+    p.cluster = pick_cluster((long long) blocks * chunks, p.w.row_tiles, sm_count);
+    const unsigned x = blocks * (unsigned) p.cluster;
+    if (p.w.group_shift == 7) return launch_clustered(q4_linear_dx_kernel<T, NT, 1>, x, chunks, p.cluster, p, s);
+    if (p.w.group_shift == 6) return launch_clustered(q4_linear_dx_kernel<T, NT, 2>, x, chunks, p.cluster, p, s);
+    return launch_clustered(q4_linear_dx_kernel<T, NT, 4>, x, chunks, p.cluster, p, s);
+}
 template <typename T>
 int launch_dx(Q4Args& p, int sm_count, cudaStream_t s) {
-    const int tiles = (p.rows + 7) / 8, NT = tiles >= 2 ? 2 : 1;
-    const long long chunks = (tiles + NT - 1) / NT;
-    if (chunks > 65535) {
-        set_error("q4_linear_dx: too many rows");
-        return CAKEB200_ERR_TOO_LARGE;
-    }
-    p.cluster = pick_cluster(p.w.k_blocks * chunks, p.w.row_tiles, sm_count);
-    const unsigned x = (unsigned) p.w.k_blocks * (unsigned) p.cluster, y = (unsigned) chunks;
-    if (NT == 1) return launch_clustered(q4_linear_dx_kernel<T, 1>, x, y, p.cluster, p, s);
-    return launch_clustered(q4_linear_dx_kernel<T, 2>, x, y, p.cluster, p, s);
+    if (p.rows <= 8) return launch_dx_form<T, 1>(p, sm_count, s);
+    return launch_dx_form<T, 2>(p, sm_count, s);
 }
 
 // Common checks of the two products.  in_cols / out_cols: row lengths of the operand and of the result.
@@ -641,15 +669,14 @@ int q4_view(const cakeb200_q4* w, const char* who, Q4View* out) {
     if ((uintptr_t) w->packed % 16) return bad(who, "packed weights start on a 16-byte boundary");
     out->N = w->out_features;
     out->K = w->in_features;
-    out->group = w->group;
-    out->groups = q4_groups(out->K, out->group);
+    out->group_shift = shift_of(w->group);
     out->row_tiles = q4_row_tiles(out->N);
-    out->k_blocks = q4_k_blocks(out->K);
+    out->steps = q4_steps(out->K);
     out->scale_bf16 = w->scale_type == CAKEB200_BF16;
     const char* base = (const char*) w->packed;
     out->codes = (const uint4*) base;
     out->scales = (const uint16_t*) (base + codes_bytes(out->N, out->K));
-    out->zeros = w->has_zeros ? (const uint8_t*) (out->scales + scales_count(out->N, out->K, out->group)) : nullptr;
+    out->zeros = w->has_zeros ? (const uint8_t*) (out->scales + scales_count(out->N, out->K, w->group)) : nullptr;
     return CAKEB200_OK;
 }
 
@@ -709,16 +736,18 @@ int cakeb200_q4_pack(const void* codes, long long ldq, const void* scales, const
     if (!st) return CAKEB200_ERR_NO_DEVICE;
     if (!on_current_device(codes) || !on_current_device(scales) || !on_current_device(packed) || (zeros && !on_current_device(zeros)))
         return bad(who, "operands must be device pointers of the current device");
-    const int rts = q4_row_tiles(out_features), kbs = q4_k_blocks(in_features), groups = q4_groups(in_features, group);
+    const cakeb200_q4 desc = {packed, out_features, in_features, group, scale_type, zeros != nullptr};
+    Q4View v;
+    if ((rc = q4_view(&desc, who, &v))) return rc;
     unsigned b0, b1;
-    if ((rc = blocks_for(who, (long long) rts * kbs * 32, &b0)) || (rc = blocks_for(who, (long long) rts * groups * 16, &b1))) return rc;
+    if ((rc = blocks_for(who, (long long) v.row_tiles * v.steps * 64, &b0)) ||
+        (rc = blocks_for(who, (long long) scales_count(out_features, in_features, group), &b1)))
+        return rc;
     cudaStream_t s = (cudaStream_t) stream;
-    uint16_t* out_s = (uint16_t*) ((char*) packed + codes_bytes(out_features, in_features));
-    uint8_t* out_z = zeros ? (uint8_t*) (out_s + scales_count(out_features, in_features, group)) : nullptr;
-    q4_pack_kernel<<<b0, 256, 0, s>>>((const uint8_t*) codes, ldq, out_features, in_features, rts, kbs, (uint4*) packed);
+    q4_pack_kernel<<<b0, 256, 0, s>>>((const uint8_t*) codes, ldq, out_features, in_features, v.row_tiles, 2 * v.steps, (uint4*) packed);
     CAKE_CUDA_OK(cudaGetLastError());
-    q4_pack_scales_kernel<<<b1, 256, 0, s>>>((const uint16_t*) scales, (const uint8_t*) zeros, out_features,
-                                             (in_features + group - 1) / group, rts, groups, out_s, out_z);
+    q4_pack_scales_kernel<<<b1, 256, 0, s>>>((const uint16_t*) scales, (const uint8_t*) zeros, (in_features + group - 1) / group, v,
+                                             (uint16_t*) v.scales, (uint8_t*) v.zeros);
     CAKE_CUDA_OK(cudaGetLastError());
     thread_stats()->launches = 2;
     return CAKEB200_OK;
@@ -737,7 +766,7 @@ int cakeb200_q4_dequantize(const cakeb200_q4* w, void* W, long long ldw, int typ
     if (!st) return CAKEB200_ERR_NO_DEVICE;
     if (!on_current_device(w->packed) || !on_current_device(W)) return bad(who, "operands must be device pointers of the current device");
     unsigned blocks;
-    if ((rc = blocks_for(who, (long long) v.row_tiles * v.k_blocks * 32, &blocks))) return rc;
+    if ((rc = blocks_for(who, (long long) v.row_tiles * v.steps * 64, &blocks))) return rc;
     cudaStream_t s = (cudaStream_t) stream;
     if (type == CAKEB200_F32) q4_unpack_kernel<float><<<blocks, 256, 0, s>>>(v, (float*) W, ldw);
     else if (type == CAKEB200_F16) q4_unpack_kernel<__half><<<blocks, 256, 0, s>>>(v, (__half*) W, ldw);

@@ -13,7 +13,9 @@
 // hold the pair of consecutive features (k, k + 1) of fragment register i: i & 1 picks row a or a + 8, i >> 1 the
 // lower or upper pair.  A mask and a shift then leave a pair of codes in the two halves of a register.
 //
-// Scales (16 bit) and zero points (8 bit) follow, 16 per block row and group, the ones of rows a and a + 8 adjacent.
+// Blocks come in pairs, 128 features (a "step", the largest group).  Scales (16 bit) and then zero points (8 bit) follow the
+// codes, for every block row and step those of rows a and a + 8 of its 1, 2 or 4 groups: [a][group][row a, row a + 8], one load
+// per lane.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -24,20 +26,25 @@
 namespace cakeb200 {
 
 struct Q4View {
-    const uint4* codes;       // [row_tiles][k_blocks][32 lanes]
-    const uint16_t* scales;   // [row_tiles][groups][16]
+    const uint4* codes;       // [row_tiles][2 steps][32 lanes]
+    const uint16_t* scales;   // [row_tiles][steps][8][groups of a step][2]
     const uint8_t* zeros;     // same, or nullptr
     int N, K;                 // out_features, in_features
-    int group, groups;        // groups: of the features padded to whole blocks
-    int row_tiles, k_blocks;
+    int group_shift;          // the group is 1 << group_shift features
+    int row_tiles, steps;
     int scale_bf16;
 };
 
 inline __host__ __device__ int q4_row_tiles(int N) { return (N + 15) / 16; }
-inline __host__ __device__ int q4_k_blocks(int K) { return (K + 63) / 64; }
-inline __host__ __device__ int q4_groups(int K, int group) { return (q4_k_blocks(K) * 64 + group - 1) / group; }
-// place of local row i (0..15) of a block row among its 16 scales
-inline __host__ __device__ int q4_scale_place(int i) { return (i & 7) * 2 + (i >> 3); }
+inline __host__ __device__ int q4_steps(int K) { return (K + 127) / 128; }
+// Place of the scale of local row i (0..15) of a block row for the group that holds feature k of its step (0..127).
+inline __host__ __device__ int q4_scale_place(int i, int k, int group_shift) {
+    return (((i & 7) << (7 - group_shift)) + (k >> group_shift)) * 2 + (i >> 3);
+}
+// Scales of a block row and step: 16 for each of its groups.
+inline __host__ __device__ long long q4_scale_at(const Q4View& w, int rt, int step) {
+    return ((long long) rt * w.steps + step) << (4 + 7 - w.group_shift);
+}
 
 // Checks the descriptor (no device access) and fills the view.
 int q4_view(const cakeb200_q4* w, const char* who, Q4View* out);

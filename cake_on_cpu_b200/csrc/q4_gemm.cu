@@ -39,11 +39,11 @@ expand_kernel(const Q4View w, int rt0, int rts, int kb0, int kbs, const Planes o
     if (i >= (long long) rts * kbs * 32) return;
     const int lane = (int) (i & 31), a = lane >> 2, t = lane & 3;
     const int block = (int) (i >> 5), kb = block % kbs, rt = block / kbs;
-    const uint4 c = __ldg(w.codes + ((long long) (rt0 + rt) * w.k_blocks + kb0 + kb) * 32 + lane);
+    const uint4 c = __ldg(w.codes + ((long long) (rt0 + rt) * w.steps * 2 + kb0 + kb) * 32 + lane);
     const uint32_t words[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const long long at = ((long long) (rt0 + rt) * w.groups + ((kb0 + kb) * 64 + h * 32) / w.group) * 16 + a * 2;
+        const long long at = q4_scale_at(w, rt0 + rt, (kb0 + kb) >> 1) + q4_scale_place(a, ((kb0 + kb) & 1) * 64 + h * 32, w.group_shift);
         const uint32_t pair = __ldg(reinterpret_cast<const uint32_t*>(w.scales + at));
         const uint32_t z = w.zeros ? __ldg(reinterpret_cast<const uint16_t*>(w.zeros + at)) : 0x0808u;
         const int k = kb * 64 + h * 32 + t * 8;
@@ -188,7 +188,7 @@ int run(const Q4View& w, const void* in, long long ld_in, const void* bias, void
         Planes p = m.w;
         (dx ? p.cols : p.rows) = n;
         p.ld = plane::padded(p.cols);
-        const int rt0 = dx ? 0 : c0 / 16, rts = q4_row_tiles(p.rows), kb0 = dx ? c0 / 64 : 0, kbs = q4_k_blocks(p.cols);
+        const int rt0 = dx ? 0 : c0 / 16, rts = q4_row_tiles(p.rows), kb0 = dx ? c0 / 64 : 0, kbs = (p.cols + 63) / 64;
         expand_kernel<K::W><<<(unsigned) (((long long) rts * kbs * 32 + 255) / 256), 256, 0, s>>>(w, rt0, rts, kb0, kbs, p);
         CAKE_CUDA_OK(cudaGetLastError());
         *launches += 1;
