@@ -4,82 +4,108 @@
 //
 // With few rows both are bound by reading the codes from HBM: half a byte per multiply-add and row.  What stands in
 // the way of that bound is the work of turning codes into numbers.  At 6.4 TB/s an SM receives 46 codes per clock, so a
-// lane may spend 2.8 instructions on one.  Converting a code to FP32 and multiplying takes about four; here a pair of
-// codes becomes a pair of exact 16-bit integers q - z with one LOP3 and one packed subtraction (the code is placed in
-// the mantissa of a power of two, 128 or 1024, which is subtracted again together with z), and mma.m16n8k16 multiplies
-// 16 x 16 of them with up to eight rows of x at once: 1.4 instructions per code, whatever the number of rows up to eight.
-// The products are exact and summed in FP32; a group's sum is multiplied by its scale in FP32 and added to the row's
-// total, so scales are never rounded into the weights.  (tcgen05.mma would take the weights from shared memory: writing
-// converted codes there costs four times the bytes that are read from HBM.)
-//
+// lane may spend 2.8 instructions on one.  Converting a code to FP32 and multiplying takes about four; here a mask and a
+// shift place a pair of codes in the mantissas of two 16-bit numbers, which are the codes and a known offset, exactly,
+// and mma.m16n8k16 multiplies 16 x 16 of them with up to eight rows of x at once.  The products are exact and summed in
+// FP32; offset and zero point are taken out of the sum of a block (64 features) with the block's sum of x, which a further MMA
+// with ones gives for all output features; then the sum is multiplied by its scale in FP32 and added to the row's total,
+// so scales are never rounded into the weights.  (tcgen05.mma would take the weights from shared memory: writing converted
+// codes there costs four times the bytes that are read from HBM.)
+//   FP16 x: the code is a subnormal FP16, q 2^-24 or, left where it lies four bits up, 16 q 2^-24: no offset.
+//   BF16 x: 128 + q, the code in the last bits of the mantissa.  The offset makes the sums some thirty times larger than
+//           without it, which costs them five of their 24 bits and leaves them far below the result's own 2^-8.
+//   FP32 x: 128 + q, and 128 + z subtracted from every pair right away, which leaves sums as small as they can be.
 // A 32-bit x goes through the 16-bit multiplier as three terms x = x0 + x1 + x2 of 8 mantissa bits each (truncations,
 // so the split is exact and cannot overflow); the three products land in the same FP32 sums.
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "q4.cuh"
 
 namespace cakeb200 {
 namespace {
 
-constexpr int WARPS = 8;
-constexpr int THREADS = WARPS * 32;
 constexpr int MAX_CLUSTER = 8;
 
 // ------------------------------------------------------------------ small device helpers
 
-template <typename T> struct Mma;
-template <> struct Mma<__half> {
-    static constexpr uint32_t MAGIC = 0x64006400u;  // 1024 in both halves: its last mantissa bit counts 1
-    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-        const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-    static __device__ __forceinline__ void run(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+template <typename M>
+__device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(M) == 2 && std::is_same<M, __half>::value)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-template <> struct Mma<__nv_bfloat16> {
-    static constexpr uint32_t MAGIC = 0x43004300u;  // 128 in both halves
-    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-    static __device__ __forceinline__ void run(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-// element type of the MMA and number of terms per element of x
-template <typename T> struct Input { using M = T; static constexpr int TERMS = 1; };
-template <> struct Input<float> { using M = __nv_bfloat16; static constexpr int TERMS = 3; };
-
-// Codes of one word -> the four A registers of its MMA, exact integers q - z.  sub_lo / sub_hi: MAGIC + z of rows a / a + 8.
-template <typename M>
-__device__ __forceinline__ void unpack_word(uint32_t w, uint32_t sub_lo, uint32_t sub_hi, uint32_t* a) {
+}
+// The four A registers of a word's MMA.  A code in the mantissa of a power of two whose last mantissa bit counts 1 (128 + q),
+// then the power and the zero point subtracted, both halves at once: exact whole numbers.  sub_lo / sub_hi: 128 + z of rows a / a + 8.
+__device__ __forceinline__ void unpack_centred(uint32_t w, uint32_t sub_lo, uint32_t sub_hi, uint32_t* a) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | Mma<M>::MAGIC;
-        a[i] = Mma<M>::sub(v, (i & 1) ? sub_hi : sub_lo);
+        const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        const uint32_t sub = (i & 1) ? sub_hi : sub_lo;
+        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&sub));
+        a[i] = *reinterpret_cast<const uint32_t*>(&r);
     }
 }
-// 16-bit pattern of MAGIC + z in both halves (z < 16: exact, and its bits lie below the magic's)
-template <typename M>
-__device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
-    return Mma<M>::MAGIC | (z << 16) | z;
-}
+// 128 + z in both halves (z < 16)
+__device__ __forceinline__ uint32_t zero_pair(uint32_t z) { return 0x43004300u | (z << 16) | z; }
 
-__device__ __forceinline__ uint4 load_codes(const uint4* p) {
-    uint4 v;  // read once: not kept in L1, where x and the scales live
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
+// The same for the forward product's types.  OFFSET is what the numbers have on top of q; UP_LO and UP_HI are what those of rows
+// a and a + 8 (registers 0, 2 and 1, 3) are multiplied by.
+template <typename T> struct Codes;
+template <> struct Codes<__half> {
+    using M = __half;
+    static constexpr int TERMS = 1;
+    static constexpr bool SUM = true;
+    static constexpr float OFFSET = 0.f, DOWN_LO = 16777216.f, DOWN_HI = 1048576.f;
+    static constexpr uint32_t ONE = 0x3c003c00u;
+    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t, uint32_t, uint32_t* a) {
+        a[0] = w & 0x000f000fu;
+        a[1] = w & 0x00f000f0u;
+        w >>= 8;
+        a[2] = w & 0x000f000fu;
+        a[3] = w & 0x00f000f0u;
+    }
+};
+template <> struct Codes<__nv_bfloat16> {
+    using M = __nv_bfloat16;
+    static constexpr int TERMS = 1;
+    static constexpr bool SUM = true;
+    static constexpr float OFFSET = 128.f, DOWN_LO = 1.f, DOWN_HI = 1.f;
+    static constexpr uint32_t ONE = 0x3f803f80u;
+    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t, uint32_t, uint32_t* a) {
+        a[0] = (w & 0x000f000fu) | 0x43004300u;
+#pragma unroll
+        for (int i = 1; i < 4; i++) a[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    }
+};
+template <> struct Codes<float> {
+    using M = __nv_bfloat16;
+    static constexpr int TERMS = 3;
+    static constexpr bool SUM = false;
+    static constexpr float OFFSET = 0.f, DOWN_LO = 1.f, DOWN_HI = 1.f;
+    static constexpr uint32_t ONE = 0;
+    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t sub_lo, uint32_t sub_hi, uint32_t* a) {
+        unpack_centred(w, sub_lo, sub_hi, a);
+    }
+};
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+// Codes are read once and go past L1 into a queue of the lane's own in shared memory, so that many are on their way without
+// holding registers; a lane reads back what it asked for itself.
+__device__ __forceinline__ void fetch16(uint4* to, const uint4* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t) __cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
+__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ float load_remote(const float* local, int rank) {
     uint32_t a = (uint32_t) __cvta_generic_to_shared(local), r;
     float v;
@@ -88,28 +114,20 @@ __device__ __forceinline__ float load_remote(const float* local, int rank) {
     return v;
 }
 
-// Sums `red`[WARPS][E] over the warps of the CTA and then over the CTAs of the cluster, in that fixed order, and hands
-// every element of this CTA's share to `store(e, value)`.
-template <int E, typename F>
-__device__ __forceinline__ void reduce_and_store(float* red, int rank, int cluster, F store) {
-    __syncthreads();
-    for (int e = threadIdx.x; e < E; e += THREADS) {
-        float s = red[e];
-#pragma unroll
-        for (int w = 1; w < WARPS; w++) s += red[w * E + e];
-        red[e] = s;
-        if (cluster == 1) store(e, s);
-    }
-    if (cluster == 1) return;
-    cluster_sync();
+// Hands the sums of `red`[SETS][E] over the sets of all CTAs of the cluster, in that fixed order, to `store(e, value)`: every CTA
+// finishes its share of the E elements.
+template <int E, int SETS, int WARPS, typename F>
+__device__ __forceinline__ void join(const float* red, int rank, int cluster, F store) {
     const int per = E / cluster;
-    for (int i = threadIdx.x; i < per; i += THREADS) {
+    for (int i = threadIdx.x; i < per; i += WARPS * 32) {
         const int e = rank * per + i;
         float s = 0.f;
-        for (int c = 0; c < cluster; c++) s += load_remote(red + e, c);
+        for (int c = 0; c < cluster; c++) {
+#pragma unroll
+            for (int w = 0; w < SETS; w++) s += load_remote(red + w * E + e, c);
+        }
         store(e, s);
     }
-    cluster_sync();  // nobody leaves while its sums are still being read
 }
 
 // From this many rows on the weights are expanded and multiplied on tcgen05 (q4_gemm.cu).
@@ -124,62 +142,57 @@ struct Q4Args {
     int rows;
     int vec;             // 16-byte loads of x allowed
     int cluster;
+    int chunks;          // of 8 NT rows
 };
 
 // ------------------------------------------------------------------ y = x W^T + b
 
-// B fragments of one 32-feature half of a block for one tile of eight rows: lane (a, t) holds features 8 t .. 8 t + 7 of row a.
+// B fragments of a lane for a block: features 32 h + 8 t + 0 .. 7, h = 0, 1, of its row, pairs of features to a register.  `x` points at
+// the first of them; `inside`: 16-byte loads are allowed and the block ends within the row.
 template <typename T>
-__device__ __forceinline__ void load_x(const Q4Args& p, int row, int k, uint32_t (*b)[Input<T>::TERMS]) {
-    constexpr int TERMS = Input<T>::TERMS;
-    if (row >= p.rows || k >= p.w.K) {
+__device__ __forceinline__ void load_x(const T* x, bool inside, int left, uint32_t (*b)[Codes<T>::TERMS]) {
+    constexpr int TERMS = Codes<T>::TERMS;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+    for (int h = 0; h < 2; h++) {
+        const T* p = x + 32 * h;
+        if constexpr (sizeof(T) == 2) {
+            if (inside) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+                b[4 * h][0] = v.x; b[4 * h + 1][0] = v.y; b[4 * h + 2][0] = v.z; b[4 * h + 3][0] = v.w;
+            } else {
+                const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-            for (int t = 0; t < TERMS; t++) b[i][t] = 0u;
-        return;
-    }
-    const T* x = (const T*) p.in + row * p.ld_in + k;
-    if constexpr (sizeof(T) == 2) {
-        if (p.vec && k + 8 <= p.w.K) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(x));
-            b[0][0] = v.x; b[1][0] = v.y; b[2][0] = v.z; b[3][0] = v.w;
-        } else {
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t lo = k + 2 * i < p.w.K ? __ldg(h + 2 * i) : 0, hi = k + 2 * i + 1 < p.w.K ? __ldg(h + 2 * i + 1) : 0;
-                b[i][0] = lo | (hi << 16);
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t lo = 32 * h + 2 * i < left ? __ldg(u + 2 * i) : 0, hi = 32 * h + 2 * i + 1 < left ? __ldg(u + 2 * i + 1) : 0;
+                    b[4 * h + i][0] = lo | (hi << 16);
+                }
             }
-        }
-    } else {
-        float v[8];
-        if (p.vec && k + 8 <= p.w.K) {
-            const float4 u0 = __ldg(reinterpret_cast<const float4*>(x)), u1 = __ldg(reinterpret_cast<const float4*>(x) + 1);
-            v[0] = u0.x; v[1] = u0.y; v[2] = u0.z; v[3] = u0.w; v[4] = u1.x; v[5] = u1.y; v[6] = u1.z; v[7] = u1.w;
         } else {
+            float v[8];
+            if (inside) {
+                const float4 u0 = __ldg(reinterpret_cast<const float4*>(p)), u1 = __ldg(reinterpret_cast<const float4*>(p) + 1);
+                v[0] = u0.x; v[1] = u0.y; v[2] = u0.z; v[3] = u0.w; v[4] = u1.x; v[5] = u1.y; v[6] = u1.z; v[7] = u1.w;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = k + i < p.w.K ? __ldg(x + i) : 0.f;
+                for (int i = 0; i < 8; i++) v[i] = 32 * h + i < left ? __ldg(p + i) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) split_pair<TERMS>(v[2 * i], v[2 * i + 1], b[4 * h + i]);
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) split_pair<TERMS>(v[2 * i], v[2 * i + 1], b[i]);
     }
 }
 
-// What a warp holds of one block row and step: codes of two blocks, scales and zero points of rows a and a + 8.
+// Scales and zero points of rows a and a + 8 for one block row and step.
 template <int GROUPS>
-struct Step {
-    uint4 codes[2];
+struct Scales {
     uint32_t scales[GROUPS];   // two to a word
     uint32_t zeros[(GROUPS + 1) / 2];
 };
+// `at`: block row times steps plus step.
 template <int GROUPS>
-__device__ __forceinline__ void load_step(const Q4View& w, int rt, int step, int lane, Step<GROUPS>& s) {
-    const uint4* c = w.codes + ((long long) rt * w.steps + step) * 64 + lane;
-    s.codes[0] = load_codes(c);
-    s.codes[1] = load_codes(c + 32);
-    const long long at = ((long long) rt * w.steps + step) * (16 * GROUPS) + (lane >> 2) * (2 * GROUPS);
-    const uint16_t* p = w.scales + at;
+__device__ __forceinline__ void load_scales(const Q4View& w, int at, int a, Scales<GROUPS>& s) {
+    const long long place = (long long) at * (16 * GROUPS) + a * (2 * GROUPS);
+    const uint16_t* p = w.scales + place;
     if constexpr (GROUPS == 1) {
         s.scales[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
     } else if constexpr (GROUPS == 2) {
@@ -190,7 +203,7 @@ __device__ __forceinline__ void load_step(const Q4View& w, int rt, int step, int
         s.scales[0] = v.x; s.scales[1] = v.y; s.scales[2] = v.z; s.scales[3] = v.w;
     }
     if (w.zeros) {
-        const uint8_t* z = w.zeros + at;
+        const uint8_t* z = w.zeros + place;
         if constexpr (GROUPS == 1) s.zeros[0] = __ldg(reinterpret_cast<const uint16_t*>(z));
         else if constexpr (GROUPS == 2) s.zeros[0] = __ldg(reinterpret_cast<const uint32_t*>(z));
         else {
@@ -203,84 +216,211 @@ __device__ __forceinline__ void load_step(const Q4View& w, int rt, int step, int
     }
 }
 
-// A CTA computes R block rows (16 R output features) x 8 NT rows of x; its warps share out the steps of the CTA, the CTAs of a
-// cluster those of the product.  The next step's codes, scales and zero points are on their way while a step is multiplied.
-template <typename T, int NT, int R, int GROUPS>
-__global__ void __launch_bounds__(THREADS)
+// An item is R block rows (16 R output features) x 8 NT rows of x.  Clusters take items in turn; the warps of a cluster share
+// out an item's steps.  While a step is multiplied the codes of the next two and the scales of the next one are on their way,
+// across the ends of items, and the sums of an item are joined while the next one is multiplied: warps leave them in shared
+// memory, arrive at the cluster's barrier, and only wait for it at the end of the next item.  (With one CTA per item and
+// the join at its end the machine stood a quarter idle: 512 items do not divide among 148 SMs.)
+constexpr int AHEAD = 3;  // steps in a lane's queue
+
+template <typename T, int NT, int R, int GROUPS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32)
 q4_linear_kernel(const Q4Args p) {
-    using M = typename Input<T>::M;
-    constexpr int TERMS = Input<T>::TERMS;
+    using C = Codes<T>;
+    using M = typename C::M;
+    constexpr int TERMS = C::TERMS;
     constexpr int E = R * NT * 128;
-    __shared__ float red[WARPS * E];
+    constexpr int QUEUE = AHEAD * R * 64;  // of a warp, in 16-byte pieces
+    // with few columns there are registers for what keeps a lone warp busy: x of a whole step loaded at its start, and two chains of
+    // dependent MMAs per sum
+    constexpr int HALVES = NT == 1 && TERMS == 1 ? 2 : 1, CHAINS = NT == 1 ? 2 : 1;
+    extern __shared__ uint4 shared[];      // queues, then two sets of sums
+    float* red = (float*) (shared + WARPS * QUEUE);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, a = lane >> 2, t = lane & 3;
-    const int rank = (int) blockIdx.x % p.cluster, rb = (int) blockIdx.x / p.cluster;
-    const int row0 = (int) blockIdx.y * 8 * NT;
+    uint4* queue = shared + warp * QUEUE + lane;
+    const int rank = (int) blockIdx.x % p.cluster, unit = (int) blockIdx.x / p.cluster, units = (int) gridDim.x / p.cluster;
+    const int rbs = p.w.row_tiles / R, items = rbs * p.chunks;
     const int part = rank * WARPS + warp, parts = p.cluster * WARPS;
     const int s0 = (int) ((long long) p.w.steps * part / parts), s1 = (int) ((long long) p.w.steps * (part + 1) / parts);
+    const int mine = s1 > s0 ? (items - unit + units - 1) / units * (s1 - s0) : 0;  // steps of this warp, over all its items
 
-    float total[R][NT][4] = {};
-    Step<GROUPS> next[R];
-    if (s0 < s1) {
-#pragma unroll
-        for (int r = 0; r < R; r++) load_step(p.w, min(rb * R + r, p.w.row_tiles - 1), s0, lane, next[r]);  // a block row past the end repeats the last one
-    }
-    for (int step = s0; step < s1; step++) {
-        Step<GROUPS> now[R];
+    // Steps in the order in which this warp does them; `at` of block row r is r * steps further.
+    struct Cursor {
+        int item, left, at;
+    };
+    auto place = [&](int item) { return item % rbs * R * p.w.steps + s0; };
+    auto advance = [&](Cursor& c) {
+        c.at++;
+        if (--c.left == 0) {
+            c.left = s1 - s0;
+            c.item += units;
+            c.at = place(c.item);
+        }
+    };
+    auto fetch = [&](const Cursor& c, int where) {
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            now[r] = next[r];
-            if (step + 1 < s1) load_step(p.w, min(rb * R + r, p.w.row_tiles - 1), step + 1, lane, next[r]);
+            const uint4* from = p.w.codes + (long long) (c.at + r * p.w.steps) * 64 + lane;
+            fetch16(queue + (where * R + r) * 64, from);
+            fetch16(queue + (where * R + r) * 64 + 32, from + 32);
         }
+    };
+    Cursor codes_cursor = {unit, s1 - s0, place(unit)}, scales_cursor = codes_cursor;
+    Scales<GROUPS> next[R];
 #pragma unroll
-        for (int half = 0; half < 2; half++) {  // a block of 64 features
-            uint32_t b[NT][8][TERMS];
+    for (int i = 0; i < AHEAD - 1; i++) {
+        if (i < mine) {
+            fetch(codes_cursor, i);
+            advance(codes_cursor);
+        }
+        fetch_commit();
+    }
+    if (mine) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+        for (int r = 0; r < R; r++) load_scales(p.w, scales_cursor.at + r * p.w.steps, a, next[r]);
+        advance(scales_cursor);
+    }
+
+    T* out = (T*) p.out;
+    const T* bias = (const T*) p.bias;
+    auto finish = [&](int item, int set) {
+        const int rb = item % rbs, row0 = item / rbs * 8 * NT;
+        join<E, WARPS, WARPS>(red + set * WARPS * E, rank, p.cluster, [&](int e, float v) {
+            const int l = e & 31, i = (e >> 5) & 3, nt = (e >> 7) % NT, r = (e >> 7) / NT;
+            const int n = (rb * R + r) * 16 + (l >> 2) + (i >> 1) * 8, row = row0 + nt * 8 + (l & 3) * 2 + (i & 1);
+            if (n >= p.w.N || row >= p.rows) return;
+            if (bias) v += to_float(bias[n]);
+            out[row * p.ld_out + n] = from_float<T>(v);
+        });
+    };
+
+    int slot = 0, free = AHEAD - 1, done = 0, set = 0;
+    for (int item = unit; item < items; item += units, set ^= 1) {
+        const int row0 = item / rbs * 8 * NT;
+        const T* x[NT];  // rows past the last repeat it; their columns of the MMA are not stored
 #pragma unroll
-                for (int h = 0; h < 2; h++) load_x<T>(p, row0 + nt * 8 + a, step * 128 + half * 64 + h * 32 + t * 8, &b[nt][4 * h]);
+        for (int nt = 0; nt < NT; nt++) x[nt] = (const T*) p.in + (long long) min(row0 + nt * 8 + a, p.rows - 1) * p.ld_in + s0 * 128 + t * 8;
+        float total[R][NT][4] = {};
+        for (int step = s0; step < s1; step++, done++) {
+            Scales<GROUPS> now[R];
+            const bool inside = p.vec && step * 128 + 128 <= p.w.K;
+            uint32_t b[HALVES][NT][8][TERMS];
+            auto load = [&](int half) {
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                const uint4 c = now[r].codes[half];
-                const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-                float acc[NT][4] = {};
+                for (int nt = 0; nt < NT; nt++) {
+                    load_x<T>(x[nt], inside, p.w.K - (step * 128 + half * 64 + t * 8), b[half % HALVES][nt]);
+                    x[nt] += 64;
+                }
+            };
+            if (HALVES == 2) { load(0); load(1); }
+            if (done + AHEAD - 1 < mine) {
+                fetch(codes_cursor, free);
+                advance(codes_cursor);
+            }
+            fetch_commit();
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int g = (half * 4 + j) * GROUPS / 8;  // of the step
-                    const uint32_t z = now[r].zeros[g / 2] >> (16 * (g & 1));
-                    uint32_t w[4];
-                    unpack_word<M>(words[j], zero_pair<M>(z & 15u), zero_pair<M>((z >> 8) & 15u), w);
+            for (int r = 0; r < R; r++) now[r] = next[r];
+            if (done + 1 < mine) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
+                for (int r = 0; r < R; r++) load_scales(p.w, scales_cursor.at + r * p.w.steps, a, next[r]);
+                advance(scales_cursor);
+            }
+            fetch_wait<AHEAD - 1>();
+            float acc[R][NT][CHAINS][4], sums[NT][CHAINS][4];
 #pragma unroll
-                        for (int u = TERMS - 1; u >= 0; u--) Mma<M>::run(acc[nt], w, b[nt][2 * j][u], b[nt][2 * j + 1][u]);
-                    if (j == 3 || (j == 1 && GROUPS == 4)) {  // the group (or its half in this block) is complete
-                        const float s_lo = q4_scale((uint16_t) now[r].scales[g], p.w.scale_bf16), s_hi = q4_scale((uint16_t) (now[r].scales[g] >> 16), p.w.scale_bf16);
+            for (int half = 0; half < 2; half++) {  // a block of 64 features
+                if (HALVES == 1) load(half);
+#pragma unroll
+                for (int part = 0; part < 2; part++) {  // 32 features, words 2 part and 2 part + 1
+                    constexpr int PARTS = 4 / GROUPS;   // of a group
+                    const int g = (half * 2 + part) / PARTS;
+                    const bool first = (half * 2 + part) % PARTS == 0, last = (half * 2 + part) % PARTS == PARTS - 1;
+                    if (first) {
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            total[r][nt][0] += s_lo * acc[nt][0]; total[r][nt][1] += s_lo * acc[nt][1];
-                            total[r][nt][2] += s_hi * acc[nt][2]; total[r][nt][3] += s_hi * acc[nt][3];
-                            acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+                            for (int i = 0; i < CHAINS * 4; i++) {
+                                sums[nt][i / 4][i % 4] = 0.f;
+#pragma unroll
+                                for (int r = 0; r < R; r++) acc[r][nt][i / 4][i % 4] = 0.f;
+                            }
+                        }
+                    }
+                    if (C::SUM) {
+                        const uint32_t ones[4] = {C::ONE, C::ONE, C::ONE, C::ONE};
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int j = 2 * part; j < 2 * part + 2; j++) mma<M>(sums[nt][j % CHAINS], ones, b[half % HALVES][nt][2 * j][0], b[half % HALVES][nt][2 * j + 1][0]);
+                    }
+                    uint2 c[R];
+#pragma unroll
+                    for (int r = 0; r < R; r++) c[r] = reinterpret_cast<const uint2*>(&queue[(slot * R + r) * 64 + half * 32])[part];
+#pragma unroll
+                    for (int j = 2 * part; j < 2 * part + 2; j++) {
+#pragma unroll
+                        for (int r = 0; r < R; r++) {
+                            const uint32_t z = now[r].zeros[g / 2] >> (16 * (g & 1));
+                            uint32_t w[4];
+                            C::unpack(j & 1 ? c[r].y : c[r].x, zero_pair(z & 15u), zero_pair((z >> 8) & 15u), w);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                for (int u = TERMS - 1; u >= 0; u--)
+                                    mma<M>(acc[r][nt][j % CHAINS], w, b[half % HALVES][nt][2 * j][u], b[half % HALVES][nt][2 * j + 1][u]);
+                        }
+                    }
+                    if (last) {  // the group is complete
+#pragma unroll
+                        for (int r = 0; r < R; r++) {
+                            const uint32_t z = now[r].zeros[g / 2] >> (16 * (g & 1));
+                            const float s_lo = q4_scale((uint16_t) now[r].scales[g], p.w.scale_bf16), s_hi = q4_scale((uint16_t) (now[r].scales[g] >> 16), p.w.scale_bf16);
+                            const float z_lo = s_lo * (C::OFFSET + (float) (z & 15u)), z_hi = s_hi * (C::OFFSET + (float) ((z >> 8) & 15u));
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                                for (int i = 0; i < 2; i++) {
+                                    float lo = acc[r][nt][0][i], hi = acc[r][nt][0][i + 2], x_sum = sums[nt][0][i];
+                                    if (CHAINS == 2) {
+                                        lo += acc[r][nt][CHAINS - 1][i];
+                                        hi += acc[r][nt][CHAINS - 1][i + 2];
+                                        x_sum += sums[nt][CHAINS - 1][i];
+                                    }
+                                    if (C::SUM) {
+                                        total[r][nt][i] += fmaf(s_lo * C::DOWN_LO, lo, -z_lo * x_sum);
+                                        total[r][nt][i + 2] += fmaf(s_hi * C::DOWN_HI, hi, -z_hi * x_sum);
+                                    } else {
+                                        total[r][nt][i] = fmaf(s_lo, lo, total[r][nt][i]);
+                                        total[r][nt][i + 2] = fmaf(s_hi, hi, total[r][nt][i + 2]);
+                                    }
+                                }
+                            }
                         }
                     }
                 }
             }
+            free = slot;
+            if (++slot == AHEAD) slot = 0;
+        }
+        if (item != unit) {  // the item before this one: everybody's sums of it are there
+            cluster_wait();
+            finish(item - units, set ^ 1);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) red[(set * WARPS + warp) * E + ((r * NT + nt) * 4 + i) * 32 + lane] = total[r][nt][i];
+        __syncwarp();
+        cluster_arrive();
+        if (item + units >= items) {
+            cluster_wait();
+            finish(item, set);
         }
     }
-#pragma unroll
-    for (int r = 0; r < R; r++)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) red[warp * E + ((r * NT + nt) * 4 + i) * 32 + lane] = total[r][nt][i];
-    T* out = (T*) p.out;
-    const T* bias = (const T*) p.bias;
-    reduce_and_store<E>(red, rank, p.cluster, [&](int e, float v) {
-        const int l = e & 31, i = (e >> 5) & 3, nt = (e >> 7) % NT, r = (e >> 7) / NT;
-        const int n = (rb * R + r) * 16 + (l >> 2) + (i >> 1) * 8, row = row0 + nt * 8 + (l & 3) * 2 + (i & 1);
-        if (n >= p.w.N || row >= p.rows) return;
-        if (bias) v += to_float(bias[n]);
-        out[row * p.ld_out + n] = from_float<T>(v);
-    });
+    cluster_arrive();  // nobody leaves while its sums may still be read
+    cluster_wait();
 }
 
 // ------------------------------------------------------------------ dx = dy W
@@ -296,14 +436,17 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 // of a cluster those of the product.  The reduction runs over output features, whose scales differ, so the scale goes
 // into the other operand: dy[r, n] s[n, g], formed in FP32 and split into TERMS bf16 terms (two for 16-bit types: 2^-16
 // relative, far below their own rounding; three for FP32).  Sums of one block row (16 n) leave the MMA for an FP32 total.
-template <typename T, int NT, int GROUPS>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, int NT, int GROUPS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32)
 q4_linear_dx_kernel(const Q4Args p) {
     using M = __nv_bfloat16;
     constexpr int TERMS = sizeof(T) == 4 ? 3 : 2;
     constexpr int E = NT * 512;
-    __shared__ float red[WARPS * E];
+    constexpr int DX_AHEAD = 8;            // block rows in a lane's queue
+    __shared__ uint4 shared[WARPS * (DX_AHEAD * 128 > E ? DX_AHEAD * 32 : E / 4)];
+    float* red = (float*) shared;          // the queues' place, once they are empty
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, a = lane >> 2, t = lane & 3;
+    uint4* queue = shared + warp * DX_AHEAD * 32 + lane;
     const int rank = (int) blockIdx.x % p.cluster, kb = (int) blockIdx.x / p.cluster;  // block of 64 features
     const int row0 = (int) blockIdx.y * 8 * NT;
     const int part = rank * WARPS + warp, parts = p.cluster * WARPS;
@@ -314,13 +457,11 @@ q4_linear_dx_kernel(const Q4Args p) {
     // scales of rows 2 t, 2 t + 8 and 2 t + 1, 2 t + 9
     constexpr int MINE = GROUPS == 4 ? 2 : 1;
     struct Row {
-        uint4 codes;
         uint32_t zeros[MINE], scales[MINE][2];
     };
     const int first = (kb & 1) * GROUPS / 2;  // the block's first group in its step
     auto load = [&](int rt, Row& r) {
         const long long at = ((long long) rt * p.w.steps + (kb >> 1)) * (16 * GROUPS);
-        r.codes = load_codes(p.w.codes + ((long long) rt * p.w.steps * 2 + kb) * 32 + lane);
 #pragma unroll
         for (int m = 0; m < MINE; m++) {
             r.zeros[m] = p.w.zeros ? __ldg(reinterpret_cast<const uint16_t*>(p.w.zeros + at + (a * GROUPS + first + m) * 2)) : 0x0808u;
@@ -329,12 +470,28 @@ q4_linear_dx_kernel(const Q4Args p) {
         }
     };
     float total[4][NT][4] = {};
+    const uint4* codes = p.w.codes + ((long long) rt0 * p.w.steps * 2 + kb) * 32 + lane;
+    const long long stride = (long long) p.w.steps * 64;
+#pragma unroll
+    for (int i = 0; i < DX_AHEAD - 1; i++) {
+        if (rt0 + i < rt1) fetch16(queue + i * 32, codes);
+        codes += stride;
+        fetch_commit();
+    }
     Row next = {};
     if (rt0 < rt1) load(rt0, next);
+    int slot = 0, free = DX_AHEAD - 1;
     for (int rt = rt0; rt < rt1; rt++) {
         const Row now = next;
+        if (rt + DX_AHEAD - 1 < rt1) fetch16(queue + free * 32, codes);
+        codes += stride;
+        fetch_commit();
         if (rt + 1 < rt1) load(rt + 1, next);
-        const uint32_t words[4] = {now.codes.x, now.codes.y, now.codes.z, now.codes.w};
+        fetch_wait<DX_AHEAD - 1>();
+        const uint4 c = queue[slot * 32];
+        free = slot;
+        slot = (slot + 1) % DX_AHEAD;
+        const uint32_t words[4] = {c.x, c.y, c.z, c.w};
         // this lane's four output features: 16 rt + {2 t, 2 t + 1, 2 t + 8, 2 t + 9}
         float v[NT][4];
 #pragma unroll
@@ -357,11 +514,11 @@ q4_linear_dx_kernel(const Q4Args p) {
                 split_pair<TERMS>(v[nt][0] * s[0], v[nt][1] * s[1], b[nt][0]);
                 split_pair<TERMS>(v[nt][2] * s[2], v[nt][3] * s[3], b[nt][1]);
             }
-            const uint32_t sub_lo = zero_pair<M>(now.zeros[m] & 15u), sub_hi = zero_pair<M>((now.zeros[m] >> 8) & 15u);
+            const uint32_t sub_lo = zero_pair(now.zeros[m] & 15u), sub_hi = zero_pair((now.zeros[m] >> 8) & 15u);
 #pragma unroll
             for (int j = m * 4 / MINE; j < (m + 1) * 4 / MINE; j++) {
                 uint32_t w[4], wt[4];
-                unpack_word<M>(words[j], sub_lo, sub_hi, w);
+                unpack_centred(words[j], sub_lo, sub_hi, w);
                 // registers 0, 1 hold the lower pairs of rows 0-7, 8-15, registers 2, 3 the upper pairs; transposed, the
                 // features are the rows of the A operand and 1 and 2 change places
                 wt[0] = transpose8(w[0]); wt[1] = transpose8(w[2]); wt[2] = transpose8(w[1]); wt[3] = transpose8(w[3]);
@@ -369,21 +526,32 @@ q4_linear_dx_kernel(const Q4Args p) {
                 for (int nt = 0; nt < NT; nt++) {
                     float acc[4] = {};
 #pragma unroll
-                    for (int u = TERMS - 1; u >= 0; u--) Mma<M>::run(acc, wt, b[nt][0][u], b[nt][1][u]);
+                    for (int u = TERMS - 1; u >= 0; u--) mma<M>(acc, wt, b[nt][0][u], b[nt][1][u]);
 #pragma unroll
                     for (int i = 0; i < 4; i++) total[j][nt][i] += acc[i];
                 }
             }
         }
     }
+    __syncthreads();  // all queues are empty
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int i = 0; i < 4; i++) red[warp * E + ((j * NT + nt) * 4 + i) * 32 + lane] = total[j][nt][i];
+    __syncthreads();
+#pragma unroll
+    for (int e = threadIdx.x; e < E; e += WARPS * 32) {  // over the warps first
+        float v = red[e];
+#pragma unroll
+        for (int w = 1; w < WARPS; w++) v += red[w * E + e];
+        red[e] = v;
+    }
     T* out = (T*) p.out;
-    reduce_and_store<E>(red, rank, p.cluster, [&](int e, float val) {
+    cluster_arrive();
+    cluster_wait();
+    join<E, 1, WARPS>(red, rank, p.cluster, [&](int e, float val) {
         const int l = e & 31, i = (e >> 5) & 3, nt = (e >> 7) % NT, j = (e >> 7) / NT;
         // row a of the transposed matrix is the feature of lane group a / 2, element a & 1 of its pair; rows 8..15 are the upper pairs
         const int ar = l >> 2;
@@ -392,6 +560,8 @@ q4_linear_dx_kernel(const Q4Args p) {
         if (k >= p.w.K || row >= p.rows) return;
         out[row * p.ld_out + k] = from_float<T>(val);
     });
+    cluster_arrive();  // nobody leaves while its sums may still be read
+    cluster_wait();
 }
 
 // ------------------------------------------------------------------ quantising, packing, unpacking
@@ -557,10 +727,11 @@ int blocks_for(const char* who, long long threads, unsigned* out) {
 }
 
 template <typename K>
-int launch_clustered(K kernel, unsigned x, unsigned y, int cluster, const Q4Args& args, cudaStream_t s) {
+int launch_clustered(K kernel, unsigned x, unsigned y, int cluster, int warps, size_t smem, const Q4Args& args, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(x, y);
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3((unsigned) warps * 32);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -571,44 +742,83 @@ int launch_clustered(K kernel, unsigned x, unsigned y, int cluster, const Q4Args
     CAKE_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args));
     return CAKEB200_OK;
 }
-
-// CTAs per product along the reduction: enough of them that the machine holds a few per SM, each warp with at least one
-// block to do; a power of two up to the portable cluster size.
-int pick_cluster(long long ctas, int blocks, int sm_count) {
+// CTAs of a cluster that share out the reduction: at least `least`, and more while there are fewer than `wanted` CTAs and each
+// of the cluster's warps still has `per_warp` steps (block rows) of it.
+int pick_cluster(long long items, int depth, int warps, int per_warp, int least, long long wanted) {
     int c = 1;
-    while (c < MAX_CLUSTER && ctas * c < 4LL * sm_count && blocks >= 2 * c * WARPS) c *= 2;
+    while (c < MAX_CLUSTER && depth >= 2 * c * warps * per_warp && (c < least || items * c < wanted)) c *= 2;
     return c;
 }
 
-template <typename T, int NT, int R>
-int launch_linear_form(Q4Args& p, int sm_count, cudaStream_t s) {
-    const unsigned rbs = (unsigned) ((p.w.row_tiles + R - 1) / R), chunks = (unsigned) ((p.rows + 8 * NT - 1) / (8 * NT));
-    p.cluster = pick_cluster((long long) rbs * chunks, p.w.steps, sm_count);
-    const unsigned x = rbs * (unsigned) p.cluster;
-    if (p.w.group_shift == 7) return launch_clustered(q4_linear_kernel<T, NT, R, 1>, x, chunks, p.cluster, p, s);
-    if (p.w.group_shift == 6) return launch_clustered(q4_linear_kernel<T, NT, R, 2>, x, chunks, p.cluster, p, s);
-    return launch_clustered(q4_linear_kernel<T, NT, R, 4>, x, chunks, p.cluster, p, s);
+// The forward product runs CTAs of four warps, as many as fit, two or more to a cluster.  Times in us over warps per CTA x CTAs per
+// cluster x CTAs per SM, one row: 16384 x 16384 FP32 4x1x4 90, 4x2x4 79, 8x1x2 89, 8x2x2 77, 8x4x2 133; 16384 x 8192 BF16
+// 4x1x4 33, 4x2x4 30, 4x2x5 27, 8x1x2 33, 8x2x2 30; 4096 x 4096 FP16 4x1 9.1, 4x2 7.2, 4x4 6.5; 2048 x 2048 BF16 4x1 6.4,
+// 4x2 4.8, 4x4 4.7.
+constexpr int LINEAR_WARPS = 4;
+
+// One wave: as many clusters as the device holds of this kernel (asked once per device and cluster size), or one per item.
+template <typename T, int NT, int R, int GROUPS>
+int launch_linear_as(Q4Args& p, long long items, int device, cudaStream_t s) {
+    static std::atomic<int> known[64][4];  // by device and log2 of the cluster size
+    const auto kernel = q4_linear_kernel<T, NT, R, GROUPS, LINEAR_WARPS>;
+    constexpr size_t smem = (size_t) LINEAR_WARPS * (AHEAD * R * 1024 + 2 * R * NT * 512);
+    const int log2 = p.cluster == 1 ? 0 : p.cluster == 2 ? 1 : p.cluster == 4 ? 2 : 3;
+    int fit = device < 64 ? known[device][log2].load() : 0;
+    if (fit == 0) {
+        CAKE_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned) p.cluster);
+        cfg.blockDim = dim3(LINEAR_WARPS * 32);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned) p.cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        CAKE_CUDA_OK(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
+        if (fit < 1) {
+            set_error("q4_linear: the kernel does not fit the device");
+            return CAKEB200_ERR_CUDA;
+        }
+        if (device < 64) known[device][log2] = fit;
+    }
+    const unsigned grid = (unsigned) (std::min<long long>(items, fit) * p.cluster);
+    return launch_clustered(kernel, grid, 1, p.cluster, LINEAR_WARPS, smem, p, s);
+}
+template <typename T, int NT>
+int launch_linear_rows(Q4Args& p, const DeviceState* st, cudaStream_t s) {
+    constexpr int R = 2;
+    p.chunks = (p.rows + 8 * NT - 1) / (8 * NT);
+    const long long items = (long long) (p.w.row_tiles / R) * p.chunks;
+    p.cluster = pick_cluster(items, p.w.steps, LINEAR_WARPS, 1, 2, 2LL * st->sm_count);
+    if (p.w.group_shift == 7) return launch_linear_as<T, NT, R, 1>(p, items, st->device, s);
+    if (p.w.group_shift == 6) return launch_linear_as<T, NT, R, 2>(p, items, st->device, s);
+    return launch_linear_as<T, NT, R, 4>(p, items, st->device, s);
 }
 template <typename T>
-int launch_linear(Q4Args& p, int sm_count, cudaStream_t s) {
-    if (p.rows <= 8) return launch_linear_form<T, 1, 2>(p, sm_count, s);
-    if (p.rows <= 16) return launch_linear_form<T, 2, 2>(p, sm_count, s);
-    return launch_linear_form<T, 4, 2>(p, sm_count, s);
+int launch_linear(Q4Args& p, const DeviceState* st, cudaStream_t s) {
+    if (p.rows <= 8) return launch_linear_rows<T, 1>(p, st, s);
+    if (p.rows <= 16) return launch_linear_rows<T, 2>(p, st, s);
+    return launch_linear_rows<T, 4>(p, st, s);
 }
 
+// The gradient's CTAs have eight warps and one block of 64 input features each.  us over warps per CTA x CTAs per cluster, one row:
+// 16384 x 8192 BF16 4x1 183, 4x4 58, 8x1 100, 8x4 52, 8x8 52; 4096 x 4096 FP32 4x1 34, 8x4 10.1, 8x8 10.5; 2048 x 2048 FP32
+// 8x1 11.3, 8x4 5.6, 8x8 5.0.
+constexpr int DX_WARPS = 8;
 template <typename T, int NT>
-int launch_dx_form(Q4Args& p, int sm_count, cudaStream_t s) {
+int launch_dx_rows(Q4Args& p, int sm_count, cudaStream_t s) {
     const unsigned blocks = 2u * (unsigned) p.w.steps, chunks = (unsigned) ((p.rows + 8 * NT - 1) / (8 * NT));
-    p.cluster = pick_cluster((long long) blocks * chunks, p.w.row_tiles, sm_count);
+    p.cluster = pick_cluster((long long) blocks * chunks, p.w.row_tiles, DX_WARPS, 1, 1, 4LL * sm_count);
     const unsigned x = blocks * (unsigned) p.cluster;
-    if (p.w.group_shift == 7) return launch_clustered(q4_linear_dx_kernel<T, NT, 1>, x, chunks, p.cluster, p, s);
-    if (p.w.group_shift == 6) return launch_clustered(q4_linear_dx_kernel<T, NT, 2>, x, chunks, p.cluster, p, s);
-    return launch_clustered(q4_linear_dx_kernel<T, NT, 4>, x, chunks, p.cluster, p, s);
+    if (p.w.group_shift == 7) return launch_clustered(q4_linear_dx_kernel<T, NT, 1, DX_WARPS>, x, chunks, p.cluster, DX_WARPS, 0, p, s);
+    if (p.w.group_shift == 6) return launch_clustered(q4_linear_dx_kernel<T, NT, 2, DX_WARPS>, x, chunks, p.cluster, DX_WARPS, 0, p, s);
+    return launch_clustered(q4_linear_dx_kernel<T, NT, 4, DX_WARPS>, x, chunks, p.cluster, DX_WARPS, 0, p, s);
 }
 template <typename T>
 int launch_dx(Q4Args& p, int sm_count, cudaStream_t s) {
-    if (p.rows <= 8) return launch_dx_form<T, 1>(p, sm_count, s);
-    return launch_dx_form<T, 2>(p, sm_count, s);
+    return p.rows <= 8 ? launch_dx_rows<T, 1>(p, sm_count, s) : launch_dx_rows<T, 2>(p, sm_count, s);
 }
 
 // Common checks of the two products.  in_cols / out_cols: row lengths of the operand and of the result.
@@ -644,8 +854,8 @@ int product(const char* who, const cakeb200_q4* w, const void* in, long long ld_
         rc = type == CAKEB200_F32 ? launch_dx<float>(p, st->sm_count, s)
              : type == CAKEB200_F16 ? launch_dx<__half>(p, st->sm_count, s) : launch_dx<__nv_bfloat16>(p, st->sm_count, s);
     else
-        rc = type == CAKEB200_F32 ? launch_linear<float>(p, st->sm_count, s)
-             : type == CAKEB200_F16 ? launch_linear<__half>(p, st->sm_count, s) : launch_linear<__nv_bfloat16>(p, st->sm_count, s);
+        rc = type == CAKEB200_F32 ? launch_linear<float>(p, st, s)
+             : type == CAKEB200_F16 ? launch_linear<__half>(p, st, s) : launch_linear<__nv_bfloat16>(p, st, s);
     if (!rc) thread_stats()->launches = 1;
     return rc;
 }

@@ -35,7 +35,7 @@ struct Q4View {
     int scale_bf16;
 };
 
-inline __host__ __device__ int q4_row_tiles(int N) { return (N + 15) / 16; }
+inline __host__ __device__ int q4_row_tiles(int N) { return (N + 31) / 32 * 2; }  // in pairs, as the forward product takes them
 inline __host__ __device__ int q4_steps(int K) { return (K + 127) / 128; }
 // Place of the scale of local row i (0..15) of a block row for the group that holds feature k of its step (0..127).
 inline __host__ __device__ int q4_scale_place(int i, int k, int group_shift) {
@@ -64,16 +64,15 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // v = t0 + t1 + ... with every term a bf16 (the upper half of an FP32), by truncation; a pair of values at a time.
-// An infinite value has only its first term (inf - inf would make the sum NaN where the product is infinite).
+// Terms of a value that is not finite are not all finite.
 template <int TERMS>
 __device__ __forceinline__ void split_pair(float v0, float v1, uint32_t* out) {
 #pragma unroll
     for (int t = 0; t < TERMS; t++) {
         out[t] = __byte_perm(__float_as_uint(v0), __float_as_uint(v1), 0x7632);
         if (t + 1 < TERMS) {
-            const float h0 = __uint_as_float(__float_as_uint(v0) & 0xffff0000u), h1 = __uint_as_float(__float_as_uint(v1) & 0xffff0000u);
-            v0 = (t == 0 && isinf(v0)) ? 0.f : v0 - h0;
-            v1 = (t == 0 && isinf(v1)) ? 0.f : v1 - h1;
+            v0 -= __uint_as_float(__float_as_uint(v0) & 0xffff0000u);
+            v1 -= __uint_as_float(__float_as_uint(v1) & 0xffff0000u);
         }
     }
 }

@@ -188,7 +188,7 @@ int run(const Q4View& w, const void* in, long long ld_in, const void* bias, void
         Planes p = m.w;
         (dx ? p.cols : p.rows) = n;
         p.ld = plane::padded(p.cols);
-        const int rt0 = dx ? 0 : c0 / 16, rts = q4_row_tiles(p.rows), kb0 = dx ? c0 / 64 : 0, kbs = (p.cols + 63) / 64;
+        const int rt0 = dx ? 0 : c0 / 16, rts = (p.rows + 15) / 16, kb0 = dx ? c0 / 64 : 0, kbs = (p.cols + 63) / 64;
         expand_kernel<K::W><<<(unsigned) (((long long) rts * kbs * 32 + 255) / 256), 256, 0, s>>>(w, rt0, rts, kb0, kbs, p);
         CAKE_CUDA_OK(cudaGetLastError());
         *launches += 1;

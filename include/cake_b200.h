@@ -430,7 +430,8 @@ int cakeb200_unpack_B(float* B, const float* B_p, int K, int N, int p, const cak
  * are multiplied with the weights as they are, the scales applied in FP32; for many rows the weights are expanded first, a
  * slab at a time: exactly for FP32, to 17 bits for FP16, rounded once to BF16 for BF16.  _workspace tells how many bytes
  * of device memory, on a 1024-byte boundary, the call needs for that (0 for few rows: workspace may then be NULL); two
- * calls that may overlap on the GPU need one each.  The result must not overlap the operands.  `rows` may be 0.  Device
+ * calls that may overlap on the GPU need one each.  A row with an infinity or a NaN gives results
+ * that are not finite, and does not touch other rows.  The result must not overlap the operands.  `rows` may be 0.  Device
  * pointers of the current device only; work is enqueued on `stream`.  Results do not depend on timing.  Waits inside the
  * kernels are bounded; one that gave up shows in the status of the next blocking product (cakeb200_sgemm). */
 typedef struct cakeb200_q4 {

@@ -184,8 +184,8 @@ def test_values_that_are_not_finite_stay_in_their_row(cake, dtype):
         clean = cake.cake_q4_linear(x, W4)
         x[1, 7], x[2, 149] = float("inf"), float("nan")
         y = cake.cake_q4_linear(x, W4)
-        # (with many rows an infinity also meets the zeros of the weights' second plane)
-        assert bool((y[1] == float("inf")).all() if rows < 65 else (~torch.isfinite(y[1])).all()) and bool(torch.isnan(y[2]).all())
+        # (an infinity meets itself where offsets or second planes are taken out again, so what comes of it may be a NaN)
+        assert bool((~torch.isfinite(y[1])).all()) and bool(torch.isnan(y[2]).all())
         keep = [r for r in range(rows) if r not in (1, 2)]
         assert torch.equal(y[keep], clean[keep])
 

@@ -18,9 +18,9 @@ def _q4(packed=0x10000, n=32, k=64, group=64, scale=1, zeros=0):
 
 def test_q4_sizes(cake):
     L = cake.lib()
-    # 16 x 128 blocks of 1024 bytes, 16 scales (2 bytes) and zero points (1 byte) per block row and group
-    assert L.cakeb200_q4_packed_bytes(16, 64, 64, 0) == 1024 + 2 * 32
-    assert L.cakeb200_q4_packed_bytes(17, 129, 32, 1) == 2 * 2 * 1024 + 2 * 8 * 16 * 3
+    # pairs of 16 x 128 blocks of 1024 bytes, 16 scales (2 bytes) and zero points (1 byte) per block row and group
+    assert L.cakeb200_q4_packed_bytes(16, 64, 64, 0) == 2 * (1024 + 2 * 32)
+    assert L.cakeb200_q4_packed_bytes(33, 129, 32, 1) == 4 * 2 * 1024 + 4 * 8 * 16 * 3
     assert L.cakeb200_q4_packed_bytes(16384, 16384, 128, 0) == 16384 * 16384 // 2 + 16384 * 128 * 2
     for bad in ((0, 64, 64, 0), (16, 0, 64, 0), (16, 64, 48, 0), (16, -1, 64, 0), (2 ** 30 + 1, 64, 64, 0)):
         assert L.cakeb200_q4_packed_bytes(*bad) == 0
