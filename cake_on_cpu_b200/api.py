@@ -756,16 +756,35 @@ class Q4Weights:
             _need_shape(zeros, (self.out_features, groups), "zeros")
             if not torch.cuda.is_current_stream_capturing() and int(zeros.max()) > 15:
                 raise ValueError("zero points are 0..15")
-        self.device = codes.device
+        self.device, self.has_zeros = codes.device, zeros is not None
         n = lib().cakeb200_q4_packed_bytes(self.out_features, self.in_features, self.group, int(zeros is not None))
         with _on_device(self.device, stream) as s:
             self.packed = torch.empty(n, dtype=torch.uint8, device=self.device)
-            self._c = _Q4(self.packed.data_ptr(), self.out_features, self.in_features, self.group, self.scale_type, int(zeros is not None))
-            self._ref = ctypes.byref(self._c)
-            self._workspace = {}  # bytes needed by (rows, type, gradient)
+            self._bind()
             _check(lib().cakeb200_q4_pack(_vp(codes.data_ptr()), codes.stride(0), _vp(scales.data_ptr()),
                                           _vp(zeros.data_ptr()) if zeros is not None else None, self.out_features, self.in_features,
                                           self.group, self.scale_type, _vp(self.packed.data_ptr()), s))
+
+    @classmethod
+    def from_packed(cls, packed, out_features, in_features, group, scale_type, has_zeros):
+        """The weights whose packed form (the ``packed`` tensor of another object of that geometry) is given."""
+        n = lib().cakeb200_q4_packed_bytes(out_features, in_features, group, int(has_zeros))
+        import torch
+        if not (_is_torch(packed) and packed.is_cuda and packed.dtype == torch.uint8 and packed.is_contiguous()):
+            raise TypeError("packed weights are a contiguous uint8 CUDA tensor")
+        if n == 0:
+            _check(-1)
+        _need_shape(packed, (n,), "packed")
+        self = object.__new__(cls)
+        self.out_features, self.in_features, self.group, self.scale_type = int(out_features), int(in_features), int(group), int(scale_type)
+        self.has_zeros, self.device, self.packed = bool(has_zeros), packed.device, packed
+        self._bind()
+        return self
+
+    def _bind(self):
+        self._c = _Q4(self.packed.data_ptr(), self.out_features, self.in_features, self.group, self.scale_type, int(self.has_zeros))
+        self._ref = ctypes.byref(self._c)
+        self._workspace = {}  # bytes needed by (rows, type, gradient)
 
     @staticmethod
     def quantize_codes(W, group=128, symmetric=True, scale_dtype=None, stream=None):

@@ -8,6 +8,9 @@ handed device pointers, transposed operands are read where they lie (the weight
 of the forward product and dY of the weight gradient; the reference makes
 contiguous transposed copies at src/linear.cpp:22 and :76-80) and the bias is
 added in the product's epilogue instead of a second pass (:44-46).
+
+Around the layer: ``cake_muon``, an optimiser that moves its weight by orthogonalised updates, and
+``cake_linear_q4``, the layer with its weight held in 4 bits.
 """
 import os
 
@@ -95,3 +98,87 @@ class cake_linear(nn.Module):
 
     def forward(self, data):
         return cake_linear_function.apply(data, self.weight, self.bias)
+
+
+class cake_linear_q4_function(torch.autograd.Function):
+    """y = x W^T + b with W a ``Q4Weights``, and its gradients for x and b; the 4-bit weight itself has none."""
+
+    @staticmethod
+    def forward(ctx, data, weights, bias=None):
+        ctx.weights, ctx.has_bias = weights, bias is not None
+        return api.cake_q4_linear(data, weights, bias)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        dy = grad_output if grad_output.is_contiguous() else grad_output.contiguous()
+        gi = api.cake_q4_linear_dx(dy, ctx.weights) if ctx.needs_input_grad[0] else None
+        gb = None
+        if ctx.has_bias and ctx.needs_input_grad[2]:
+            gb = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(dy.dtype)
+        return gi, None, gb
+
+
+class cake_linear_q4(nn.Module):
+    """``cake_linear`` with its weight in 4 bits: for serving, and for training what lies in front of it.  The packed weight is a
+    buffer (it moves with the module and is part of its state), the bias a parameter of the type of the activations."""
+
+    def __init__(self, weights, bias=None):
+        super().__init__()
+        if not isinstance(weights, api.Q4Weights):
+            raise TypeError("the weights must be a Q4Weights object")
+        self.input_features, self.output_features = weights.in_features, weights.out_features
+        self._geometry = (weights.out_features, weights.in_features, weights.group, weights.scale_type, weights.has_zeros)
+        self.register_buffer("packed", weights.packed)
+        self._weights = weights
+        if bias is None:
+            self.register_parameter("bias", None)
+        else:
+            self.bias = Parameter(bias.detach().clone())
+
+    @classmethod
+    def from_linear(cls, layer, group=128, symmetric=True, scale_dtype=None):
+        """The 4-bit form of a layer with ``weight`` (out_features, in_features) and ``bias``."""
+        return cls(api.Q4Weights.quantize(layer.weight.detach(), group, symmetric, scale_dtype), layer.bias)
+
+    @property
+    def weights(self):
+        if self._weights.packed is not self.packed:  # moved, or loaded
+            self._weights = api.Q4Weights.from_packed(self.packed, *self._geometry)
+        return self._weights
+
+    def forward(self, data):
+        return cake_linear_q4_function.apply(data, self.weights, self.bias)
+
+
+class cake_muon(torch.optim.Optimizer):
+    """Steps weight matrices along the orthogonalisation of their momentum (``cake_muon_step``).  Takes matrices in float32 or
+    bfloat16 on the GPU; the momentum is kept in float32.  ``scale`` None: sqrt(max(1, rows / cols)) of each matrix."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5, coeffs=api.NS_COEFFS, eps=1e-7):
+        if lr < 0 or not 0 <= momentum <= 1 or weight_decay < 0:
+            raise ValueError("lr and weight_decay are not negative, momentum lies between 0 and 1")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, scale=scale, steps=steps,
+                                      coeffs=tuple(coeffs), eps=eps))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() != 2:
+                    raise ValueError("cake_muon takes matrices; give other parameters to another optimiser")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("cake_muon takes dense gradients")
+                state = self.state[p]
+                if "momentum" not in state:
+                    state["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                api.cake_muon_step(p, _rows(p.grad), state["momentum"], group["lr"], group["momentum"], group["nesterov"], group["weight_decay"],
+                                   group["scale"], group["steps"], group["coeffs"], group["eps"])
+        return loss

@@ -1,0 +1,119 @@
+"""The operators on a linear layer's weight as a program uses them: two layers trained with cake_muon, then held in 4 bits and
+asked token by token."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _orthogonal(u):
+    x = u / (np.linalg.norm(u) + 1e-7)
+    tall = x.shape[0] > x.shape[1]
+    x = x.T if tall else x
+    for _ in range(5):
+        p = x @ x.T
+        x = 3.4445 * x + (-4.7750 * p + 2.0315 * (p @ p)) @ x
+    return x.T if tall else x
+
+
+def test_train_then_serve(cake):
+    """Three steps of two layers against the same steps in float64, then the same layers in 4 bits: rows of a batch one by one
+    give what the batch gives, and both what the dequantised weights give."""
+    import torch
+    from cake_on_cpu_b200.cake import cake_linear, cake_linear_q4, cake_muon
+    torch.manual_seed(3)
+    first, second = cake_linear(96, 200).cuda(), cake_linear(200, 64).cuda()
+    opt = cake_muon([first.weight, second.weight], lr=0.05, weight_decay=0.01)
+    x, t = torch.randn(150, 96, device="cuda"), torch.randn(150, 64, device="cuda")
+    w = [first.weight.detach().double().cpu().numpy(), second.weight.detach().double().cpu().numpy()]
+    b = [first.bias.detach().double().cpu().numpy(), second.bias.detach().double().cpu().numpy()]
+    m = [np.zeros_like(v) for v in w]
+    x64, t64 = x.double().cpu().numpy(), t.double().cpu().numpy()
+    for _ in range(3):
+        opt.zero_grad()
+        ((second(torch.tanh(first(x))) - t) ** 2).mean().backward()
+        opt.step()
+        h = np.tanh(x64 @ w[0].T + b[0])
+        d = 2 * (h @ w[1].T + b[1] - t64) / t64.size
+        grads = [((d @ w[1]) * (1 - h * h)).T @ x64, d.T @ h]
+        for i in range(2):
+            m[i] = 0.95 * m[i] + 0.05 * grads[i]
+            w[i] = (1 - 0.05 * 0.01) * w[i] - 0.05 * max(1, w[i].shape[0] / w[i].shape[1]) ** 0.5 * _orthogonal(0.95 * m[i] + 0.05 * grads[i])
+    for layer, want in zip((first, second), w):
+        # a gradient in FP32 is off by some 2^-20; small singular directions of it come out 480 times as large, in every step
+        assert np.linalg.norm(layer.weight.detach().double().cpu().numpy() - want) <= 3 * 0.05 * 480 * 2.0 ** -20 * want.shape[0] ** 0.5
+
+    served = [cake_linear_q4.from_linear(layer, group=32, symmetric=False) for layer in (first, second)]
+    with torch.no_grad():
+        y = served[1](torch.tanh(served[0](x)))
+        d = [s.weights.dequantize().double() for s in served]
+        want = torch.tanh(x.double() @ d[0].T + first.bias.double()) @ d[1].T + second.bias.double()
+        # two products of FP32 sums with 96 and 200 terms, tanh's slope is at most one
+        assert float((y.double() - want).abs().max()) <= 2.0 ** -18 * float((d[1].abs().sum(1)).max())
+        for i in (0, 77, 149):
+            one = served[1](torch.tanh(served[0](x[i])))
+            assert float((one.double() - want[i]).abs().max()) <= 2.0 ** -18 * float((d[1].abs().sum(1)).max())
+        # half a step of the codes, one with the rounding of the zero point
+        for s, layer in zip(served, (first, second)):
+            worst = (layer.weight.detach().amax(1) - layer.weight.detach().amin(1)) / 15
+            assert float(((s.weights.dequantize() - layer.weight.detach()).abs() / worst[:, None]).max()) <= 1.02
+
+
+@pytest.mark.parametrize("rows", [3, 100])
+def test_gradients_through_a_frozen_layer(cake, rows):
+    """d(loss)/dx and d(loss)/db against the formula and against differences of the layer's own output."""
+    import torch
+    from cake_on_cpu_b200.cake import cake_linear, cake_linear_q4
+    torch.manual_seed(rows)
+    layer = cake_linear_q4.from_linear(cake_linear(130, 70).cuda(), group=64)
+    x = torch.randn(2, rows, 130, device="cuda", requires_grad=True)
+    c = torch.randn(2, rows, 70, device="cuda")
+    (layer(x) * c).sum().backward()
+    w = layer.weights.dequantize().double()
+    S = c.double().abs() @ w.abs()
+    assert bool(((x.grad.double() - c.double() @ w).abs() <= 2.0 ** -18 * S).all())  # 70 products in FP32
+    want = c.double().sum((0, 1))
+    assert bool(((layer.bias.grad.double() - want).abs() <= 2.0 ** -18 * c.double().abs().sum((0, 1))).all())
+    # the layer is linear in x, so a central difference has no error but that of the outputs, 2^-18 of their terms, over the step
+    step, where = 0.5, (1, rows // 2, 77)
+    e = torch.zeros_like(x)
+    e[where] = step
+    with torch.no_grad():
+        diff = float(((layer(x + e).double() - layer(x - e).double()) * c.double()).sum()) / (2 * step)
+        terms = (x.detach().double().abs() + step) @ w.abs().T + layer.bias.detach().double().abs()
+    assert abs(diff - float(x.grad[where])) <= 2 * 2.0 ** -18 * float((terms * c.double().abs())[where[0], where[1]].sum()) / (2 * step) + 1e-4 * abs(diff)
+    # no gradient wanted: none computed
+    y = layer(torch.randn(4, 130, device="cuda"))
+    y.sum().backward()
+
+
+def test_module_moves_and_reloads(cake):
+    import torch
+    from cake_on_cpu_b200.cake import cake_linear, cake_linear_q4
+    a, b = (cake_linear_q4.from_linear(cake_linear(64, 48).cuda(), group=32) for _ in range(2))
+    x = torch.randn(5, 64, device="cuda")
+    assert not torch.equal(a(x), b(x))
+    b.load_state_dict(a.state_dict())
+    assert torch.equal(a(x), b(x))
+    c = b.cpu().cuda()
+    assert torch.equal(c(x), a(x))
+
+
+def test_muon_refuses_what_is_not_a_matrix(cake):
+    import torch
+    from cake_on_cpu_b200.cake import cake_muon
+    with pytest.raises(ValueError):
+        cake_muon([torch.nn.Parameter(torch.zeros(4, device="cuda"))])
+    with pytest.raises(ValueError):
+        cake_muon([torch.nn.Parameter(torch.zeros(4, 4, device="cuda"))], momentum=1.5)
+    p = torch.nn.Parameter(torch.randn(6, 9, device="cuda"))
+    q = torch.nn.Parameter(torch.randn(6, 9, device="cuda"))
+    opt = cake_muon([p, q], lr=0.1)
+    keep = q.detach().clone()
+    (p * 2).sum().backward()
+    opt.step()  # q has no gradient and stays
+    assert torch.equal(q.detach(), keep) and opt.state[p]["momentum"].dtype == torch.float32
+    # a gradient that is stored by columns
+    p.grad = torch.randn(9, 6, device="cuda").t()
+    opt.step()
+    assert bool(torch.isfinite(p).all())
