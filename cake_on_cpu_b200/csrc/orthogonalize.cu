@@ -191,12 +191,18 @@ struct ResultEpilogue {
         int rows, cols;
         float f;
     };
-    static __device__ __forceinline__ void block(const Args& a, const TileAt& at, const float* v, uint32_t* patch, int lane) {
-        T* p = a.out.base + at.batch * a.out.stride + at.row * a.out.ld + at.col + lane;
-        const int rows = at.col + lane < a.cols ? a.rows - at.row : 0;
-        plane::by_rows(v, patch, lane, [&](int r, float x) {
-            if (r < rows) put(p + r * a.out.ld, a.f * x);
-        });
+    // one value of the block's row r, in the lane's column of it
+    struct Writer {
+        T* p;
+        long long ld;
+        int rows;
+        float f;
+        __device__ __forceinline__ void operator()(int r, float x) const {
+            if (r < rows) put(p + r * ld, f * x);
+        }
+    };
+    static __device__ __forceinline__ Writer writer(const Args& a, const TileAt& at, int lane) {
+        return {a.out.base + at.batch * a.out.stride + at.row * a.out.ld + at.col + lane, a.out.ld, at.col + lane < a.cols ? a.rows - at.row : 0, a.f};
     }
 };
 
@@ -208,12 +214,17 @@ struct StepEpilogue {
         int rows, cols;
         float f, keep, step;
     };
-    static __device__ __forceinline__ void block(const Args& a, const TileAt& at, const float* v, uint32_t* patch, int lane) {
-        T* p = a.w.base + at.row * a.w.ld + at.col + lane;
-        const int rows = at.col + lane < a.cols ? a.rows - at.row : 0;
-        plane::by_rows(v, patch, lane, [&](int r, float x) {
-            if (r < rows) put(p + r * a.w.ld, a.keep * get(p + r * a.w.ld) - a.step * (a.f * x));
-        });
+    struct Writer {
+        T* p;
+        long long ld;
+        int rows;
+        float f, keep, step;
+        __device__ __forceinline__ void operator()(int r, float x) const {
+            if (r < rows) put(p + r * ld, keep * get(p + r * ld) - step * (f * x));
+        }
+    };
+    static __device__ __forceinline__ Writer writer(const Args& a, const TileAt& at, int lane) {
+        return {a.w.base + at.row * a.w.ld + at.col + lane, a.w.ld, at.col + lane < a.cols ? a.rows - at.row : 0, a.f, a.keep, a.step};
     }
 };
 
@@ -348,7 +359,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
             auto finish = [&](const TileAt& at, const float* v) {
                 if (at.row >= g.rows || at.col >= g.cols) return;
                 if (kind == 3) {
-                    Last::block(last, at, v, (uint32_t*) e.patch, e.lane);
+                    plane::by_rows(v, (uint32_t*) e.patch, e.lane, Last::writer(last, at, e.lane));
                     return;
                 }
                 plane::by_eights(v, (uint32_t*) e.patch, e.lane, [&](int r, int col, float* u) {
@@ -400,6 +411,344 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
         }
     }
     e.close();
+}
+
+// ------------------------------------------------------------------ matrices that fit into the shared memory of a cluster
+
+// X of at most 128 rows and 256 columns per CTA of a cluster stays in shared memory from the first step to the last, as planes
+// in the layout that the MMAs read; one launch does a whole batch, a cluster per matrix, and memory is touched to read G and
+// to write the result.  The grid-wide barriers, stores and loads between products are what small matrices spend their time
+// on otherwise (five steps, FP32: 12 x 96 x 960 188 us in the chain above, 64 here; 1 x 64 x 64 133 and 29).
+//
+// A step of CTA k, which holds the columns X_k:
+//     X_k X_k^T on its own; the parts of P are exchanged: every CTA adds up 128 / cluster rows of all parts, in order of the
+//     CTAs, and sends them as planes to all;
+//     Q = a I + b P + c P P, by every CTA for itself;
+//     X_k <- Q X_k, with the planes of X_k read down their columns.
+// The sixteen warps share the 128 x 128 results in 32 x 32 blocks; one thread issues the MMAs of a product, all wait for it.
+// Products, blocks and the exchange stop at the rows and columns that there are, rounded up to 32.
+constexpr int SMALL_THREADS = 512, SMALL_ROWS = 128, SMALL_COLUMNS = 256, SMALL_CLUSTER = 8;
+constexpr int SUB_BYTES = 128 * 128;          // 128 rows of 64 values, 128-byte swizzled
+constexpr int SQUARE_BYTES = 2 * TERMS * SUB_BYTES;  // planes of 128 x 128 values: [plane][64 columns]
+constexpr int HALF_PATCH = 16 * 128;          // 16 rows of 32 FP32
+constexpr int SMALL_SMEM = 1024 + 2 * SQUARE_BYTES + SQUARE_BYTES + 16 * HALF_PATCH + 512;
+static_assert(SMALL_SMEM <= plane::MAX_SMEM, "X, P and the patches fit");
+static_assert(SQUARE_BYTES + 16 * HALF_PATCH >= 16 * plane::PATCH_FLOATS * 4, "the patches of the result lie where P and the others were");
+
+struct Small {
+    int m, n, tall, batch, steps, cluster, slice;  // slice: columns of X per CTA
+    float eps, f0, ka, kb, kc;
+    double up;
+    int* status_word;
+};
+
+// byte offset of row r, column c (of 128) in a plane of a square
+__device__ __forceinline__ uint32_t square_at(int r, int c) { return (uint32_t) ((c >> 6) * SUB_BYTES + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2); }
+
+// 32 consecutive values (columns c0 ...) of row r of a square, from FP32 and back
+__device__ __forceinline__ void put_row(uint8_t* square, int r, int c0, const float* value) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = value[8 * q + e];
+#pragma unroll
+        for (int t = 0; t < TERMS; t++) {
+            uint4 o;
+            o.x = Fp16Planes::next(v[0], v[1]); o.y = Fp16Planes::next(v[2], v[3]);
+            o.z = Fp16Planes::next(v[4], v[5]); o.w = Fp16Planes::next(v[6], v[7]);
+            *reinterpret_cast<uint4*>(square + t * 2 * SUB_BYTES + square_at(r, c0 + 8 * q)) = o;
+        }
+    }
+}
+__device__ __forceinline__ void get_row(const uint8_t* square, int r, int c0, float* v) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const uint4 h = *reinterpret_cast<const uint4*>(square + square_at(r, c0 + 8 * q)), l = *reinterpret_cast<const uint4*>(square + 2 * SUB_BYTES + square_at(r, c0 + 8 * q));
+        const uint32_t hi[4] = {h.x, h.y, h.z, h.w}, lo[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float2 a = Fp16Planes::value(hi[e]), b = Fp16Planes::value(lo[e]);
+            v[8 * q + 2 * e] = fmaf(b.x, 1.f / Fp16Planes::TERM, a.x);
+            v[8 * q + 2 * e + 1] = fmaf(b.y, 1.f / Fp16Planes::TERM, a.y);
+        }
+    }
+}
+
+// D(main) = A B, D(cross) (+)= its two smaller products: squares a and b, b along its rows or down its columns; n columns of
+// the result, `depth` of K, both multiples of 32
+__device__ __forceinline__ void square_product(uint32_t main, uint32_t cross, uint32_t a, uint32_t b, bool down, bool more, int n, int depth) {
+    const uint32_t idesc = plane::idesc_16(Fp16Planes::FORMAT, 128, n) | (down ? 1u << 16 : 0u);
+    // down: 64 columns further is a sub-tile (leading offset), 16 rows of K are 2048 bytes; along: 16 of K are 32 bytes, 64 a sub-tile
+    const uint64_t da = ptx::make_kmajor_sw128_desc(a), db = ptx::make_kmajor_sw128_desc(b) + (down ? (uint64_t) ((SUB_BYTES >> 4) - 1) << 16 : 0);
+#pragma unroll 1
+    for (int k = 0; k < depth / 16; k++) {
+        const uint32_t ka = (uint32_t) ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4, kb = down ? (uint32_t) (k * 2048) >> 4 : ka;
+        const uint32_t plane = 2 * SUB_BYTES >> 4, first = more || k > 0;
+        plane::umma<false>(cross, da + plane + ka, db + kb, idesc, first);
+        plane::umma<false>(cross, da + ka, db + plane + kb, idesc, 1u);
+        plane::umma<false>(main, da + ka, db + kb, idesc, k > 0);
+    }
+}
+
+__device__ __forceinline__ uint32_t remote(uint32_t local, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+    return r;
+}
+
+template <typename T, class Last>
+__global__ void __launch_bounds__(SMALL_THREADS, 1)
+small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* x = (uint8_t*) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);  // one or two squares
+    uint8_t* square = x + 2 * SQUARE_BYTES;                                     // P, Q, and the parts of P
+    uint8_t* patches = square + SQUARE_BYTES;
+    double* sums = (double*) (patches + 16 * HALF_PATCH);                       // per warp, then per CTA
+    uint64_t* bar = (uint64_t*) (sums + 32);
+    uint32_t* tmem_slot = (uint32_t*) (bar + 1);
+    volatile int* abort_flag = (volatile int*) (tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = p.cluster > 1 ? (int) ptx::cluster_ctarank() : 0, batch = (int) blockIdx.x / p.cluster;
+    const int c0 = rank * p.slice, columns = max(0, min(p.slice, p.n - c0)), squares = p.slice > 128 ? 2 : 1;
+    const uint32_t done = ptx::smem_u32(bar);
+    auto meet = [&]() {  // all CTAs of the cluster
+        if (p.cluster > 1) ptx::cluster_sync_all();
+        else __syncthreads();
+    };
+
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(done, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) ptx::tmem_alloc<false>(ptx::smem_u32(tmem_slot), 512);
+    // the source: X's columns [c0, c0 + columns) are eights along rows of G, or rows of G where X is its transpose
+    const int lines = p.tall ? columns : p.m, eights = ((p.tall ? p.m : columns) + 7) / 8, row0 = p.tall ? c0 : 0, col0 = p.tall ? 0 : c0;
+    double sum = 0;
+    for (int i = threadIdx.x; i < lines * eights; i += SMALL_THREADS) {
+        const int r = i / eights, c = (i - r * eights) * 8;
+        float v[8];
+        source8<T, true>(s, batch, row0 + r, col0 + c, v);
+        const int have = min(8, (p.tall ? p.m : columns) - c);  // the last eight may reach into the next CTA's columns
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < have) sum += (double) v[e] * v[e];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[warp] = sum;
+    for (uint4* z = (uint4*) x + threadIdx.x; z < (uint4*) (x + squares * SQUARE_BYTES); z += SMALL_THREADS) *z = make_uint4(0, 0, 0, 0);
+    ptx::tcgen05_fence_before();
+    meet();
+    ptx::tcgen05_fence_after();
+    if (threadIdx.x < p.cluster) {
+        sum = 0;
+        for (int w = 0; w < 16; w++) sum += sums[w];
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote(ptx::smem_u32(sums + 16 + rank), (int) threadIdx.x)), "d"(sum) : "memory");
+    }
+    meet();
+    sum = 0;
+    for (int k = 0; k < p.cluster; k++) sum += sums[16 + k];
+    const double inverse = p.up / (sqrt(sum) + (double) p.eps);
+    const uint32_t tmem = *tmem_slot;
+
+    for (int i = threadIdx.x; i < lines * eights; i += SMALL_THREADS) {
+        const int r = i / eights, c = (i - r * eights) * 8;
+        const int have = min(8, (p.tall ? p.m : columns) - c);
+        float v[8];
+        source8<T, false>(s, batch, row0 + r, col0 + c, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = e < have ? (float) ((double) v[e] * inverse) : 0.f;
+        if (!p.tall) {
+            uint8_t* to = x + (c >> 7) * SQUARE_BYTES + square_at(r, c & 127);
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
+                uint4 o;
+                o.x = Fp16Planes::next(v[0], v[1]); o.y = Fp16Planes::next(v[2], v[3]);
+                o.z = Fp16Planes::next(v[4], v[5]); o.w = Fp16Planes::next(v[6], v[7]);
+                *reinterpret_cast<uint4*>(to + t * 2 * SUB_BYTES) = o;
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const uint32_t o = Fp16Planes::next(v[e], v[e + 1]);
+                    uint8_t* to = x + (r >> 7) * SQUARE_BYTES + t * 2 * SUB_BYTES;
+                    if (e < have) *reinterpret_cast<uint16_t*>(to + square_at(c + e, r & 127)) = (uint16_t) o;
+                    if (e + 1 < have) *reinterpret_cast<uint16_t*>(to + square_at(c + e + 1, r & 127)) = (uint16_t) (o >> 16);
+                }
+            }
+        }
+    }
+
+    const int quarter = warp & 3, wide = (warp >> 2) * 32;            // this warp's block of a square: rows and columns
+    const uint32_t lanes = (uint32_t) (quarter * 32) << 16;
+    const int row = quarter * 32 + lane;
+    const int m32 = (p.m + 31) / 32 * 32;
+    const bool in_square = quarter * 32 < m32 && wide < m32;
+    auto width = [&](int q) { return min(128, (columns - 128 * q + 31) / 32 * 32); };  // of a square of X; nothing or less: none
+    // room for the parts: the second square of X if there is none, else the place of P and Q, which then needs two more meetings
+    const bool apart = squares == 1;
+    uint8_t* parts = apart ? x + SQUARE_BYTES : square;
+    // eight additions into an accumulator of 128 of K, see plane::Engine::collect
+    const float debias = 1.f + 0.18f * 1.1920929e-7f * 9.f;
+    uint32_t phase = 0;
+    // shared memory that this thread wrote is there for the MMAs of all; then one thread issues them and all wait
+    auto multiply = [&](auto issue) {
+        ptx::fence_proxy_async_smem();
+        ptx::tcgen05_fence_before();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            ptx::tcgen05_fence_after();
+            issue();
+            ptx::umma_commit(done);
+        }
+        ptx::mbar_wait(done, phase, abort_flag, p.status_word, 560);
+        __syncwarp();
+        phase ^= 1;
+        ptx::tcgen05_fence_after();
+    };
+    auto read = [&](uint32_t column, float* v) {
+        ptx::tmem_ld32(tmem + lanes + column + (uint32_t) wide, v);
+        ptx::tmem_ld_wait();
+    };
+
+    for (int step = 0; step < p.steps; step++) {
+        const float f = step == 0 ? p.f0 : 1.f;
+        float v[32], u[32];
+        // ---- P: main sums of the squares in columns 0 and 256, both squares' smaller products in 128
+        multiply([&]() {
+            for (int q = 0; q < squares; q++) {
+                const uint32_t at = ptx::smem_u32(x + q * SQUARE_BYTES);
+                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 128, at, at, false, q > 0, m32, width(q));
+            }
+        });
+        if (in_square) {
+            const bool any = columns > 0;  // a last CTA without columns has nothing to add
+            read(0, v);
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = any ? v[j] * debias : 0.f;
+            if (width(1) > 0 && squares == 2) {
+                read(256, u);
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], debias, v[j]);
+            }
+            read(128, u);
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = any ? f * f * fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]) : 0.f;
+            if (p.cluster == 1) put_row(square, row, wide, v);
+        }
+        if (p.cluster > 1) {
+            const int own = m32 / p.cluster;  // rows that a CTA adds up
+            if (!apart) meet();               // nobody needs its Q any more
+            if (in_square) {                  // parts are [CTA][row][128]
+                float* patch = (float*) (patches + warp * HALF_PATCH);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {  // sixteen rows at a time through the patch, so that remote stores are whole lines
+                    if ((lane >> 4) == h) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            *reinterpret_cast<float4*>(patch + (lane & 15) * 32 + 4 * (j ^ (lane & 7))) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = 4 * i + (lane >> 3), to = quarter * 32 + 16 * h + r, owner = to / own;
+                        const float4 o = *reinterpret_cast<const float4*>(patch + r * 32 + 4 * ((lane & 7) ^ (r & 7)));
+                        const uint32_t at = remote(ptx::smem_u32(parts) + (uint32_t) (((rank * own + to - owner * own) * 128 + wide + 4 * (lane & 7)) * 4), owner);
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(o.x), "f"(o.y), "f"(o.z), "f"(o.w) : "memory");
+                    }
+                    __syncwarp();
+                }
+            }
+            meet();
+            constexpr int TURNS = SMALL_ROWS / 2 * 32 / SMALL_THREADS;  // four values of a row each; two CTAs are the fewest that share
+            float4 mine[TURNS];
+#pragma unroll
+            for (int q = 0; q < TURNS; q++) {
+                const int i = q * SMALL_THREADS + threadIdx.x;
+                if (i >= own * 32 || i % 32 * 4 >= m32) continue;
+                const float4* part = (const float4*) parts + i;
+                mine[q] = part[0];
+                for (int k = 1; k < p.cluster; k++) {
+                    const float4 o = part[k * own * 32];
+                    mine[q].x += o.x; mine[q].y += o.y; mine[q].z += o.z; mine[q].w += o.w;
+                }
+            }
+            if (!apart) meet();  // all parts have been read: P takes their place
+#pragma unroll
+            for (int q = 0; q < TURNS; q++) {
+                const int i = q * SMALL_THREADS + threadIdx.x, r = rank * own + i / 32, c = i % 32 * 4;
+                if (i >= own * 32 || c >= m32) continue;
+                float e[4] = {mine[q].x, mine[q].y, mine[q].z, mine[q].w};
+#pragma unroll
+                for (int t = 0; t < TERMS; t++) {
+                    const uint32_t a = Fp16Planes::next(e[0], e[1]), b = Fp16Planes::next(e[2], e[3]);
+                    const uint32_t at = ptx::smem_u32(square) + (uint32_t) (t * 2 * SUB_BYTES) + square_at(r, c);
+                    for (int k = 0; k < p.cluster; k++)
+                        asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(remote(at, k)), "r"(a), "r"(b) : "memory");
+                }
+            }
+            asm volatile("fence.proxy.async;" ::: "memory");
+            meet();
+        }
+        // ---- Q, in place of P
+        const uint32_t sq = ptx::smem_u32(square);
+        multiply([&]() { square_product(tmem, tmem + 128, sq, sq, false, false, m32, m32); });
+        if (in_square) {
+            read(0, v);
+            read(128, u);
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j] * debias);
+            get_row(square, row, wide, u);
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = p.kc * v[j] + p.kb * u[j] + (row == wide + j && row < p.m ? p.ka : 0.f);
+            put_row(square, row, wide, v);
+        }
+        // ---- X
+        multiply([&]() {
+            for (int q = 0; q < squares; q++)
+                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * q + 128, sq, ptx::smem_u32(x + q * SQUARE_BYTES), true, false, width(q), m32);
+        });
+        for (int q = 0; q < squares; q++) {
+            if (quarter * 32 >= m32 || wide >= width(q)) continue;
+            read(256 * q, v);
+            read(256 * q + 128, u);
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j] * debias);
+            if (step + 1 < p.steps) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] *= f;
+                put_row(x + q * SQUARE_BYTES, row, wide, v);
+            } else {
+                const int column = c0 + q * 128 + wide;
+                TileAt at;
+                at.batch = batch;
+                at.row = p.tall ? column : quarter * 32;
+                at.col = p.tall ? quarter * 32 : column;
+                const int end = c0 + columns;  // the columns after them are another CTA's
+                if (p.tall) {
+                    const auto write = Last::writer(last, at, lane);
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (column + j < end) write(j, v[j]);
+                } else {
+                    auto write = Last::writer(last, at, lane);
+                    if (column + lane >= end) write.rows = 0;
+                    plane::by_rows(v, (uint32_t*) square + warp * plane::PATCH_FLOATS, lane, write);
+                    __syncwarp();
+                }
+            }
+        }
+    }
+    ptx::tcgen05_fence_before();
+    meet();
+    if (warp == 0) {
+        ptx::tcgen05_fence_after();
+        ptx::tmem_free<false>(tmem, 512);
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -573,14 +922,66 @@ int launch_chain(const Maps& maps, const Chain& c, const typename Last::Args& la
     return CAKEB200_OK;
 }
 
+// Whether the matrices fit clusters, and how.
+bool fits_small(int m, int n, int batch, int sm_count, Small* p) {
+    if (m > SMALL_ROWS || n > SMALL_COLUMNS * SMALL_CLUSTER) return false;
+    int c = 1;
+    while (c * SMALL_COLUMNS < n) c *= 2;
+    // half as many columns per CTA make a step shorter as long as all clusters are resident together
+    while (c < SMALL_CLUSTER && n > 128 * c && (long long) batch * 2 * c <= sm_count * 3 / 4) c *= 2;
+    // One CTA per matrix is faster than the chain for any batch (2000 of 64 x 128: 0.60 ms, 1.09 in the chain).  Clusters are
+    // as long as few wait for others: of 8 CTAs, 128 x 2048, 32 matrices 298 us (chain 320), 64 matrices 497 (474).
+    if (c > 1 && (long long) batch * c > 3ll * sm_count) return false;
+    p->cluster = c;
+    p->slice = ((n + c - 1) / c + 7) / 8 * 8;
+    return true;
+}
+
+template <typename T, class Last>
+int launch_small(const Source<T>& src, const Small& p, const typename Last::Args& last, int device, cudaStream_t s) {
+    const auto kernel = small_kernel<T, Last>;
+    static std::atomic<unsigned long long> opted{0};  // devices whose shared-memory limit has been raised for this kernel
+    if (device >= 64 || !(opted.load() >> device & 1)) {
+        CAKE_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM));
+        if (device < 64) opted |= 1ull << device;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) (p.batch * p.cluster));
+    cfg.blockDim = dim3(SMALL_THREADS);
+    cfg.dynamicSmemBytes = SMALL_SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned) p.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CAKE_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, src, p, last));
+    return CAKEB200_OK;
+}
+
 // From the source to the last X, which goes through `Last`.  chunk: K blocks of 64 between folds of the main accumulator.
 template <typename T, class Last>
 int run(const Source<T>& src, int batch, const Coefficients& k, int chunk, void* workspace, typename Last::Args last, DeviceState* st, cudaStream_t s) {
     const int rows = src.rows, cols = src.cols;
     const bool tall = rows > cols;
     const int m = tall ? cols : rows, n = tall ? rows : cols;
-    const Layout l = lay_out((char*) workspace, batch, m, n);
+    // X_0 is held 2^up times itself: around sqrt(m n), below the 2^16 at which its largest possible element would overflow
+    const int up = std::min(15, (int) (0.5 * std::log2((double) m * n)));
+    const float down = std::ldexp(1.f, -up);
+    last.f = k.steps == 1 ? down : 1.f;
     int rc, units_single = 0, units_pair = 0;
+    Small small = {};
+    if (option_get(OPT_PAIR) == 0 && option_get(OPT_K_PIECES) == 0 && fits_small(m, n, batch, st->sm_count, &small)) {  // those options are about the chain
+        small.m = m; small.n = n; small.tall = tall; small.batch = batch; small.steps = k.steps;
+        small.eps = k.eps; small.f0 = down; small.ka = k.a; small.kb = k.b; small.kc = k.c;
+        small.up = std::ldexp(1.0, up);
+        small.status_word = st->status_word;
+        if ((rc = launch_small<T, Last>(src, small, last, st->device, s))) return rc;
+        thread_stats()->launches = 1;
+        return CAKEB200_OK;
+    }
+    const Layout l = lay_out((char*) workspace, batch, m, n);
     if ((rc = resident_units<false, Last>(&units_single)) || (rc = resident_units<true, Last>(&units_pair))) return rc;
     const long long tiles = plane::count_tiles(m, n, batch, false, 128);
     if (tiles > (1LL << 27)) {
@@ -592,17 +993,14 @@ int run(const Source<T>& src, int batch, const Coefficients& k, int chunk, void*
         (rc = plane::encode_planes<Fp16Planes>(maps.p.m, l.p, TERMS)) || (rc = plane::encode_planes<Fp16Planes>(maps.q.m, l.q, TERMS)))
         return rc;
 
-    // X_0 is held 2^up times itself: around sqrt(m n), below the 2^16 at which its largest possible element would overflow
-    const int up = std::min(15, (int) (0.5 * std::log2((double) m * n)));
     Chain c = {};
     c.x[0] = l.x[0]; c.x[1] = l.x[1]; c.p = l.p; c.q = l.q;
     c.batch = batch; c.steps = k.steps; c.chunk = chunk;
-    c.f0 = std::ldexp(1.f, -up);
+    c.f0 = down;
     c.ka = k.a; c.kb = k.b; c.kc = k.c;
     c.parts = l.parts;
     c.arrived = l.arrived;
     c.status_word = st->status_word;
-    last.f = k.steps == 1 ? c.f0 : 1.f;
     const int forced = option_get(OPT_PAIR);  // 1: pairs, 2: single SMs, 0: the faster by the model
     Chain other = c;
     const double t_single = plan(&c.gram, &c.poly, &c.apply, &c.last, m, n, tall, batch, false, units_single);

@@ -98,6 +98,34 @@ def test_forms_of_the_product(cake, shape, form):
         _hold(o, _plain(g, np.float64), _plain(g, np.float32).astype(np.float64), "float32")
 
 
+# (batch, rows, cols): one CTA per matrix, with one and two squares of 128 columns; clusters of 2, 4 and 8; ends inside an
+# eight, a block of 32 and a square; the last sizes that fit, and the first ones that do not
+SMALL = [(1, 128, 128), (150, 65, 130), (150, 128, 256), (80, 33, 257), (40, 97, 1000), (1, 128, 2048), (1, 2, 2047), (3, 100, 1025), (20, 127, 1111),
+         (1, 129, 128), (1, 128, 2056), (60, 30, 1300)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("tall", [False, True], ids=["wide", "tall"])
+@pytest.mark.parametrize("size", SMALL, ids=str)
+def test_small_matrices(cake, size, tall, dtype):
+    """Matrices that stay in the shared memory of a cluster from the first step to the last, inside wider rows: nothing around
+    the result changes, and the same bits come every time."""
+    import torch
+    rng = np.random.default_rng(size[0] + size[2])
+    b, m, n = size
+    r, c = (n, m) if tall else (m, n)
+    G = torch.from_numpy(np.stack([_gradient(rng, r, c, ("noise", "tokens")[i % 2]) for i in range(b)]).astype(np.float32)).to(getattr(torch, dtype))
+    frame = torch.full((b, r + 1, c + 13), 7.0, dtype=G.dtype, device="cuda")
+    O = frame[:, :r, 5:5 + c]
+    cake.cake_orthogonalize(G.cuda(), out=O)
+    for i in sorted({0, b // 2, b - 1}):
+        g = G[i].double().numpy()
+        _hold(O[i].double().cpu().numpy(), _plain(g, np.float64), _plain(g, np.float32).astype(np.float64), dtype)
+    assert torch.equal(cake.cake_orthogonalize(G.cuda()), O)
+    O.fill_(7.0)
+    assert bool((frame == 7).all())
+
+
 @pytest.mark.parametrize("pair", [1, 2])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_many_tiles(cake, dtype, pair):
@@ -199,6 +227,19 @@ def test_muon_step(cake, shape, tw, tg):
         else:
             tol = lr * f * 480 * 5 ** 0.5 * 2.0 ** -18 + torch.finfo(torch.bfloat16).eps / 2 * np.linalg.norm(want)
         assert err <= tol, (err, tol)
+
+
+@pytest.mark.parametrize("shape", [(128, 1500), (900, 70), (20, 2048), (5, 5)], ids=str)
+def test_muon_step_of_small_matrices_is_the_steps_of_its_parts(cake, shape):
+    """The step's result through the optimiser's entry is W - lr f O of the same update, to the roundings of that line."""
+    import torch
+    torch.manual_seed(shape[0])
+    W, G, M = (torch.randn(shape, device="cuda") for _ in range(3))
+    w, m = W.clone(), M.clone()
+    cake.cake_muon_step(w, G, m, 0.1, momentum=0.5, nesterov=False, scale=1.0)
+    assert torch.equal(m, 0.5 * M + 0.5 * G)  # exact but for one rounding, the same in both
+    want = W.double() - 0.1 * cake.cake_orthogonalize(m).double()
+    assert bool(((w.double() - want).abs() <= 2.0 ** -23 * (want.abs() + 0.2)).all())
 
 
 def test_muon_step_inside_larger_tensors(cake):
