@@ -232,8 +232,9 @@ q4_linear_kernel(const Q4Args p) {
     constexpr int E = R * NT * 128;
     constexpr int QUEUE = AHEAD * R * 64;  // of a warp, in 16-byte pieces
     // with few columns there are registers for what keeps a lone warp busy: x of a whole step loaded at its start, and two chains of
-    // dependent MMAs per sum
-    constexpr int HALVES = NT == 1 && TERMS == 1 ? 2 : 1, CHAINS = NT == 1 ? 2 : 1;
+    // dependent MMAs per sum.  FP32 takes the products with the leading terms of x apart from the others: an MMA truncates the sum
+    // that it adds to, and 8 such additions per group of 128 instead of 24 leave a third of that
+    constexpr int HALVES = NT == 1 && TERMS == 1 ? 2 : 1, CHAINS = NT == 1 || TERMS > 1 ? 2 : 1;
     extern __shared__ uint4 shared[];      // queues, then two sets of sums
     float* red = (float*) (shared + WARPS * QUEUE);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, a = lane >> 2, t = lane & 3;
@@ -367,7 +368,7 @@ q4_linear_kernel(const Q4Args p) {
                             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                                 for (int u = TERMS - 1; u >= 0; u--)
-                                    mma<M>(acc[r][nt][j % CHAINS], w, b[half % HALVES][nt][2 * j][u], b[half % HALVES][nt][2 * j + 1][u]);
+                                    mma<M>(acc[r][nt][TERMS > 1 ? u > 0 : j % CHAINS], w, b[half % HALVES][nt][2 * j][u], b[half % HALVES][nt][2 * j + 1][u]);
                         }
                     }
                     if (last) {  // the group is complete
