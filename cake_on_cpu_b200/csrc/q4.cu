@@ -5,18 +5,16 @@
 // With few rows both are bound by reading the codes from HBM: half a byte per multiply-add and row.  What stands in
 // the way of that bound is the work of turning codes into numbers.  At 6.4 TB/s an SM receives 46 codes per clock, so a
 // lane may spend 2.8 instructions on one.  Converting a code to FP32 and multiplying takes about four; here a mask and a
-// shift place a pair of codes in the mantissas of two 16-bit numbers, which are the codes and a known offset, exactly,
-// and mma.m16n8k16 multiplies 16 x 16 of them with up to eight rows of x at once.  The products are exact and summed in
-// FP32; offset and zero point are taken out of the sum of a block (64 features) with the block's sum of x, which a further MMA
-// with ones gives for all output features; then the sum is multiplied by its scale in FP32 and added to the row's total,
-// so scales are never rounded into the weights.  (tcgen05.mma would take the weights from shared memory: writing converted
+// shift place a pair of codes in the mantissas of two 16-bit numbers, exactly, and mma.m16n8k16 multiplies 16 x 16 of them with
+// up to eight rows of x at once.  The products are exact and summed in FP32; the sum of a group is multiplied by its scale
+// in FP32 and added to the row's total, so scales are never rounded into the weights.  (tcgen05.mma would take the weights from shared memory: writing converted
 // codes there costs four times the bytes that are read from HBM.)
-//   FP16 x: the code is a subnormal FP16, q 2^-24 or, left where it lies four bits up, 16 q 2^-24: no offset.
-//   BF16 x: 128 + q, the code in the last bits of the mantissa.  The offset makes the sums some thirty times larger than
-//           without it, which costs them five of their 24 bits and leaves them far below the result's own 2^-8.
-//   FP32 x: 128 + q, and 128 + z subtracted from every pair right away, which leaves sums as small as they can be.
+//   Centred: 128 + q as BF16 or 1024 + q as FP16, the code in the last bits of the mantissa, and 128 + z or 1024 + z subtracted
+//   from every pair right away.
+//   FP16 x, up to eight rows: the code is a subnormal FP16, q 2^-24 or, left where it lies four bits up, 16 q 2^-24; the zero
+//   point is taken out of the group's sum with its sum of x, which a further MMA with ones gives for all output features.
 // A 32-bit x goes through the 16-bit multiplier as three terms x = x0 + x1 + x2 of 8 mantissa bits each (truncations,
-// so the split is exact and cannot overflow); the three products land in the same FP32 sums.
+// so the split is exact and cannot overflow); their products are summed in FP32.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -41,28 +39,42 @@ __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, ui
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The four A registers of a word's MMA.  A code in the mantissa of a power of two whose last mantissa bit counts 1 (128 + q),
-// then the power and the zero point subtracted, both halves at once: exact whole numbers.  sub_lo / sub_hi: 128 + z of rows a / a + 8.
+// The power of two whose last mantissa bit counts 1, in both halves of a word: 128 as BF16, 1024 as FP16.
+template <typename M> constexpr uint32_t POWER = std::is_same<M, __half>::value ? 0x64006400u : 0x43004300u;
+// that power + z in both halves (z < 16)
+template <typename M>
+__device__ __forceinline__ uint32_t zero_pair(uint32_t z) { return POWER<M> | (z << 16) | z; }
+// The four A registers of a word's MMA.  A code in the mantissa of that power, then the power and the zero point subtracted, both
+// halves at once: exact whole numbers.  sub_lo / sub_hi: zero_pair of rows a / a + 8.
+template <typename M>
 __device__ __forceinline__ void unpack_centred(uint32_t w, uint32_t sub_lo, uint32_t sub_hi, uint32_t* a) {
+    using M2 = typename std::conditional<std::is_same<M, __half>::value, __half2, __nv_bfloat162>::type;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | POWER<M>;
         const uint32_t sub = (i & 1) ? sub_hi : sub_lo;
-        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&sub));
+        const M2 r = __hsub2(*reinterpret_cast<const M2*>(&v), *reinterpret_cast<const M2*>(&sub));
         a[i] = *reinterpret_cast<const uint32_t*>(&r);
     }
 }
-// 128 + z in both halves (z < 16)
-__device__ __forceinline__ uint32_t zero_pair(uint32_t z) { return 0x43004300u | (z << 16) | z; }
 
-// The same for the forward product's types.  OFFSET is what the numbers have on top of q; UP_LO and UP_HI are what those of rows
-// a and a + 8 (registers 0, 2 and 1, 3) are multiplied by.
-template <typename T> struct Codes;
-template <> struct Codes<__half> {
+// Codes as numbers of the MMA's type, for the forward product.  Centred, they are w / scale.  The other form saves the subtractions
+// and half of the shifts and leaves the zero point to the sums of x (SUM); DOWN_LO and DOWN_HI are what takes the sums of rows a and
+// a + 8 (registers 0, 2 and 1, 3) back to codes.
+template <typename T, bool CENTRED>
+struct Codes {
+    using M = typename std::conditional<std::is_same<T, __half>::value, __half, __nv_bfloat16>::type;
+    static constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;  // of x
+    static constexpr bool SUM = false;
+    static constexpr float DOWN_LO = 1.f, DOWN_HI = 1.f;
+    static constexpr uint32_t ONE = 0;
+    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t sub_lo, uint32_t sub_hi, uint32_t* a) { unpack_centred<M>(w, sub_lo, sub_hi, a); }
+};
+template <> struct Codes<__half, false> {
     using M = __half;
     static constexpr int TERMS = 1;
     static constexpr bool SUM = true;
-    static constexpr float OFFSET = 0.f, DOWN_LO = 16777216.f, DOWN_HI = 1048576.f;
+    static constexpr float DOWN_LO = 16777216.f, DOWN_HI = 1048576.f;
     static constexpr uint32_t ONE = 0x3c003c00u;
     static __device__ __forceinline__ void unpack(uint32_t w, uint32_t, uint32_t, uint32_t* a) {
         a[0] = w & 0x000f000fu;
@@ -72,29 +84,6 @@ template <> struct Codes<__half> {
         a[3] = w & 0x00f000f0u;
     }
 };
-template <> struct Codes<__nv_bfloat16> {
-    using M = __nv_bfloat16;
-    static constexpr int TERMS = 1;
-    static constexpr bool SUM = true;
-    static constexpr float OFFSET = 128.f, DOWN_LO = 1.f, DOWN_HI = 1.f;
-    static constexpr uint32_t ONE = 0x3f803f80u;
-    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t, uint32_t, uint32_t* a) {
-        a[0] = (w & 0x000f000fu) | 0x43004300u;
-#pragma unroll
-        for (int i = 1; i < 4; i++) a[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-    }
-};
-template <> struct Codes<float> {
-    using M = __nv_bfloat16;
-    static constexpr int TERMS = 3;
-    static constexpr bool SUM = false;
-    static constexpr float OFFSET = 0.f, DOWN_LO = 1.f, DOWN_HI = 1.f;
-    static constexpr uint32_t ONE = 0;
-    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t sub_lo, uint32_t sub_hi, uint32_t* a) {
-        unpack_centred(w, sub_lo, sub_hi, a);
-    }
-};
-
 // Codes are read once and go past L1 into a queue of the lane's own in shared memory, so that many are on their way without
 // holding registers; a lane reads back what it asked for itself.
 __device__ __forceinline__ void fetch16(uint4* to, const uint4* from) {
@@ -150,8 +139,8 @@ struct Q4Args {
 // B fragments of a lane for a block: features 32 h + 8 t + 0 .. 7, h = 0, 1, of its row, pairs of features to a register.  `x` points at
 // the first of them; `inside`: 16-byte loads are allowed and the block ends within the row.
 template <typename T>
-__device__ __forceinline__ void load_x(const T* x, bool inside, int left, uint32_t (*b)[Codes<T>::TERMS]) {
-    constexpr int TERMS = Codes<T>::TERMS;
+__device__ __forceinline__ void load_x(const T* x, bool inside, int left, uint32_t (*b)[Codes<T, true>::TERMS]) {
+    constexpr int TERMS = Codes<T, true>::TERMS;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const T* p = x + 32 * h;
@@ -226,7 +215,10 @@ constexpr int AHEAD = 3;  // steps in a lane's queue
 template <typename T, int NT, int R, int GROUPS, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
 q4_linear_kernel(const Q4Args p) {
-    using C = Codes<T>;
+    // FP16 with ones instead of subtractions pays up to eight rows, where unpacking is what takes the time (us, 4096 x 4096: 6.6,
+    // centred 7.2; 16384 x 512: 5.3 and 6.1).  With more rows the products do, and those with ones are half as many (16384 x 8192, 32
+    // rows: 55.0, centred 51.3).  BF16 would need an offset in the sums and gains nothing (27.3, centred 26.3).
+    using C = Codes<T, !std::is_same<T, __half>::value || (NT > 1)>;
     using M = typename C::M;
     constexpr int TERMS = C::TERMS;
     constexpr int E = R * NT * 128;
@@ -363,7 +355,7 @@ q4_linear_kernel(const Q4Args p) {
                         for (int r = 0; r < R; r++) {
                             const uint32_t z = now[r].zeros[g / 2] >> (16 * (g & 1));
                             uint32_t w[4];
-                            C::unpack(j & 1 ? c[r].y : c[r].x, zero_pair(z & 15u), zero_pair((z >> 8) & 15u), w);
+                            C::unpack(j & 1 ? c[r].y : c[r].x, zero_pair<M>(z & 15u), zero_pair<M>((z >> 8) & 15u), w);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -376,7 +368,7 @@ q4_linear_kernel(const Q4Args p) {
                         for (int r = 0; r < R; r++) {
                             const uint32_t z = now[r].zeros[g / 2] >> (16 * (g & 1));
                             const float s_lo = q4_scale((uint16_t) now[r].scales[g], p.w.scale_bf16), s_hi = q4_scale((uint16_t) (now[r].scales[g] >> 16), p.w.scale_bf16);
-                            const float z_lo = s_lo * (C::OFFSET + (float) (z & 15u)), z_hi = s_hi * (C::OFFSET + (float) ((z >> 8) & 15u));
+                            const float z_lo = s_lo * (float) (z & 15u), z_hi = s_hi * (float) ((z >> 8) & 15u);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -515,11 +507,11 @@ q4_linear_dx_kernel(const Q4Args p) {
                 split_pair<TERMS>(v[nt][0] * s[0], v[nt][1] * s[1], b[nt][0]);
                 split_pair<TERMS>(v[nt][2] * s[2], v[nt][3] * s[3], b[nt][1]);
             }
-            const uint32_t sub_lo = zero_pair(now.zeros[m] & 15u), sub_hi = zero_pair((now.zeros[m] >> 8) & 15u);
+            const uint32_t sub_lo = zero_pair<M>(now.zeros[m] & 15u), sub_hi = zero_pair<M>((now.zeros[m] >> 8) & 15u);
 #pragma unroll
             for (int j = m * 4 / MINE; j < (m + 1) * 4 / MINE; j++) {
                 uint32_t w[4], wt[4];
-                unpack_centred(words[j], sub_lo, sub_hi, w);
+                unpack_centred<M>(words[j], sub_lo, sub_hi, w);
                 // registers 0, 1 hold the lower pairs of rows 0-7, 8-15, registers 2, 3 the upper pairs; transposed, the
                 // features are the rows of the A operand and 1 and 2 change places
                 wt[0] = transpose8(w[0]); wt[1] = transpose8(w[2]); wt[2] = transpose8(w[1]); wt[3] = transpose8(w[3]);
