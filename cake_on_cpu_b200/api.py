@@ -919,7 +919,8 @@ def cake_orthogonalize(G, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7, stream=
     """The orthogonalisation of a matrix, or of every matrix of a batch, by Newton-Schulz products (cakeb200_orthogonalize),
     enqueued on the current stream: X = G / (|G|_F + eps), then ``steps`` times X <- a X + b (X X^T) X + c (X X^T)^2 X.
 
-    G: CUDA tensor (rows, cols) or (batch, rows, cols), float32 or bfloat16, rows contiguous.  ``out`` may be G."""
+    G: CUDA tensor (rows, cols) or (batch, rows, cols), float32 or bfloat16, rows contiguous.  ``out`` may be G
+    or overlap it."""
     import torch
     if not (_is_torch(G) and G.is_cuda):
         raise TypeError("G must be a CUDA tensor")
@@ -951,7 +952,7 @@ def cake_muon_step(W, G, M, lr, momentum=0.95, nesterov=True, weight_decay=0.0, 
     M <- momentum M + (1 - momentum) G;  U = momentum M + (1 - momentum) G, or M without ``nesterov``;
     W <- (1 - lr weight_decay) W - lr scale O(U).  ``scale`` defaults to sqrt(max(1, rows / cols)).
 
-    W and G: float32 or bfloat16 CUDA matrices with contiguous rows, M: the same in float32.  Returns W."""
+    W and G: float32 or bfloat16 CUDA matrices with contiguous rows, M: the same in float32, in memory of its own.  Returns W."""
     if not (_is_torch(W) and W.is_cuda):
         raise TypeError("W must be a CUDA tensor")
     if W.dim() != 2:

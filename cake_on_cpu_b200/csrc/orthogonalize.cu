@@ -826,6 +826,16 @@ int check_shape(const char* who, int rows, int cols, int batch) {
     return CAKEB200_OK;
 }
 
+// Whether two matrices of `rows` rows share memory: addresses, bytes of a row, bytes from row to row.  Rows of the same pitch may lie
+// beside one another.
+bool overlap(const void* a, long long width_a, long long pitch_a, const void* b, long long width_b, long long pitch_b, int rows) {
+    const long long from_a = (long long) (uintptr_t) a, from_b = (long long) (uintptr_t) b;
+    if (from_a + (rows - 1) * pitch_a + width_a <= from_b || from_b + (rows - 1) * pitch_b + width_b <= from_a) return false;
+    if (pitch_a != pitch_b) return true;
+    const long long d = ((from_b - from_a) % pitch_a + pitch_a) % pitch_a;
+    return d < width_a || d + width_b > pitch_a;
+}
+
 struct Coefficients {
     int steps;
     float a, b, c, eps;
@@ -961,8 +971,9 @@ int launch_small(const Source<T>& src, const Small& p, const typename Last::Args
 }
 
 // From the source to the last X, which goes through `Last`.  chunk: K blocks of 64 between folds of the main accumulator.
+// early: the results of one matrix may be stored while other matrices are still read.
 template <typename T, class Last>
-int run(const Source<T>& src, int batch, const Coefficients& k, int chunk, void* workspace, typename Last::Args last, DeviceState* st, cudaStream_t s) {
+int run(const Source<T>& src, int batch, bool early, const Coefficients& k, int chunk, void* workspace, typename Last::Args last, DeviceState* st, cudaStream_t s) {
     const int rows = src.rows, cols = src.cols;
     const bool tall = rows > cols;
     const int m = tall ? cols : rows, n = tall ? rows : cols;
@@ -972,7 +983,7 @@ int run(const Source<T>& src, int batch, const Coefficients& k, int chunk, void*
     last.f = k.steps == 1 ? down : 1.f;
     int rc, units_single = 0, units_pair = 0;
     Small small = {};
-    if (option_get(OPT_PAIR) == 0 && option_get(OPT_K_PIECES) == 0 && fits_small(m, n, batch, st->sm_count, &small)) {  // those options are about the chain
+    if (early && option_get(OPT_PAIR) == 0 && option_get(OPT_K_PIECES) == 0 && fits_small(m, n, batch, st->sm_count, &small)) {  // those options are about the chain
         small.m = m; small.n = n; small.tall = tall; small.batch = batch; small.steps = k.steps;
         small.eps = k.eps; small.f0 = down; small.ka = k.a; small.kb = k.b; small.kc = k.c;
         small.up = std::ldexp(1.0, up);
@@ -1038,7 +1049,11 @@ int orthogonalize(const void* G, long long ldg, long long stride_g, void* out, l
     src.rows = rows;
     src.cols = cols;
     typename ResultEpilogue<T>::Args last = {matrix((T*) out, ldo, stride_o, rows, batch), rows, cols, 1.f};
-    return run<T, ResultEpilogue<T>>(src, batch, k, chunk, workspace, last, st, s);
+    // in place is fine matrix by matrix; a result that lies across its operands has to wait for all of them
+    const long long size = sizeof(T), reach_g = (rows - 1) * ldg + cols + (batch - 1) * stride_g, reach_o = (rows - 1) * ldo + cols + (batch - 1) * stride_o;
+    const bool same = G == out && ldg == ldo && (batch == 1 || stride_g == stride_o);
+    const bool early = batch == 1 || same || (stride_g >= 0 && !overlap(G, reach_g * size, reach_g * size, out, reach_o * size, reach_o * size, 1));
+    return run<T, ResultEpilogue<T>>(src, batch, early, k, chunk, workspace, last, st, s);
 }
 
 template <typename TW, typename TG>
@@ -1055,7 +1070,7 @@ int muon(void* W, long long ldw, const void* G, long long ldg, float* M, long lo
     src.rows = rows;
     src.cols = cols;
     typename StepEpilogue<TW>::Args last = {matrix((TW*) W, ldw, 0, rows, 1), rows, cols, 1.f, (float) (1.0 - lr * weight_decay), (float) (lr * scale)};
-    return run<TG, StepEpilogue<TW>>(src, 1, k, chunk, workspace, last, st, s);
+    return run<TG, StepEpilogue<TW>>(src, 1, true, k, chunk, workspace, last, st, s);
 }
 
 }  // namespace
@@ -1118,6 +1133,9 @@ int cakeb200_muon_step(void* W, long long ldw, int type_w, const void* G, long l
     if (workspace_bytes < cakeb200_orthogonalize_workspace(rows, cols, 1, type_w)) return bad(who, "the workspace is too small");
     if ((uintptr_t) W % (type_w == CAKEB200_F32 ? 4 : 2) || (uintptr_t) G % (type_g == CAKEB200_F32 ? 4 : 2) || (uintptr_t) M % 4)
         return bad(who, "a pointer is not aligned to its type");
+    const long long size_w = type_w == CAKEB200_F32 ? 4 : 2, size_g = type_g == CAKEB200_F32 ? 4 : 2;
+    if (overlap(M, cols * 4LL, ldm * 4, W, cols * size_w, ldw * size_w, rows) || overlap(M, cols * 4LL, ldm * 4, G, cols * size_g, ldg * size_g, rows))
+        return bad(who, "M overlaps W or G");
     DeviceState* st = device_state();
     if (!st) return CAKEB200_ERR_NO_DEVICE;
     if (!on_current_device(W) || !on_current_device(G) || !on_current_device(M) || !on_current_device(workspace))

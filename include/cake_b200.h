@@ -149,7 +149,8 @@ int cakeb200_sgemm_after(const float* A, const float* B, float* C, int M, int N,
  *               of 256 instead of 128 adds more than 7 % of rows.  Both forms give the same bits when no tile is
  *               cut along K ("k_pieces" 1).  The products inside cakeb200_orthogonalize and cakeb200_muon_step follow it
  *               too (1 = always pairs; rule: a model of their time), and "k_pieces" gives the number of parts the tiles of a
- *               last round are cut into there (1 = never cut).
+ *               last round are cut into there (1 = never cut).  With either option set, small matrices (up to 128 x 2048) go
+ *               through the same kernel as large ones.
  * They take the place of the block sizes a caller of the reference forces with mcu / kcu / ncu
  * (reference include/cake.h:12-14, src/block_sizing.cpp:363-368) and of update_mr_nr
  * (src/block_sizing.cpp:78-83): on a GPU the blocks a caller may pin are the tile, the walk and
@@ -461,15 +462,15 @@ int cakeb200_q4_linear_dx(const cakeb200_q4* w, const void* dy, long long lddy, 
  * singular values of X end up near 1 whatever those of G were.
  *
  * _orthogonalize works on `batch` matrices `stride` elements apart, each rows x cols with leading dimension ld (elements).
- * G and out have one type, CAKEB200_F32 or CAKEB200_BF16; out may be G itself.  FP32 matrices are multiplied with operands
- * of 24 bits, BF16 ones with operands of 16, all sums in FP32; the result is rounded once.  A G that is zero gives zero; one
+ * G and out have one type, CAKEB200_F32 or CAKEB200_BF16; out may be G itself or lie across it.  All products have operands of
+ * 22 bits and a sign, held in pairs of FP16, and sums in FP32; the result is rounded once.  A G that is zero gives zero; one
  * that is not finite gives NaN.
  *
  * _muon_step is one optimiser step on one matrix, in place:
  *     M <- momentum M + (1 - momentum) G
  *     U  = momentum M + (1 - momentum) G  (nesterov != 0)  or  M
  *     W <- (1 - lr weight_decay) W - lr scale O(U),    O as above.
- * W and G are CAKEB200_F32 or CAKEB200_BF16 each, M is FP32; operands of 24 bits when W is FP32.
+ * W and G are CAKEB200_F32 or CAKEB200_BF16 each, M is FP32 and shares no memory with them.
  *
  * `workspace` is device memory of the caller's, 1024-byte aligned and at least _workspace(rows, cols, batch, type of the
  * result) bytes (1 for the step's batch); its content does not matter before and after the call, but calls that may overlap on the

@@ -259,6 +259,37 @@ def test_muon_step_inside_larger_tensors(cake):
         assert bool((f == 3).all())
 
 
+@pytest.mark.parametrize("shape", [(5, 40, 100), (3, 96, 1500), (2, 150, 200)], ids=str)
+def test_results_across_the_operands(cake, shape):
+    """A result that lies over other matrices of the batch, and one beside its operand in the same rows."""
+    import torch
+    torch.manual_seed(shape[1])
+    b, r, c = shape
+    buf = torch.randn(b + 1, r, c, device="cuda")
+
+    def hold(got):
+        for i in (0, b - 1):
+            g = buf[i].double().cpu().numpy()
+            _hold(got[i].double().cpu().numpy(), _plain(g, np.float64), _plain(g, np.float32).astype(np.float64), "float32")
+
+    for src, dst in ((0, 1), (1, 0)):
+        two = torch.empty_like(buf)
+        two[src:src + b] = buf[:b]
+        hold(cake.cake_orthogonalize(two[src:src + b], out=two[dst:dst + b]))
+    rows = torch.empty(b, r, 2 * c, device="cuda")
+    rows[:, :, :c] = buf[:b]
+    hold(cake.cake_orthogonalize(rows[:, :, :c], out=rows[:, :, c:]))
+    assert torch.equal(rows[:, :, :c], buf[:b])
+    # momentum, gradient and weight side by side in the rows of one matrix
+    wide = torch.randn(r, 3 * c, device="cuda")
+    W, G, M = (wide[:, i * c:(i + 1) * c].clone() for i in range(3))
+    cake.cake_muon_step(W, G, M, 0.1)
+    cake.cake_muon_step(wide[:, :c], wide[:, c:2 * c], wide[:, 2 * c:], 0.1)
+    assert torch.equal(wide, torch.cat((W, G, M), 1))
+    with pytest.raises(cake.CakeError):
+        cake.cake_muon_step(W, M, M, 0.1)
+
+
 def test_refusals(cake):
     import torch
     G = torch.randn(8, 12, device="cuda")

@@ -126,6 +126,22 @@ def test_muon_refusals(cake):
         assert call(**change) == ERR_ARG and word in _last(cake), (change, _last(cake))
 
 
+@pytest.mark.parametrize("where", ["W", "G"])
+@pytest.mark.parametrize("off, ldm, refused", [(0, 12, True), (4 * 90, 12, True), (4 * 8 * 12, 12, False), (-4 * 8 * 12, 12, False), (4 * 11, 40, True),
+                                               (4 * 12, 40, False), (4 * 28, 40, False), (4 * 29, 40, True), (-4 * 12, 40, False), (-4, 40, True)])
+def test_muon_momentum_has_its_own_memory(cake, where, off, ldm, refused):
+    """8 x 12 matrices at made-up addresses: overlapping ones are refused, ones that follow one another or lie side by side
+    in the rows of a wider matrix go on to the next check, of the device."""
+    L = cake.lib()
+    base = 1 << 20
+    at = {"W": 1 << 24, "G": 1 << 26, "M": base + off}
+    at[where] = base
+    ld = ldm if ldm == 40 else 12
+    ws = L.cakeb200_orthogonalize_workspace(8, 12, 1, 0)
+    rc = L.cakeb200_muon_step(at["W"], ld, 0, at["G"], ld, 0, at["M"], ldm, 8, 12, 0.1, 0.9, 1, 0.0, 1.0, 5, 1.0, 0.0, 0.0, 0.0, 1 << 28, ws, None)
+    assert rc != 0 and ("overlaps" in _last(cake)) == refused, _last(cake)
+
+
 def test_orthogonalize_python_layer_takes_cuda_tensors_only(cake):
     import numpy as np
     import torch
