@@ -109,6 +109,7 @@ class cake_linear_q4_function(torch.autograd.Function):
         return api.cake_q4_linear(data, weights, bias)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
         dy = grad_output if grad_output.is_contiguous() else grad_output.contiguous()
         gi = api.cake_q4_linear_dx(dy, ctx.weights) if ctx.needs_input_grad[0] else None
@@ -181,4 +182,15 @@ class cake_muon(torch.optim.Optimizer):
                     state["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 api.cake_muon_step(p, _rows(p.grad), state["momentum"], group["lr"], group["momentum"], group["nesterov"], group["weight_decay"],
                                    group["scale"], group["steps"], group["coeffs"], group["eps"])
+                torch.autograd.graph.increment_version(p)  # written behind autograd's back
         return loss
+
+    def load_state_dict(self, state_dict):
+        """As every optimiser's, but the momentum stays in float32 (it would be rounded to the type of its parameter)."""
+        super().load_state_dict(state_dict)
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(ids, params):
+            saved = state_dict["state"].get(i, {})
+            if "momentum" in saved:
+                self.state[p]["momentum"] = saved["momentum"].to(device=p.device, dtype=torch.float32, copy=True).contiguous()

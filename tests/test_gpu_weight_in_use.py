@@ -117,3 +117,53 @@ def test_muon_refuses_what_is_not_a_matrix(cake):
     p.grad = torch.randn(9, 6, device="cuda").t()
     opt.step()
     assert bool(torch.isfinite(p).all())
+
+
+def test_step_is_seen_by_autograd(cake):
+    """A graph that saved the weight before a step refuses to go backward after it; gradients of gradients are refused too."""
+    import torch
+    from cake_on_cpu_b200.cake import cake_linear_q4, cake_muon
+    torch.manual_seed(5)
+    w = torch.nn.Parameter(torch.randn(40, 70, device="cuda"))
+    opt = cake_muon([w], lr=0.1)
+    x = torch.randn(6, 70, device="cuda", requires_grad=True)
+    old = (x @ w.t()).sum()
+    (x.detach() @ w.t()).square().sum().backward()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        old.backward()
+    layer = cake_linear_q4(cake.Q4Weights.quantize(w.detach()))
+    y = layer(x.detach().requires_grad_())
+    x2 = x.detach().requires_grad_()
+    (g,) = torch.autograd.grad(layer(x2).square().sum(), x2, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    assert y.shape == (6, 40)
+
+
+def test_resumed_training_goes_on_with_the_same_bits(cake):
+    import io
+    import torch
+    from cake_on_cpu_b200.cake import cake_muon
+    torch.manual_seed(6)
+    start = torch.randn(130, 60, device="cuda", dtype=torch.bfloat16)
+    grads = [torch.randn_like(start) for _ in range(4)]
+
+    def run(p, opt, some):
+        for g in some:
+            p.grad = g.clone()
+            opt.step()
+
+    p = torch.nn.Parameter(start.clone())
+    opt = cake_muon([p], lr=0.05)
+    run(p, opt, grads[:2])
+    f = io.BytesIO()
+    torch.save((p.detach(), opt.state_dict()), f)
+    run(p, opt, grads[2:])
+    f.seek(0)
+    kept, state = torch.load(f, map_location="cuda")
+    q = torch.nn.Parameter(kept.clone())
+    other = cake_muon([q], lr=0.9)
+    other.load_state_dict(state)
+    run(q, other, grads[2:])
+    assert torch.equal(p, q)

@@ -150,3 +150,19 @@ def test_orthogonalize_python_layer_takes_cuda_tensors_only(cake):
             cake.cake_orthogonalize(g)
         with pytest.raises(TypeError):
             cake.cake_muon_step(g, g, g, 0.1)
+
+
+def test_muon_momentum_stays_in_float32_across_a_reload():
+    import torch
+    from cake_on_cpu_b200.cake import cake_muon
+    w = [torch.nn.Parameter(torch.zeros(3, 4, dtype=torch.bfloat16)), torch.nn.Parameter(torch.zeros(2, 5))]
+    m = [torch.full((3, 4), 1 + 2.0 ** -20), torch.full((2, 5), 3.0)]
+    first = cake_muon(w, lr=0.3)
+    first.state[w[0]]["momentum"], first.state[w[1]]["momentum"] = m
+    again = [torch.nn.Parameter(p.detach().clone()) for p in w]
+    second = cake_muon(again, lr=0.1)
+    second.load_state_dict(first.state_dict())
+    assert second.param_groups[0]["lr"] == 0.3
+    for p, want in zip(again, m):
+        got = second.state[p]["momentum"]
+        assert got.dtype == torch.float32 and torch.equal(got, want) and got.data_ptr() != want.data_ptr()
