@@ -729,7 +729,7 @@ class Q4Weights:
     with values 0..15, or None for 8 everywhere.  ``group``: 32, 64 or 128.  ``in_features`` tells an odd number of input
     features from the even one above it.  ``Q4Weights.quantize(W)`` makes all of them from a matrix."""
 
-    FEW_ROWS = 64  # products of up to this many rows need no workspace
+    FEW_ROWS = 64  # products of up to this many rows never need a workspace
 
     def __init__(self, codes, scales, zeros=None, group=128, in_features=None, stream=None):
         import torch
@@ -784,7 +784,6 @@ class Q4Weights:
     def _bind(self):
         self._c = _Q4(self.packed.data_ptr(), self.out_features, self.in_features, self.group, self.scale_type, int(self.has_zeros))
         self._ref = ctypes.byref(self._c)
-        self._workspace = {}  # bytes needed by (rows, type, gradient)
 
     @staticmethod
     def quantize_codes(W, group=128, symmetric=True, scale_dtype=None, stream=None):
@@ -854,10 +853,9 @@ def _q4_product(dx, what, src, W4, cols_in, cols_out, bias, out, stream):
         buf = ws = None
         need = 0
         if rows > W4.FEW_ROWS:
-            need = W4._workspace.get((rows, t, dx))
-            if need is None:
-                need = W4._workspace[(rows, t, dx)] = lib().cakeb200_q4_workspace(W4._ref, rows, t, int(dx))
-            buf, ws = _workspace(need, W4.device)
+            need = lib().cakeb200_q4_workspace(W4._ref, rows, t, int(dx))
+            if need:
+                buf, ws = _workspace(need, W4.device)
         if dx:
             _check(lib().cakeb200_q4_linear_dx(W4._ref, p, ld, po, ldo, rows, t, ws, need, s))
         else:

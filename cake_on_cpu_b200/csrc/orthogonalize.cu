@@ -398,7 +398,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                 for (int b = (int) blockIdx.x * plane::DRAIN_WARPS + e.warp - 4; ok && b < total; b += (int) gridDim.x * plane::DRAIN_WARPS) {
                     TileAt at;
                     place(g, g.whole + b / PER_TILE, at.batch, tm, tn);
-                        at.row = tm * C::TILE_M + b % PER_TILE / WIDE * 32;
+                    at.row = tm * C::TILE_M + b % PER_TILE / WIDE * 32;
                     at.col = tn * C::BN + b % WIDE * 32;
                     if (at.row >= g.rows || at.col >= g.cols) continue;
                     float v[32];
@@ -510,7 +510,7 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
     volatile int* abort_flag = (volatile int*) (tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = p.cluster > 1 ? (int) ptx::cluster_ctarank() : 0, batch = (int) blockIdx.x / p.cluster;
-    const int c0 = rank * p.slice, columns = max(0, min(p.slice, p.n - c0)), squares = p.slice > 128 ? 2 : 1;
+    const int c0 = rank * p.slice, columns = min(p.slice, p.n - c0), squares = p.slice > 128 ? 2 : 1;
     const uint32_t done = ptx::smem_u32(bar);
     auto meet = [&]() {  // all CTAs of the cluster
         if (p.cluster > 1) ptx::cluster_sync_all();
@@ -626,18 +626,17 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
             }
         });
         if (in_square) {
-            const bool any = columns > 0;  // a last CTA without columns has nothing to add
             read(0, v);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = any ? v[j] * debias : 0.f;
-            if (width(1) > 0 && squares == 2) {
+            for (int j = 0; j < 32; j++) v[j] *= debias;
+            if (squares == 2 && width(1) > 0) {
                 read(256, u);
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], debias, v[j]);
             }
             read(128, u);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = any ? f * f * fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]) : 0.f;
+            for (int j = 0; j < 32; j++) v[j] = f * f * fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);
             if (p.cluster == 1) put_row(square, row, wide, v);
         }
         if (p.cluster > 1) {
@@ -942,7 +941,7 @@ bool fits_small(int m, int n, int batch, int sm_count, Small* p) {
     // One CTA per matrix is faster than the chain for any batch (2000 of 64 x 128: 0.60 ms, 1.09 in the chain).  Clusters are
     // as long as few wait for others: of 8 CTAs, 128 x 2048, 32 matrices 298 us (chain 320), 64 matrices 497 (474).
     if (c > 1 && (long long) batch * c > 3ll * sm_count) return false;
-    p->cluster = c;
+    p->cluster = c;  // n > 64 c, so that slices rounded up to 8 leave every CTA some columns
     p->slice = ((n + c - 1) / c + 7) / 8 * 8;
     return true;
 }

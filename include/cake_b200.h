@@ -150,7 +150,8 @@ int cakeb200_sgemm_after(const float* A, const float* B, float* C, int M, int N,
  *               cut along K ("k_pieces" 1).  The products inside cakeb200_orthogonalize and cakeb200_muon_step follow it
  *               too (1 = always pairs; rule: a model of their time), and "k_pieces" gives the number of parts the tiles of a
  *               last round are cut into there (1 = never cut).  With either option set, small matrices (up to 128 x 2048) go
- *               through the same kernel as large ones.
+ *               through the same kernel as large ones, and cakeb200_q4_linear and _linear_dx expand the weights from 65 rows
+ *               on whatever the sizes.
  * They take the place of the block sizes a caller of the reference forces with mcu / kcu / ncu
  * (reference include/cake.h:12-14, src/block_sizing.cpp:363-368) and of update_mr_nr
  * (src/block_sizing.cpp:78-83): on a GPU the blocks a caller may pin are the tile, the walk and
@@ -428,10 +429,10 @@ int cakeb200_unpack_B(float* B, const float* B_p, int K, int N, int p, const cak
  *     _linear_dx:  dx[r, k] = sum_n dy[r, n] w[n, k],              the gradient of _linear for its input
  *
  * x, bias, y, dy and dx share one type, CAKEB200_F32, _F16 or _BF16; leading dimensions are in elements; sums are FP32.  Few rows
- * are multiplied with the weights as they are, the scales applied in FP32; for many rows the weights are expanded first, a
- * slab at a time: exactly for FP32, to 17 bits for FP16, rounded once to BF16 for BF16.  _workspace tells how many bytes
- * of device memory, on a 1024-byte boundary, the call needs for that (0 for few rows: workspace may then be NULL); two
- * calls that may overlap on the GPU need one each.  A row with an infinity or a NaN gives results
+ * (up to 64, or up to 1024 of small weights) are multiplied with the weights as they are, the scales applied in FP32; for more the
+ * weights are expanded first, a slab at a time: exactly for FP32, to 17 bits for FP16, rounded once to BF16 for BF16.  _workspace
+ * tells how many bytes of device memory, on a 1024-byte boundary, the call needs for that (0 for few rows: workspace may then
+ * be NULL); two calls that may overlap on the GPU need one each.  A row with an infinity or a NaN gives results
  * that are not finite, and does not touch other rows.  The result must not overlap the operands.  `rows` may be 0.  Device
  * pointers of the current device only; work is enqueued on `stream`.  Results do not depend on timing.  Waits inside the
  * kernels are bounded; one that gave up shows in the status of the next blocking product (cakeb200_sgemm). */

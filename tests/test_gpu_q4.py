@@ -92,6 +92,34 @@ def test_linear_and_gradient(cake, shape, dtype):
     assert torch.equal(cake.cake_q4_linear_dx(dy.cuda(), W4), dx)
 
 
+@pytest.fixture(params=[False, True], ids=["", "expanded"])
+def expanded(cake, request):
+    """Second time round: products with more than 64 rows expand the weights whatever their sizes."""
+    cake.set_option("pair", 2 if request.param else 0)
+    yield request.param
+    cake.set_option("pair", 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[0] > 64] + [(65, 33, 129, 32), (257, 300, 512, 128), (1024, 70, 96, 32), (1025, 70, 96, 32)], ids=str)
+def test_more_than_64_rows_of_small_weights(cake, shape, dtype, expanded):
+    """Both ways, and where one ends.  Without the expansion the tolerance is that of few rows."""
+    import torch
+    rows, N, K, group = shape
+    rng = np.random.default_rng(rows + N)
+    codes, scales, zeros, w = _codes(rng, N, K, group, rows % 2 == 0, torch.bfloat16)
+    W4 = _weights(cake, codes, scales, zeros, group, K)
+    x, dy, b = _random(rng, (rows, K), dtype), _random(rng, (rows, N), dtype), _random(rng, (N,), dtype)
+    x64, dy64, b64 = x.double().numpy(), dy.double().numpy(), b.double().numpy()
+    many = expanded or rows > 1024
+    y = cake.cake_q4_linear(x.cuda(), W4, b.cuda())
+    _hold(y.double().cpu().numpy(), x64 @ w.T + b64, np.abs(x64) @ np.abs(w).T + np.abs(b64), np.sqrt(x64 ** 2 @ (w ** 2).T + b64 ** 2), K, dtype,
+          MANY[dtype] if many else 0.0)
+    dx = cake.cake_q4_linear_dx(dy.cuda(), W4)
+    _hold(dx.double().cpu().numpy(), dy64 @ w, np.abs(dy64) @ np.abs(w), np.sqrt(dy64 ** 2 @ w ** 2), N, dtype,
+          MANY[dtype] if many else 2.0 ** -22 if dtype == "float32" else 2.0 ** -14)
+
+
 @pytest.mark.parametrize("form", [(0, 0), (1, 1), (1, 3), (2, 1), (2, 4)], ids=str)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_many_rows_in_every_form(cake, dtype, form):
@@ -117,7 +145,7 @@ def test_many_rows_in_every_form(cake, dtype, form):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [1, 6, 40, 200])
-def test_strides_alignment_and_what_lies_around_the_result(cake, rows, dtype):
+def test_strides_alignment_and_what_lies_around_the_result(cake, rows, dtype, expanded):
     """Rows inside wider allocations, at an address that is only aligned to the element, and a result inside one."""
     import torch
     rng = np.random.default_rng(rows)
@@ -172,7 +200,7 @@ def test_leading_dimensions_vectors_and_no_rows(cake):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_values_that_are_not_finite_stay_in_their_row(cake, dtype):
+def test_values_that_are_not_finite_stay_in_their_row(cake, dtype, expanded):
     import torch
     rng = np.random.default_rng(11)
     N, K = 35, 150

@@ -59,11 +59,19 @@ def test_q4_workspace(cake):
     ref = ctypes.byref(w)
     assert all(L.cakeb200_q4_workspace(ref, rows, t, dx) == 0 for rows in (0, 1, 64) for t in (0, 1, 2) for dx in (0, 1))
     assert L.cakeb200_q4_workspace(ref, 65, 7, 0) == 0
+    # small products need none beyond that either: 2^29 multiply-adds of _linear, 2^28 of _linear_dx, 1024 rows
+    for n, k, rows, dx, none in ((300, 500, 65, 0, True), (300, 500, 1024, 0, True), (300, 500, 1025, 0, False), (1024, 1024, 512, 0, True),
+                                 (1024, 1024, 513, 0, False), (1024, 1024, 256, 1, True), (1024, 1024, 257, 1, False), (65536, 65536, 65, 1, False)):
+        assert (L.cakeb200_q4_workspace(ctypes.byref(_q4(n=n, k=k, group=128)), rows, 0, dx) == 0) == none, (n, k, rows, dx)
     up = lambda n: -(-n // 1024) * 1024
     # planes of x (65 x 500, rows of 504) and of W (300 x 500), and 6 tiles of 8 K blocks of 128 x 128 or 2 of 256 x 256
     parts = max(min(160, 3 * 8) * 65536, min(80, 2 * 8) * 262144)
-    for t, tx, tw in ((0, 3, 2), (1, 2, 2), (2, 1, 1)):
-        assert L.cakeb200_q4_workspace(ref, 65, t, 0) == up(tx * 65 * 504 * 2) + up(tw * 300 * 504 * 2) + parts
+    cake.set_option("k_pieces", 1)
+    try:
+        for t, tx, tw in ((0, 3, 2), (1, 2, 2), (2, 1, 1)):
+            assert L.cakeb200_q4_workspace(ref, 65, t, 0) == up(tx * 65 * 504 * 2) + up(tw * 300 * 504 * 2) + parts
+    finally:
+        cake.set_option("k_pieces", 0)
 
 
 def test_q4_python_layer_takes_cuda_tensors_only(cake):
