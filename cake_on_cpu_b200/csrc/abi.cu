@@ -70,10 +70,14 @@ DeviceState* device_state() {
     DeviceState* st = new DeviceState();
     st->device = dev;
     st->sm_count = prop.multiProcessorCount;
+    // the first call may be one that is being captured into a graph, which this thread's allocation is no part of
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     bool ok = cudaStreamCreateWithFlags(&st->stream, cudaStreamNonBlocking) == cudaSuccess;
     for (int i = 0; i < 6 && ok; i++) ok = cudaEventCreate(&st->ev[i]) == cudaSuccess;
     ok = ok && cudaMalloc((void**) &st->status_word, 256) == cudaSuccess;
-    ok = ok && cudaMemset(st->status_word, 0, 256) == cudaSuccess;
+    ok = ok && cudaMemsetAsync(st->status_word, 0, 256, st->stream) == cudaSuccess && cudaStreamSynchronize(st->stream) == cudaSuccess;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (!ok) {
         set_error("device state creation failed: %s", cudaGetErrorString(cudaGetLastError()));
         delete st;

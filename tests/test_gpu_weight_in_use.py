@@ -167,3 +167,59 @@ def test_resumed_training_goes_on_with_the_same_bits(cake):
     other.load_state_dict(state)
     run(q, other, grads[2:])
     assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("call", ["cake.cake_orthogonalize(g)", "cake.cake_orthogonalize(g[:, :30])", "cake.cake_muon_step(g.clone(), g, m, 0.1)",
+                                  "cake.cake_q4_linear(g, cake.Q4Weights(codes, scales))"])
+def test_first_call_of_a_process_is_captured(call):
+    """Nothing of the library has run on the device when the capture begins."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+import cake_on_cpu_b200 as cake
+g, m = torch.randn(300, 256, device="cuda"), torch.zeros(300, 256, device="cuda")
+codes, scales = torch.randint(0, 256, (64, 128), dtype=torch.uint8, device="cuda"), torch.ones((64, 2), dtype=torch.float16, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = CALL
+graph.replay()
+torch.cuda.synchronize()
+first = out.clone()
+m.zero_()
+assert torch.equal(first, CALL) and bool(torch.isfinite(first).all())
+""".replace("CALL", call)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_threads_with_streams_of_their_own(cake):
+    """Eight host threads at once, each with its stream: nobody's result changes."""
+    import threading
+    import torch
+    torch.manual_seed(0)
+    W4 = cake.Q4Weights.quantize(torch.randn(900, 700, device="cuda"))
+    gs = [torch.randn(96, 960, device="cuda") for _ in range(4)] + [torch.randn(300, 400, device="cuda") for _ in range(4)]
+    xs = [torch.randn(r, 700, device="cuda") for r in (1, 7, 33, 70, 300, 1100, 2, 16)]
+    want = [(cake.cake_orthogonalize(g), cake.cake_q4_linear(x, W4)) for g, x in zip(gs, xs)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                got = cake.cake_orthogonalize(gs[i]), cake.cake_q4_linear(xs[i], W4)
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
