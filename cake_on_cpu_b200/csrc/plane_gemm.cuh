@@ -619,7 +619,7 @@ inline Costs costs_of(int ta, int tb, int products, double between) {
 // Deals a product to `units` units of one form and returns its time by the model: 2 to the first MMA, 0.7 to read a tile's sums
 // out, 2.0 and 1.0 per 32 x 32 block of a warp, four of a pair's tile and two of a single one's; where parts are stored 1.0
 // and 0.7 instead, then 2.4 and 0.15 per part for each block that a warp joins.
-inline double plan(Tiling* g, int rows, int cols, int K, int symmetric, int batch, bool pair, int units, const Costs& costs) {
+inline double plan(Tiling* g, int rows, int cols, int K, int symmetric, int batch, bool pair, int units, const Costs& costs, bool may_cut = true) {
     const int side = pair ? 256 : 128, blocks = (K + BK - 1) / BK;
     g->rows = rows; g->cols = cols; g->K = K; g->symmetric = symmetric;
     g->tiles_m = (rows + side - 1) / side;
@@ -630,7 +630,7 @@ inline double plan(Tiling* g, int rows, int cols, int K, int symmetric, int batc
     g->whole = total; g->cut = 0; g->splits = 1;
     double best = (rounds + (left ? 1 : 0)) * round_time + 2 + (pair ? 8 : 2) + costs.between;
     const int forced = option_get(OPT_K_PIECES);
-    if (left == 0 || forced == 1) return best;
+    if (left == 0 || forced == 1 || !may_cut) return best;
     for (int splits = 1; splits <= std::min(units / left, blocks); splits++) {
         const int warps = units * (pair ? 2 : 1) * DRAIN_WARPS, per_warp = (left * (side / 32) * (side / 32) + warps - 1) / warps;
         const double time = rounds * round_time + (blocks + splits - 1) / splits * block_time + 0.7 + 2 + (pair ? 4 : 1.4) + costs.between +
@@ -687,7 +687,8 @@ int launch_form(const OperandMaps& a, const OperandMaps& b, const Problem& p, co
     return launch_kernel(join_kernel<PAIR, Epilogue>, blocks, 256u, 1u, 0, s, p, ep);
 }
 
-// One product (or p.batch of them).  `parts` of the problem holds parts_bytes(K blocks of all tiles) of the larger form.
+// One product (or p.batch of them).  `parts` of the problem holds parts_bytes(K blocks of all tiles) of the larger form; nullptr: no
+// tile is cut.
 template <class Format, int TA, int TB, int PRODUCTS, class Epilogue>
 int launch(const OperandMaps& a, const OperandMaps& b, Problem p, int rows, int cols, int K, const typename Epilogue::Args& ep, int sm_count,
            cudaStream_t s, int* launches) {
@@ -698,8 +699,8 @@ int launch(const OperandMaps& a, const OperandMaps& b, Problem p, int rows, int 
     const Costs costs = costs_of(TA, TB, PRODUCTS, 3.0);
     const int forced = option_get(OPT_PAIR);  // 1: pairs, 2: single SMs, 0: the faster by the model
     Tiling single, pair;
-    const double t_single = plan(&single, rows, cols, K, 0, p.batch, false, units_of(false, sm_count), costs);
-    const double t_pair = plan(&pair, rows, cols, K, 0, p.batch, true, units_of(true, sm_count), costs);
+    const double t_single = plan(&single, rows, cols, K, 0, p.batch, false, units_of(false, sm_count), costs, p.parts != nullptr);
+    const double t_pair = plan(&pair, rows, cols, K, 0, p.batch, true, units_of(true, sm_count), costs, p.parts != nullptr);
     const bool paired = forced ? forced == 1 : t_pair < t_single;
     p.t = paired ? pair : single;
     if (launches) *launches += p.t.cut ? 2 : 1;

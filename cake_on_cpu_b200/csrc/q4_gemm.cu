@@ -6,9 +6,11 @@
 // bytes per weight, once per slab whatever the number of rows.
 //
 // Planes per operand, by the type of x and y:
-//   BF16  x as it is, w rounded once to BF16, which is how a layer that keeps its weight in that type would hold it: its
-//         2^-8 is the result's own rounding.  One MMA per step.
-//   FP16  two planes each (x exactly, w to 2^-16): single FP16 planes could not hold every scale.  Three MMAs.
+//   BF16  x as it is, two planes of w (exactly).  Two MMAs per step.  w rounded to a single plane would cost 2^-9 of every
+//         product, as much again as the result's own rounding (error 2.4e-3 instead of 1.7e-3), and give a row other results
+//         alone than in a batch.  500 x 4096 x 4096 takes 51 us; 39 with a single plane.
+//   FP16  two planes each (both exactly): single FP16 planes could not hold every scale.  Three MMAs; the product of the
+//         second planes, below 2^-14 of the first ones', is left out.
 //   FP32  three planes of x (exactly), two of w (exactly: a 16-bit scale times a whole number below 16).  Five MMAs.
 // The gradient for the input reads the same planes of W down their columns.
 #include <algorithm>
@@ -27,7 +29,7 @@ namespace {
 constexpr long long SLAB = 1LL << 25;  // weights expanded at a time
 
 template <typename T> struct Terms;
-template <> struct Terms<__nv_bfloat16> { static constexpr int X = 1, W = 1, PRODUCTS = 1, CHUNK = 16; };
+template <> struct Terms<__nv_bfloat16> { static constexpr int X = 1, W = 2, PRODUCTS = 2, CHUNK = 16; };
 template <> struct Terms<__half> { static constexpr int X = 2, W = 2, PRODUCTS = 3, CHUNK = 16; };
 template <> struct Terms<float> { static constexpr int X = 3, W = 2, PRODUCTS = 5, CHUNK = 2; };
 
@@ -141,6 +143,7 @@ int slab_columns(const Q4View& w, bool dx) {
 struct Room {
     Planes x, w;
     float* parts;
+    bool cut;       // tiles may be cut along K, their parts stored
     size_t bytes;
 };
 
@@ -154,12 +157,16 @@ Room lay_out(char* base, const Q4View& w, int rows, bool dx) {
     at += plane::plane_bytes(Terms<T>::X, 1, rows, depth);
     m.w.base = (uint16_t*) (base + at);
     m.w.rows = dx ? w.N : slab; m.w.cols = dx ? slab : w.K; m.w.ld = plane::padded(m.w.cols); m.w.batches = 1;
-    at += plane::plane_bytes(Terms<T>::W, 1, m.w.rows, m.w.cols);
+    const size_t planes_end = at + plane::plane_bytes(Terms<T>::W, 1, m.w.rows, m.w.cols);
+    // Where tiles are never cut (option "k_pieces" 1) nothing is ever stored in the parts' room, and planes of w that x has no like of
+    // lie in it: workspaces of one plane are large enough then.
+    m.cut = option_get(OPT_K_PIECES) != 1;
+    at += plane::plane_bytes(m.cut ? Terms<T>::W : std::min(Terms<T>::X, Terms<T>::W), 1, m.w.rows, m.w.cols);
     m.parts = (float*) (base + at);
     const long long blocks = (depth + plane::BK - 1) / plane::BK;
     at += std::max(plane::parts_bytes(plane::count_tiles(rows, slab, 1, false, 128) * blocks, false),
                    plane::parts_bytes(plane::count_tiles(rows, slab, 1, false, 256) * blocks, true));
-    m.bytes = at;
+    m.bytes = std::max(at, planes_end);
     return m;
 }
 
@@ -205,7 +212,7 @@ int run(const Q4View& w, const void* in, long long ld_in, const void* bias, void
         problem.a_turn = plane::ALONG;
         problem.b_turn = dx ? plane::DOWN : plane::ALONG;
         problem.chunk = K::CHUNK;
-        problem.parts = m.parts;
+        problem.parts = m.cut ? m.parts : nullptr;
         problem.status_word = st->status_word;
         if ((rc = plane::launch<Bf16Planes, K::X, K::W, K::PRODUCTS, RowsEpilogue<T>>(map_x, map_w, problem, rows, n, depth, ep, st->sm_count, s, launches)))
             return rc;

@@ -430,7 +430,8 @@ int cakeb200_unpack_B(float* B, const float* B_p, int K, int N, int p, const cak
  *
  * x, bias, y, dy and dx share one type, CAKEB200_F32, _F16 or _BF16; leading dimensions are in elements; sums are FP32.  Few rows
  * (up to 64, or up to 1024 of small weights) are multiplied with the weights as they are, the scales applied in FP32; for more the
- * weights are expanded first, a slab at a time: exactly for FP32, to 17 bits for FP16, rounded once to BF16 for BF16.  _workspace
+ * weights are expanded first, a slab at a time, into pairs of BF16 that hold them exactly.  Either way a result of 16 bits is rounded
+ * once, from FP32 (for FP16 and more rows less than 2^-14 of the products' sizes is left out before).  _workspace
  * tells how many bytes of device memory, on a 1024-byte boundary, the call needs for that (0 for few rows: workspace may then
  * be NULL); two calls that may overlap on the GPU need one each.  A row with an infinity or a NaN gives results
  * that are not finite, and does not touch other rows.  The result must not overlap the operands.  `rows` may be 0.  Device
