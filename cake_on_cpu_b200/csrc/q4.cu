@@ -9,10 +9,10 @@
 // up to eight rows of x at once.  The products are exact and summed in FP32; the sum of a group is multiplied by its scale
 // in FP32 and added to the row's total, so scales are never rounded into the weights.  (tcgen05.mma would take the weights from shared memory: writing converted
 // codes there costs four times the bytes that are read from HBM.)
-//   Centred: 128 + q as BF16 or 1024 + q as FP16, the code in the last bits of the mantissa, and 128 + z or 1024 + z subtracted
-//   from every pair right away.
-//   FP16 x, up to eight rows: the code is a subnormal FP16, q 2^-24 or, left where it lies four bits up, 16 q 2^-24; the zero
-//   point is taken out of the group's sum with its sum of x, which a further MMA with ones gives for all output features.
+// The numbers are 128 + q as BF16 or 1024 + q as FP16, the code in the last bits of the mantissa, and 128 + z or 1024 + z is
+// subtracted from every pair right away, so that a product is w x / scale.  (Codes as subnormal FP16 and the zero point taken out of the
+// group's sum with its sum of x would save the subtractions, 7.0 to 6.3 us at one row of 4096 x 4096; but then the error goes with
+// the sum of |x| q: a large x under a weight of zero leaves its rounding in the result.)
 // A 32-bit x goes through the 16-bit multiplier as three terms x = x0 + x1 + x2 of 8 mantissa bits each (truncations,
 // so the split is exact and cannot overflow); their products are summed in FP32.
 #include <algorithm>
@@ -58,31 +58,11 @@ __device__ __forceinline__ void unpack_centred(uint32_t w, uint32_t sub_lo, uint
     }
 }
 
-// Codes as numbers of the MMA's type, for the forward product.  Centred, they are w / scale.  The other form saves the subtractions
-// and half of the shifts and leaves the zero point to the sums of x (SUM); DOWN_LO and DOWN_HI are what takes the sums of rows a and
-// a + 8 (registers 0, 2 and 1, 3) back to codes.
-template <typename T, bool CENTRED>
+// The MMA's type and the number of terms of x, for the forward product.
+template <typename T>
 struct Codes {
     using M = typename std::conditional<std::is_same<T, __half>::value, __half, __nv_bfloat16>::type;
-    static constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;  // of x
-    static constexpr bool SUM = false;
-    static constexpr float DOWN_LO = 1.f, DOWN_HI = 1.f;
-    static constexpr uint32_t ONE = 0;
-    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t sub_lo, uint32_t sub_hi, uint32_t* a) { unpack_centred<M>(w, sub_lo, sub_hi, a); }
-};
-template <> struct Codes<__half, false> {
-    using M = __half;
-    static constexpr int TERMS = 1;
-    static constexpr bool SUM = true;
-    static constexpr float DOWN_LO = 16777216.f, DOWN_HI = 1048576.f;
-    static constexpr uint32_t ONE = 0x3c003c00u;
-    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t, uint32_t, uint32_t* a) {
-        a[0] = w & 0x000f000fu;
-        a[1] = w & 0x00f000f0u;
-        w >>= 8;
-        a[2] = w & 0x000f000fu;
-        a[3] = w & 0x00f000f0u;
-    }
+    static constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
 };
 // Codes are read once and go past L1 into a queue of the lane's own in shared memory, so that many are on their way without
 // holding registers; a lane reads back what it asked for itself.
@@ -147,8 +127,8 @@ struct Q4Args {
 // B fragments of a lane for a block: features 32 h + 8 t + 0 .. 7, h = 0, 1, of its row, pairs of features to a register.  `x` points at
 // the first of them; `inside`: 16-byte loads are allowed and the block ends within the row.
 template <typename T>
-__device__ __forceinline__ void load_x(const T* x, bool inside, int left, uint32_t (*b)[Codes<T, true>::TERMS]) {
-    constexpr int TERMS = Codes<T, true>::TERMS;
+__device__ __forceinline__ void load_x(const T* x, bool inside, int left, uint32_t (*b)[Codes<T>::TERMS]) {
+    constexpr int TERMS = Codes<T>::TERMS;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const T* p = x + 32 * h;
@@ -223,12 +203,8 @@ constexpr int AHEAD = 3;  // steps in a lane's queue
 template <typename T, int NT, int R, int GROUPS, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
 q4_linear_kernel(const Q4Args p) {
-    // FP16 with ones instead of subtractions pays up to eight rows, where unpacking is what takes the time (us, 4096 x 4096: 6.6,
-    // centred 7.2; 16384 x 512: 5.3 and 6.1).  With more rows the products do, and those with ones are half as many (16384 x 8192, 32
-    // rows: 55.0, centred 51.3).  BF16 would need an offset in the sums and gains nothing (27.3, centred 26.3).
-    using C = Codes<T, !std::is_same<T, __half>::value || (NT > 1)>;
-    using M = typename C::M;
-    constexpr int TERMS = C::TERMS;
+    using M = typename Codes<T>::M;
+    constexpr int TERMS = Codes<T>::TERMS;
     constexpr int E = R * NT * 128;
     constexpr int QUEUE = AHEAD * R * 64;  // of a warp, in 16-byte pieces
     // with few columns there are registers for what keeps a lone warp busy: x of a whole step loaded at its start, and two chains of
@@ -327,7 +303,7 @@ q4_linear_kernel(const Q4Args p) {
                 advance(scales_cursor);
             }
             fetch_wait<AHEAD - 1>();
-            float acc[R][NT][CHAINS][4], sums[NT][CHAINS][4];
+            float acc[R][NT][CHAINS][4];
 #pragma unroll
             for (int half = 0; half < 2; half++) {  // a block of 64 features
                 if (HALVES == 1) load(half);
@@ -341,18 +317,10 @@ q4_linear_kernel(const Q4Args p) {
                         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                             for (int i = 0; i < CHAINS * 4; i++) {
-                                sums[nt][i / 4][i % 4] = 0.f;
 #pragma unroll
                                 for (int r = 0; r < R; r++) acc[r][nt][i / 4][i % 4] = 0.f;
                             }
                         }
-                    }
-                    if (C::SUM) {
-                        const uint32_t ones[4] = {C::ONE, C::ONE, C::ONE, C::ONE};
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int j = 2 * part; j < 2 * part + 2; j++) mma<M>(sums[nt][j % CHAINS], ones, b[half % HALVES][nt][2 * j][0], b[half % HALVES][nt][2 * j + 1][0]);
                     }
                     uint2 c[R];
 #pragma unroll
@@ -363,7 +331,7 @@ q4_linear_kernel(const Q4Args p) {
                         for (int r = 0; r < R; r++) {
                             const uint32_t z = now[r].zeros[g / 2] >> (16 * (g & 1));
                             uint32_t w[4];
-                            C::unpack(j & 1 ? c[r].y : c[r].x, zero_pair<M>(z & 15u), zero_pair<M>((z >> 8) & 15u), w);
+                            unpack_centred<M>(j & 1 ? c[r].y : c[r].x, zero_pair<M>(z & 15u), zero_pair<M>((z >> 8) & 15u), w);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -374,26 +342,18 @@ q4_linear_kernel(const Q4Args p) {
                     if (last) {  // the group is complete
 #pragma unroll
                         for (int r = 0; r < R; r++) {
-                            const uint32_t z = now[r].zeros[g / 2] >> (16 * (g & 1));
                             const float s_lo = q4_scale((uint16_t) now[r].scales[g], p.w.scale_bf16), s_hi = q4_scale((uint16_t) (now[r].scales[g] >> 16), p.w.scale_bf16);
-                            const float z_lo = s_lo * (float) (z & 15u), z_hi = s_hi * (float) ((z >> 8) & 15u);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                                 for (int i = 0; i < 2; i++) {
-                                    float lo = acc[r][nt][0][i], hi = acc[r][nt][0][i + 2], x_sum = sums[nt][0][i];
+                                    float lo = acc[r][nt][0][i], hi = acc[r][nt][0][i + 2];
                                     if (CHAINS == 2) {
                                         lo += acc[r][nt][CHAINS - 1][i];
                                         hi += acc[r][nt][CHAINS - 1][i + 2];
-                                        x_sum += sums[nt][CHAINS - 1][i];
                                     }
-                                    if (C::SUM) {
-                                        total[r][nt][i] += fmaf(s_lo * C::DOWN_LO, lo, -z_lo * x_sum);
-                                        total[r][nt][i + 2] += fmaf(s_hi * C::DOWN_HI, hi, -z_hi * x_sum);
-                                    } else {
-                                        total[r][nt][i] = fmaf(s_lo, lo, total[r][nt][i]);
-                                        total[r][nt][i + 2] = fmaf(s_hi, hi, total[r][nt][i + 2]);
-                                    }
+                                    total[r][nt][i] = fmaf(s_lo, lo, total[r][nt][i]);
+                                    total[r][nt][i + 2] = fmaf(s_hi, hi, total[r][nt][i + 2]);
                                 }
                             }
                         }

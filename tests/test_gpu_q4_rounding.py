@@ -57,3 +57,28 @@ def test_16_bit_results_are_rounded_once(cake, rows, group, dtype, expanded):
         err = np.linalg.norm(got.double().cpu().numpy() - want)
         tol = _one_rounding(want, dtype) + (np.sqrt(depth / 16 + 40) * 2.0 ** -22 + 2.0 ** -14) * np.linalg.norm(walk)
         assert err <= tol, (err / np.linalg.norm(want), tol / np.linalg.norm(want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 7, 12, 40, 90])
+def test_large_features_of_zero_weights_leave_nothing(cake, rows, dtype, expanded):
+    """Codes equal to their zero point are weights of zero, exactly, however large the feature is: errors go with sum |x| |w|."""
+    import torch
+    rng = np.random.default_rng(rows)
+    N, K, group = 40, 384, 128
+    for zeros in (False, None):
+        z = rng.integers(0, 16, (N, K // group), dtype=np.uint8) if zeros is None else False
+        q = rng.integers(0, 16, (N, K), dtype=np.uint8)
+        for k in (5, 130, 131, 300):
+            q[:, k] = 8 if z is False else z[:, k // group]
+        W4, w = _make(cake, rng, N, K, group, z, torch.float16, q)
+        t = getattr(torch, dtype)
+        x = torch.from_numpy(0.1 * rng.standard_normal((rows, K)).astype(np.float32))
+        x[:, 5], x[:, 130], x[:, 131], x[:, 300] = 60000.0, -31000.0, 47001.0, 12345.0
+        x = x.to(t)
+        got = cake.cake_q4_linear(x.cuda(), W4).double().cpu().numpy()
+        a = x.double().numpy()
+        want, S = a @ w.T, np.abs(a) @ np.abs(w).T
+        operand = 0.0 if rows <= 64 or not expanded else {"float32": 2.0 ** -22, "float16": 2.0 ** -14, "bfloat16": 0.0}[dtype]
+        tol = torch.finfo(t).eps / 2 * np.abs(want) * (1 + 2 ** -20) + ((K / 16 + 40) * 2.0 ** -22 + operand) * S
+        assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
