@@ -30,6 +30,15 @@ using plane::Fp16Planes;
 
 constexpr int TERMS = 2;
 constexpr int NORM_BLOCKS = 512;  // partial sums of squares per matrix
+// K blocks of 64 between folds of the main accumulator, whatever the result's type.  4096 x 4096 FP32 with folds every 64 / 128 / 256 /
+// 1024 of K: errors against 64 bits 1.2e-6, 1.6e-6, 3.1e-6, 1.1e-5 (a plain FP32 evaluation: 4.8e-6), 3.36 / 3.16 / 3.05 / 2.97 ms.  With
+// folds every 1024 a BF16 result of 1024 x 4096 differs from the correctly rounded one by 1.7e-4, with these by 9e-5.
+constexpr int FOLD = 2;
+// The tensor core truncates the sum that it adds to.  n additions that grow it evenly, as squares do on the diagonals of X X^T and
+// of its square, lose half a unit in the last place each, on average over the mantissas 0.36 2^-23 of the sum so far, which is (n + 1) / 2
+// times the last one's: that part has a sign, and is put back into those two products.  Not into Q X, whose sums are of either sign
+// and, while X is small, of a single term.
+constexpr float EVEN_GROWTH = 0.18f * 1.1920929e-7f;
 
 // eight consecutive elements; `vec`: all eight exist and the address is 16-byte aligned
 __device__ __forceinline__ void get8(const float* p, int n, bool vec, float* v) {
@@ -243,7 +252,7 @@ struct Product : plane::Tiling {
 struct Chain {
     Planes x[2], p, q;           // step s reads x[s % 2] and writes the other
     Product gram, poly, apply, last;
-    int batch, steps, chunk;
+    int batch, steps;
     float f0;                    // X_0 is held 1 / f0 times itself
     float ka, kb, kc;
     float* parts;                // of cut tiles: [slot][32 x 32 block][1024]
@@ -326,7 +335,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                 const Product& g = product(i);
                 for (int k = 0; ok && item_at(g, k, unit, units, w); k++) {
                     place(g, w.tile, batch, tm, tn);
-                    ok = e.multiply(turn(g.a, tm), turn(g.b, tn), w.kb0, w.kb1, c.chunk);
+                    ok = e.multiply(turn(g.a, tm), turn(g.b, tn), w.kb0, w.kb1, FOLD);
                 }
             }
         }
@@ -378,7 +387,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                 });
             };
             for (int k = 0; ok && item_at(g, k, unit, units, w); k++) {
-                ok = e.collect(w.kb0, w.kb1, c.chunk, sum);
+                ok = e.collect(w.kb0, w.kb1, FOLD, g.K, kind < 2 ? EVEN_GROWTH : 0.f, sum);
                 if (!ok) break;
                 TileAt at;
                 place(g, w.tile, at.batch, tm, tn);
@@ -475,9 +484,9 @@ __device__ __forceinline__ void get_row(const uint8_t* square, int r, int c0, fl
     }
 }
 
-// D(main) = A B, D(cross) (+)= its two smaller products: squares a and b, b along its rows or down its columns; n columns of
-// the result, `depth` of K, both multiples of 32
-__device__ __forceinline__ void square_product(uint32_t main, uint32_t cross, uint32_t a, uint32_t b, bool down, bool more, int n, int depth) {
+// D(main) + D(main2) = A B, D(cross) (+)= its two smaller products: squares a and b, b along its rows or down its columns; n columns of
+// the result, `depth` of K, both multiples of 32.  main2 takes the second half of K, or is main.
+__device__ __forceinline__ void square_product(uint32_t main, uint32_t main2, uint32_t cross, uint32_t a, uint32_t b, bool down, bool more, int n, int depth) {
     const uint32_t idesc = plane::idesc_16(Fp16Planes::FORMAT, 128, n) | (down ? 1u << 16 : 0u);
     // down: 64 columns further is a sub-tile (leading offset), 16 rows of K are 2048 bytes; along: 16 of K are 32 bytes, 64 a sub-tile
     const uint64_t da = ptx::make_kmajor_sw128_desc(a), db = ptx::make_kmajor_sw128_desc(b) + (down ? (uint64_t) ((SUB_BYTES >> 4) - 1) << 16 : 0);
@@ -487,7 +496,8 @@ __device__ __forceinline__ void square_product(uint32_t main, uint32_t cross, ui
         const uint32_t plane = 2 * SUB_BYTES >> 4, first = more || k > 0;
         plane::umma<false>(cross, da + plane + ka, db + kb, idesc, first);
         plane::umma<false>(cross, da + ka, db + plane + kb, idesc, 1u);
-        plane::umma<false>(main, da + ka, db + kb, idesc, k > 0);
+        const bool second = main2 != main && k >= depth / 32;
+        plane::umma<false>(second ? main2 : main, da + ka, db + kb, idesc, k > (second ? depth / 32 : 0));
     }
 }
 
@@ -592,8 +602,8 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
     // room for the parts: the second square of X if there is none, else the place of P and Q, which then needs two more meetings
     const bool apart = squares == 1;
     uint8_t* parts = apart ? x + SQUARE_BYTES : square;
-    // eight additions into an accumulator of 128 of K, see plane::Engine::collect
-    const float debias = 1.f + 0.18f * 1.1920929e-7f * 9.f;
+    // what makes up for truncation in a square's main sums over `depth` values, `padded` with zeros
+    auto grown = [&](int depth, int padded) { return 1.f + EVEN_GROWTH * (float) (min((depth + 15) / 16, padded / (apart ? 32 : 16)) + 1); };
     uint32_t phase = 0;
     // shared memory that this thread wrote is there for the MMAs of all; then one thread issues them and all wait
     auto multiply = [&](auto issue) {
@@ -615,6 +625,16 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         ptx::tmem_ld_wait();
     };
 
+    // with one square of X there is tensor memory to add up the two halves of K apart: half as many truncated additions each
+    const uint32_t second = apart ? 256 : 0;
+    auto read_main = [&](uint32_t column, float* v, float* u) {
+        read(column, v);
+        if (!apart) return;
+        read(column + 256, u);
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] += u[j];
+    };
+
     for (int step = 0; step < p.steps; step++) {
         const float f = step == 0 ? p.f0 : 1.f;
         float v[32], u[32];
@@ -622,17 +642,17 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         multiply([&]() {
             for (int q = 0; q < squares; q++) {
                 const uint32_t at = ptx::smem_u32(x + q * SQUARE_BYTES);
-                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 128, at, at, false, q > 0, m32, width(q));
+                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * (apart ? 1 : q), tmem + 128, at, at, false, q > 0, m32, width(q));
             }
         });
         if (in_square) {
             read(0, v);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] *= debias;
-            if (squares == 2 && width(1) > 0) {
+            for (int j = 0; j < 32; j++) v[j] *= grown(columns, width(0));
+            if (apart || width(1) > 0) {
                 read(256, u);
 #pragma unroll
-                for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], debias, v[j]);
+                for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], apart ? grown(columns, width(0)) : grown(columns - 128, width(1)), v[j]);
             }
             read(128, u);
 #pragma unroll
@@ -695,12 +715,12 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         }
         // ---- Q, in place of P
         const uint32_t sq = ptx::smem_u32(square);
-        multiply([&]() { square_product(tmem, tmem + 128, sq, sq, false, false, m32, m32); });
+        multiply([&]() { square_product(tmem, tmem + second, tmem + 128, sq, sq, false, false, m32, m32); });
         if (in_square) {
-            read(0, v);
+            read_main(0, v, u);
             read(128, u);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j] * debias);
+            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j] * grown(p.m, m32));
             get_row(square, row, wide, u);
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = p.kc * v[j] + p.kb * u[j] + (row == wide + j && row < p.m ? p.ka : 0.f);
@@ -709,14 +729,14 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         // ---- X
         multiply([&]() {
             for (int q = 0; q < squares; q++)
-                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * q + 128, sq, ptx::smem_u32(x + q * SQUARE_BYTES), true, false, width(q), m32);
+                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * q + second, tmem + 256 * q + 128, sq, ptx::smem_u32(x + q * SQUARE_BYTES), true, false, width(q), m32);
         });
         for (int q = 0; q < squares; q++) {
             if (quarter * 32 >= m32 || wide >= width(q)) continue;
-            read(256 * q, v);
+            read_main(256 * q, v, u);
             read(256 * q + 128, u);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j] * debias);
+            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);
             if (step + 1 < p.steps) {
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] *= f;
@@ -969,10 +989,10 @@ int launch_small(const Source<T>& src, const Small& p, const typename Last::Args
     return CAKEB200_OK;
 }
 
-// From the source to the last X, which goes through `Last`.  chunk: K blocks of 64 between folds of the main accumulator.
+// From the source to the last X, which goes through `Last`.
 // early: the results of one matrix may be stored while other matrices are still read.
 template <typename T, class Last>
-int run(const Source<T>& src, int batch, bool early, const Coefficients& k, int chunk, void* workspace, typename Last::Args last, DeviceState* st, cudaStream_t s) {
+int run(const Source<T>& src, int batch, bool early, const Coefficients& k, void* workspace, typename Last::Args last, DeviceState* st, cudaStream_t s) {
     const int rows = src.rows, cols = src.cols;
     const bool tall = rows > cols;
     const int m = tall ? cols : rows, n = tall ? rows : cols;
@@ -1005,7 +1025,7 @@ int run(const Source<T>& src, int batch, bool early, const Coefficients& k, int 
 
     Chain c = {};
     c.x[0] = l.x[0]; c.x[1] = l.x[1]; c.p = l.p; c.q = l.q;
-    c.batch = batch; c.steps = k.steps; c.chunk = chunk;
+    c.batch = batch; c.steps = k.steps;
     c.f0 = down;
     c.ka = k.a; c.kb = k.b; c.kc = k.c;
     c.parts = l.parts;
@@ -1034,15 +1054,11 @@ int run(const Source<T>& src, int batch, bool early, const Coefficients& k, int 
     return rc;
 }
 
-// An FP32 result is folded every 128 of K, a BF16 one every 1024.  Errors of 4096 x 4096 FP32 against 64 bits with folds every
-// 64 / 128 / 256 / 1024: 1.2e-6, 1.3e-6, 1.7e-6, 4.7e-6 (a plain FP32 evaluation: 2.9e-6); times 3.56 / 3.53 / 3.51 / 3.40 ms.
-int chunk_for(int type) { return type == CAKEB200_F32 ? 2 : 16; }
-
 bool known(int type) { return type == CAKEB200_F32 || type == CAKEB200_BF16; }
 
 template <typename T>
 int orthogonalize(const void* G, long long ldg, long long stride_g, void* out, long long ldo, long long stride_o, int rows, int cols, int batch,
-                  const Coefficients& k, int chunk, void* workspace, DeviceState* st, cudaStream_t s) {
+                  const Coefficients& k, void* workspace, DeviceState* st, cudaStream_t s) {
     Source<T> src = {};
     src.g = matrix((const T*) G, ldg, stride_g, rows, batch);
     src.rows = rows;
@@ -1052,12 +1068,12 @@ int orthogonalize(const void* G, long long ldg, long long stride_g, void* out, l
     const long long size = sizeof(T), reach_g = (rows - 1) * ldg + cols + (batch - 1) * stride_g, reach_o = (rows - 1) * ldo + cols + (batch - 1) * stride_o;
     const bool same = G == out && ldg == ldo && (batch == 1 || stride_g == stride_o);
     const bool early = batch == 1 || same || (stride_g >= 0 && !overlap(G, reach_g * size, reach_g * size, out, reach_o * size, reach_o * size, 1));
-    return run<T, ResultEpilogue<T>>(src, batch, early, k, chunk, workspace, last, st, s);
+    return run<T, ResultEpilogue<T>>(src, batch, early, k, workspace, last, st, s);
 }
 
 template <typename TW, typename TG>
 int muon(void* W, long long ldw, const void* G, long long ldg, float* M, long long ldm, int rows, int cols, double lr, double mu, int nesterov,
-         double weight_decay, double scale, const Coefficients& k, int chunk, void* workspace, DeviceState* st, cudaStream_t s) {
+         double weight_decay, double scale, const Coefficients& k, void* workspace, DeviceState* st, cudaStream_t s) {
     Source<TG> src = {};
     src.g = matrix((const TG*) G, ldg, 0, rows, 1);
     src.m = M;
@@ -1069,7 +1085,7 @@ int muon(void* W, long long ldw, const void* G, long long ldg, float* M, long lo
     src.rows = rows;
     src.cols = cols;
     typename StepEpilogue<TW>::Args last = {matrix((TW*) W, ldw, 0, rows, 1), rows, cols, 1.f, (float) (1.0 - lr * weight_decay), (float) (lr * scale)};
-    return run<TG, StepEpilogue<TW>>(src, 1, true, k, chunk, workspace, last, st, s);
+    return run<TG, StepEpilogue<TW>>(src, 1, true, k, workspace, last, st, s);
 }
 
 }  // namespace
@@ -1111,9 +1127,8 @@ int cakeb200_orthogonalize(const void* G, long long ldg, long long stride_g, voi
     if (!on_current_device(G) || !on_current_device(out) || !on_current_device(workspace))
         return bad(who, "operands must be device pointers of the current device");
     cudaStream_t s = (cudaStream_t) stream;
-    const int chunk = chunk_for(type);
-    if (type == CAKEB200_F32) return orthogonalize<float>(G, ldg, stride_g, out, ldo, stride_o, rows, cols, batch, k, chunk, workspace, st, s);
-    return orthogonalize<__nv_bfloat16>(G, ldg, stride_g, out, ldo, stride_o, rows, cols, batch, k, chunk, workspace, st, s);
+    if (type == CAKEB200_F32) return orthogonalize<float>(G, ldg, stride_g, out, ldo, stride_o, rows, cols, batch, k, workspace, st, s);
+    return orthogonalize<__nv_bfloat16>(G, ldg, stride_g, out, ldo, stride_o, rows, cols, batch, k, workspace, st, s);
 }
 
 int cakeb200_muon_step(void* W, long long ldw, int type_w, const void* G, long long ldg, int type_g, float* M, long long ldm, int rows, int cols,
@@ -1142,7 +1157,7 @@ int cakeb200_muon_step(void* W, long long ldw, int type_w, const void* G, long l
     cudaStream_t s = (cudaStream_t) stream;
     nesterov = nesterov ? 1 : 0;
 #define CAKE_MUON(TW, TG) \
-    return muon<TW, TG>(W, ldw, G, ldg, M, ldm, rows, cols, lr, momentum, nesterov, weight_decay, scale, k, chunk_for(type_w), workspace, st, s)
+    return muon<TW, TG>(W, ldw, G, ldg, M, ldm, rows, cols, lr, momentum, nesterov, weight_decay, scale, k, workspace, st, s)
     if (type_w == CAKEB200_F32) {
         if (type_g == CAKEB200_F32) CAKE_MUON(float, float);
         CAKE_MUON(float, __nv_bfloat16);

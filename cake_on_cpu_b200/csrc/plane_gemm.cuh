@@ -383,33 +383,28 @@ struct Engine {
         return true;
     }
 
-    // Drain warps: the sums of those K blocks, this warp's 32 rows x COLS columns, a row per lane.  A warp may only touch lanes
+    // Drain warps: the sums of those K blocks (of a product over K), this warp's 32 rows x COLS columns, a row per lane.  A warp may only touch lanes
     // [32 * (warp % 4), +32) of tensor memory, so two warps share a quarter of the rows and take half of the columns each.
     __device__ __forceinline__ int quarter() const { return warp & 3; }
     __device__ __forceinline__ int half() const { return (warp - 4) >> 2; }
-    __device__ __forceinline__ bool collect(int kb0, int kb1, int chunk, float (&sum)[COLS]) {
+    __device__ __forceinline__ bool collect(int kb0, int kb1, int chunk, int K, float growth, float (&sum)[COLS]) {
         const uint32_t at = ((uint32_t) (quarter() * 32) << 16) + (uint32_t) (half() * COLS);
         float v[64];
+#pragma unroll
+        for (int j = 0; j < COLS; j++) sum[j] = 0.f;
         for (int kb = kb0; kb < kb1; kb += chunk) {
             bool ok = mbar_wait_for(main_full(), fold_phase, abort_flag, status_word, 540, WAIT_LIMIT_NS, 32);
             if (!__all_sync(0xffffffffu, ok)) return false;  // the tensor-memory loads below need the whole warp
             fold_phase ^= 1;
             tcgen05_fence_after();
-            // Truncation of a sum of n additions that grow it evenly loses half a unit in the last place each time, on
-            // average over the mantissas 0.36 2^-23 of the sum so far, (n + 1) / 2 times that of the last one: the part
-            // of it that has a sign is put back here (measured on 4096 x 4096 FP32: error 2.0e-6 -> 1.3e-6).
-            const float up = 1.f + 0.18f * 1.1920929e-7f * (float) (min(chunk, kb1 - kb) * (BK / UMMA_K) + 1);
+            // sums that grow evenly: `growth` of what is read for each addition that had something to add, and one more
+            const float up = 1.f + growth * (float) (min(min(chunk, kb1 - kb) * (BK / UMMA_K), (K - kb * BK + UMMA_K - 1) / UMMA_K) + 1);
 #pragma unroll
             for (int c = 0; c < COLS; c += 64) {
                 tmem_ld64(tmem_main + at + (uint32_t) c, v);
                 tmem_ld_wait();
-                if (kb == kb0) {
 #pragma unroll
-                    for (int j = 0; j < 64; j++) sum[c + j] = v[j] * up;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 64; j++) sum[c + j] = fmaf(v[j], up, sum[c + j]);
-                }
+                for (int j = 0; j < 64; j++) sum[c + j] = fmaf(v[j], up, sum[c + j]);
             }
             tcgen05_fence_before();
             if (lane == 0) mbar_arrive_t<PAIR>(main_empty());
@@ -476,7 +471,7 @@ plane_gemm_kernel(const __grid_constant__ OperandMaps map_a, const __grid_consta
         many_registers();
         float sum[C::COLS];
         for (int k = 0; item_at(p.t, k, unit, units, w); k++) {
-            if (!e.collect(w.kb0, w.kb1, p.chunk, sum)) break;
+            if (!e.collect(w.kb0, w.kb1, p.chunk, p.t.K, 0.f, sum)) break;
             TileAt at;
             place(p.t, w.tile, at.batch, tm, tn);
             const int row = (int) e.rank * BM + e.quarter() * 32;

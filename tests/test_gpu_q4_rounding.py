@@ -82,3 +82,34 @@ def test_large_features_of_zero_weights_leave_nothing(cake, rows, dtype, expande
         operand = 0.0 if rows <= 64 or not expanded else {"float32": 2.0 ** -22, "float16": 2.0 ** -14, "bfloat16": 0.0}[dtype]
         tol = torch.finfo(t).eps / 2 * np.abs(want) * (1 + 2 ** -20) + ((K / 16 + 40) * 2.0 ** -22 + operand) * S
         assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [3, 70, 300])
+def test_sums_of_one_product_are_exact(cake, rows, dtype, expanded):
+    """One feature per row, the rest zero: x = 1 gives the weight itself, rounded once."""
+    import torch
+    rng = np.random.default_rng(rows)
+    N, K, group = 100, 330, 64
+    W4, w = _make(cake, rng, N, K, group, None, torch.float16)
+    t = getattr(torch, dtype)
+    for dx in (False, True):
+        n = N if dx else K
+        at = rng.integers(0, n, rows)
+        x = torch.zeros((rows, n), dtype=t)
+        x[torch.arange(rows), torch.from_numpy(at)] = 1.0
+        y = (cake.cake_q4_linear_dx if dx else cake.cake_q4_linear)(x.cuda(), W4)
+        want = torch.from_numpy(w[at] if dx else w[:, at].T.copy()).to(t)
+        assert torch.equal(y.cpu(), want)
+
+
+@pytest.mark.parametrize("rows", [3, 65, 200])
+def test_ends_of_the_range_of_fp32(cake, rows, expanded):
+    """The terms of an FP32 x neither overflow nor lose the smallest normal values, with few rows and with many."""
+    import torch
+    rng = np.random.default_rng(rows)
+    W4, _ = _make(cake, rng, 16, 200, 64, False, torch.float16, np.full((16, 200), 9, np.uint8), 1.0)  # w = 1
+    x = torch.zeros((rows, 200), device="cuda")
+    x[0, 3], x[1, 5], x[2, 0] = torch.finfo(torch.float32).max, 1.1754944e-38 * 65536, 1 + 2.0 ** -23
+    y = cake.cake_q4_linear(x, W4)
+    assert torch.equal(y, x.sum(1, keepdim=True).expand(rows, 16))
