@@ -727,11 +727,13 @@ class Q4Weights:
     ``codes``: uint8 CUDA tensor (out_features, ceil(in_features / 2)), two codes to a byte, the even input feature in the
     low half.  ``scales``: float16 or bfloat16, (out_features, ceil(in_features / group)).  ``zeros``: uint8 of the same shape
     with values 0..15, or None for 8 everywhere.  ``group``: 32, 64 or 128.  ``in_features`` tells an odd number of input
-    features from the even one above it.  ``Q4Weights.quantize(W)`` makes all of them from a matrix."""
+    features from the even one above it.  ``Q4Weights.quantize(W)`` makes all of them from a matrix.
+
+    Given zero points are looked at once by the host, in the order of ``stream`` (which it waits for; not while it is captured)."""
 
     FEW_ROWS = 64  # products of up to this many rows never need a workspace
 
-    def __init__(self, codes, scales, zeros=None, group=128, in_features=None, stream=None):
+    def __init__(self, codes, scales, zeros=None, group=128, in_features=None, stream=None, _checked=False):
         import torch
         for t, what in ((codes, "codes"), (scales, "scales")) + (((zeros, "zeros"),) if zeros is not None else ()):
             if not (_is_torch(t) and t.is_cuda):
@@ -754,11 +756,12 @@ class Q4Weights:
         _need_shape(scales, (self.out_features, groups), "scales")
         if zeros is not None:
             _need_shape(zeros, (self.out_features, groups), "zeros")
-            if not torch.cuda.is_current_stream_capturing() and int(zeros.max()) > 15:
-                raise ValueError("zero points are 0..15")
         self.device, self.has_zeros = codes.device, zeros is not None
         n = lib().cakeb200_q4_packed_bytes(self.out_features, self.in_features, self.group, int(zeros is not None))
         with _on_device(self.device, stream) as s:
+            # looked at on the stream that they are read on: what wrote them may still be queued there
+            if zeros is not None and not _checked and not torch.cuda.is_current_stream_capturing() and int(zeros.max()) > 15:
+                raise ValueError("zero points are 0..15")
             self.packed = torch.empty(n, dtype=torch.uint8, device=self.device)
             self._bind()
             _check(lib().cakeb200_q4_pack(_vp(codes.data_ptr()), codes.stride(0), _vp(scales.data_ptr()),
@@ -811,7 +814,7 @@ class Q4Weights:
     @classmethod
     def quantize(cls, W, group=128, symmetric=True, scale_dtype=None, stream=None):
         codes, scales, zeros = cls.quantize_codes(W, group, symmetric, scale_dtype, stream)
-        return cls(codes, scales, zeros, group=group, in_features=W.shape[1], stream=stream)  # they were allocated on `stream`
+        return cls(codes, scales, zeros, group=group, in_features=W.shape[1], stream=stream, _checked=True)  # they were allocated on `stream`
 
     def dequantize(self, dtype=None, out=None, stream=None):
         """The matrix (out_features, in_features) the codes stand for."""

@@ -1,0 +1,74 @@
+"""4-bit weights made on a stream of their own, copied, pickled and reloaded."""
+import copy
+import io
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _busy(stream):
+    """A few milliseconds of work on a stream."""
+    import torch
+    with torch.cuda.stream(stream):
+        a = torch.randn(6000, 6000, device="cuda")
+        for _ in range(6):
+            a = a @ a * 1e-2
+    return a
+
+
+def test_quantising_on_another_stream(cake):
+    """Zero points are checked where they are written, not on the current stream: memory that held other bytes
+    before is handed out again while the stream is still busy."""
+    import torch
+    torch.manual_seed(0)
+    W = torch.randn(512, 640, device="cuda")
+    want = cake.Q4Weights.quantize(W, 64, symmetric=False)
+    codes, scales, zeros = cake.Q4Weights.quantize_codes(W, 64, symmetric=False)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            old = [torch.full(s, 255, dtype=torch.uint8, device="cuda") for s in ((512, 320), (512, 20), (512, 10)) for _ in range(4)]
+        torch.cuda.synchronize()
+        del old
+        keep = _busy(side)
+        got = cake.Q4Weights.quantize(W, 64, symmetric=False, stream=side)
+        side.synchronize()
+        assert torch.equal(got.packed, want.packed)
+        # the constructor on that stream, with arrays written on it just before
+        keep = _busy(side)
+        with torch.cuda.stream(side):
+            late = torch.full(zeros.shape, 255, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        keep = _busy(side)
+        with torch.cuda.stream(side):
+            late.copy_(zeros)
+        got = cake.Q4Weights(codes, scales, late, group=64, stream=side)
+        side.synchronize()
+        assert torch.equal(got.packed, want.packed)
+        with torch.cuda.stream(side):
+            keep = _busy(side)
+            late.fill_(16)
+        with pytest.raises(ValueError):
+            cake.Q4Weights(codes, scales, late, group=64, stream=side)
+        del keep
+
+
+def test_weights_are_made_while_their_stream_is_captured(cake):
+    """The zero points cannot be looked at in the middle of a capture, whichever stream is the current one."""
+    import torch
+    torch.manual_seed(1)
+    W = torch.randn(64, 256, device="cuda")
+    codes, scales, zeros = cake.Q4Weights.quantize_codes(W, 64, symmetric=False)
+    want = cake.Q4Weights(codes, scales, zeros, group=64)
+    capture, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=capture):
+        with torch.cuda.stream(other):
+            got = cake.Q4Weights(codes, scales, zeros, group=64, stream=capture)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got.packed, want.packed)
