@@ -788,6 +788,16 @@ class Q4Weights:
         self._c = _Q4(self.packed.data_ptr(), self.out_features, self.in_features, self.group, self.scale_type, int(self.has_zeros))
         self._ref = ctypes.byref(self._c)
 
+    def __getstate__(self):
+        state = dict(self.__dict__)
+        del state["_c"], state["_ref"]  # the descriptor holds an address: a copy makes its own
+        return state
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.device = self.packed.device
+        self._bind()
+
     @staticmethod
     def quantize_codes(W, group=128, symmetric=True, scale_dtype=None, stream=None):
         """(codes, scales, zeros or None) of a float32, float16 or bfloat16 matrix (cakeb200_q4_quantize)."""

@@ -72,3 +72,26 @@ def test_weights_are_made_while_their_stream_is_captured(cake):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got.packed, want.packed)
+
+
+def test_copies_and_pickles_have_memory_of_their_own(cake):
+    import torch
+    from cake_on_cpu_b200.cake import cake_linear, cake_linear_q4
+    torch.manual_seed(2)
+    x = torch.randn(7, 200, device="cuda")
+    model = torch.nn.Sequential(cake_linear_q4.from_linear(cake_linear(200, 90).cuda(), group=64, symmetric=False), torch.nn.Tanh())
+    want = model(x).detach()
+    f = io.BytesIO()
+    torch.save(model, f)
+    twin = copy.deepcopy(model)
+    weights = copy.deepcopy(model[0].weights)
+    address = model[0].packed.data_ptr()
+    assert twin[0].packed.data_ptr() != address and weights.packed.data_ptr() != address
+    model[0].packed.fill_(255)  # whoever still looked at the original would notice
+    del model
+    f.seek(0)
+    loaded = torch.load(f, weights_only=False)
+    for m in (twin, loaded, copy.deepcopy(twin).cpu().cuda()):
+        assert m[0].weights.packed is m[0].packed
+        assert torch.equal(m(x), want)
+    assert torch.equal(torch.tanh(cake.cake_q4_linear(x, weights, twin[0].bias)), want)
