@@ -121,7 +121,11 @@ class cake_linear_q4_function(torch.autograd.Function):
 
 class cake_linear_q4(nn.Module):
     """``cake_linear`` with its weight in 4 bits: for serving, and for training what lies in front of it.  The packed weight is a
-    buffer (it moves with the module and is part of its state), the bias a parameter of the type of the activations."""
+    buffer (it moves with the module and is part of its state), the bias a parameter of the type of the activations.
+
+    The state also says what the packed bytes hold (their number does not: sizes are padded, and scales of either type take two
+    bytes).  Loading the state of another geometry raises and leaves the layer as it is; so does one that does not say it, but
+    with ``strict=False``, where only the number of bytes is compared."""
 
     def __init__(self, weights, bias=None):
         super().__init__()
@@ -146,6 +150,25 @@ class cake_linear_q4(nn.Module):
         if self._weights.packed is not self.packed:  # moved, or loaded
             self._weights = api.Q4Weights.from_packed(self.packed, *self._geometry)
         return self._weights
+
+    def get_extra_state(self):
+        return torch.tensor(self._geometry, dtype=torch.int64)
+
+    def set_extra_state(self, state):
+        pass  # compared before anything is loaded
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        state = state_dict.get(prefix + "_extra_state")
+        if state is not None:
+            theirs = tuple(int(v) for v in state)
+            if theirs != tuple(int(v) for v in self._geometry):
+                error_msgs.append("%s: the state holds weights of (out_features, in_features, group, scale type, has zeros) %s, the layer's are %s"
+                                  % (prefix or "cake_linear_q4", theirs, tuple(int(v) for v in self._geometry)))
+                return
+        elif strict:
+            missing_keys.append(prefix + "_extra_state")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
     def forward(self, data):
         return cake_linear_q4_function.apply(data, self.weights, self.bias)

@@ -95,3 +95,32 @@ def test_copies_and_pickles_have_memory_of_their_own(cake):
         assert m[0].weights.packed is m[0].packed
         assert torch.equal(m(x), want)
     assert torch.equal(torch.tanh(cake.cake_q4_linear(x, weights, twin[0].bias)), want)
+
+
+def test_reloading_another_geometry_is_refused(cake):
+    """Packed sizes are padded and do not tell the scales' type: the state does."""
+    import torch
+    from cake_on_cpu_b200.cake import cake_linear_q4
+    torch.manual_seed(3)
+
+    def layer(n, k, group=128, scale=torch.float16, symmetric=True):
+        return cake_linear_q4(cake.Q4Weights.quantize(torch.randn(n, k, device="cuda"), group, symmetric, scale))
+
+    a, x = layer(100, 128), torch.randn(3, 128, device="cuda")
+    before = a(x)
+    for other in (layer(100, 128, scale=torch.bfloat16), layer(100, 100), layer(97, 128), layer(128, 128), layer(100, 128, 64), layer(100, 128, symmetric=False)):
+        for strict in (True, False):
+            with pytest.raises(RuntimeError):
+                a.load_state_dict(other.state_dict(), strict=strict)
+            assert torch.equal(a(x), before)  # nothing of it was taken
+    same = layer(100, 128)
+    a.load_state_dict(same.state_dict())
+    assert torch.equal(a(x), same(x)) and not torch.equal(a(x), before)
+    f = io.BytesIO()
+    torch.save(torch.nn.Sequential(a).state_dict(), f)
+    f.seek(0)
+    b = torch.nn.Sequential(layer(100, 128))
+    b.load_state_dict(torch.load(f))
+    assert torch.equal(b(x), a(x))
+    b.load_state_dict(torch.nn.Sequential(layer(100, 128)).state_dict(), assign=True)
+    assert b[0].weights.packed is b[0].packed and not torch.equal(b(x), a(x))

@@ -52,3 +52,32 @@ def test_copies_of_the_layer(cake):
         layer = twin[0]
         assert layer._weights.packed is layer.packed and layer.packed.data_ptr() != model[0].packed.data_ptr()
         assert _points_at_its_own(layer._weights) and torch.equal(layer.packed, model[0].packed)
+
+
+# two geometries that pad to the same number of bytes, and ones that do not
+@pytest.mark.parametrize("change", [dict(scale_type=2), dict(k=128), dict(k=99), dict(n=64), dict(n=33), dict(group=32), dict(has_zeros=True), dict(n=100)], ids=str)
+def test_state_of_another_geometry_is_refused(cake, change):
+    from cake_on_cpu_b200.cake import cake_linear_q4
+    mine = cake_linear_q4(_weights(cake))
+    keep, address = mine.packed.clone(), mine.packed.data_ptr()
+    other = cake_linear_q4(_weights(cake, seed=1, **change))
+    for strict in (True, False):
+        for assign in (True, False):
+            with pytest.raises(RuntimeError):
+                mine.load_state_dict(other.state_dict(), strict=strict, assign=assign)
+            assert torch.equal(mine.packed, keep) and mine.packed.data_ptr() == address
+
+
+def test_state_of_the_same_geometry(cake):
+    from cake_on_cpu_b200.cake import cake_linear_q4
+    model, other = (torch.nn.ModuleDict({"a": cake_linear_q4(_weights(cake, seed=s), torch.full((40,), float(s)))}) for s in (1, 2))
+    f = io.BytesIO()
+    torch.save(other.state_dict(), f)
+    f.seek(0)
+    model.load_state_dict(torch.load(f))  # tensors only
+    assert torch.equal(model["a"].packed, other["a"].packed) and torch.equal(model["a"].bias, other["a"].bias)
+    # a state that does not say what it holds is refused, unless the caller vouches for it
+    state = {k: v for k, v in other.state_dict().items() if k in ("a.packed", "a.bias")}
+    with pytest.raises(RuntimeError):
+        model.load_state_dict(state)
+    model.load_state_dict(state, strict=False)
