@@ -100,13 +100,30 @@ class cake_linear(nn.Module):
         return cake_linear_function.apply(data, self.weight, self.bias)
 
 
+def _even_rows(t):
+    """The tensor with contiguous rows that are evenly spaced over all its leading dimensions (copies only if they are not)."""
+    if t.is_contiguous() or t.dim() == 0:
+        return t
+    if t.dim() <= 2:
+        t = _rows(t)
+        return t if t.dim() < 2 or t.shape[0] < 2 or t.stride(0) >= t.shape[1] else t.contiguous()
+    if t.stride(-1) == 1:
+        try:
+            if t.view(-1, t.shape[-1]).stride(0) >= t.shape[-1]:
+                return t
+        except RuntimeError:
+            pass
+    return t.contiguous()
+
+
 class cake_linear_q4_function(torch.autograd.Function):
-    """y = x W^T + b with W a ``Q4Weights``, and its gradients for x and b; the 4-bit weight itself has none."""
+    """y = x W^T + b with W a ``Q4Weights``, and its gradients for x and b; the 4-bit weight itself has none.  As ``cake_linear``,
+    it takes any strides."""
 
     @staticmethod
     def forward(ctx, data, weights, bias=None):
         ctx.weights, ctx.has_bias = weights, bias is not None
-        return api.cake_q4_linear(data, weights, bias)
+        return api.cake_q4_linear(_even_rows(data), weights, None if bias is None else bias.contiguous())
 
     @staticmethod
     @torch.autograd.function.once_differentiable

@@ -124,3 +124,27 @@ def test_reloading_another_geometry_is_refused(cake):
     assert torch.equal(b(x), a(x))
     b.load_state_dict(torch.nn.Sequential(layer(100, 128)).state_dict(), assign=True)
     assert b[0].weights.packed is b[0].packed and not torch.equal(b(x), a(x))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_layer_takes_what_the_fp32_layer_takes(cake, dtype):
+    """Activations whose rows are not contiguous or not evenly spaced are copied, as cake_linear does, and their gradients
+    come out all the same."""
+    import torch
+    from cake_on_cpu_b200.cake import cake_linear, cake_linear_q4
+    torch.manual_seed(4)
+    plain = cake_linear(64, 40).cuda()
+    layer = cake_linear_q4.from_linear(plain, group=32).to(getattr(torch, dtype))
+    t = getattr(torch, dtype)
+    heads = torch.randn(3, 5, 4, 64, device="cuda").to(t)
+    for x in (heads.transpose(1, 2), heads[0, 0].t().contiguous().t(), heads[:, :, 1], heads[0, 0, 0].expand(6, 64), heads[:, :1].expand(3, 5, 4, 64),
+              torch.randn(64, 9, device="cuda").to(t).t(), heads[:0].transpose(1, 2)):
+        if dtype == "float32" and x.numel():
+            plain(x)
+        a, b = x.detach().requires_grad_(), x.detach().contiguous().requires_grad_()
+        y, want = layer(a), layer(b)
+        assert y.shape == x.shape[:-1] + (40,) and torch.equal(y, want)
+        c = torch.randn_like(y)
+        y.backward(c)
+        want.backward(c)
+        assert torch.equal(a.grad, b.grad)
