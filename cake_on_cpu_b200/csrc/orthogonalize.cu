@@ -11,8 +11,8 @@
 // All matrices between the first and the last kernel are pairs of FP16 planes (plane_gemm.cuh), 22 bits and a sign: three
 // MMAs per product.  Small singular values grow by a factor a = 3.4 per step, 480 in five, and so does the rounding noise
 // of X beside them: a single 16-bit plane (2^-9 or 2^-12) would leave per cents of noise in the result, pairs leave what FP32
-// products leave.  The range of FP16 is no limit: the elements of X are at most 1 (and 1.2 later), X_0 is held 2^k times
-// itself, k near log2 sqrt(m n), which puts its elements around 1 and its resolution at 2^-36 of that.  Nothing is ever
+// products leave.  The range of FP16 is no limit: X, P and Q are held with powers of two taken out (Exponents below) that follow from
+// bounds of the singular values, so that none overflows and a small X, as of a G far below eps, keeps its bits.  Nothing is ever
 // transposed or mirrored in memory: Q X reads X, and the upper triangles of P and Q are read, down the columns of what is there
 // (an SM stores 32 bytes a clock, so bytes written are what an epilogue costs).
 #include <cmath>
@@ -29,7 +29,50 @@ namespace {
 using plane::Fp16Planes;
 
 constexpr int TERMS = 2;
-constexpr int NORM_BLOCKS = 512;  // partial sums of squares per matrix
+constexpr int NORM_BLOCKS = 512;  // room for partial sums of squares per matrix; the last place is `SHIFT_AT`
+constexpr int SHIFT_AT = NORM_BLOCKS - 1;
+constexpr int MAX_STEPS = 64;
+
+// How the matrices are held: X as 2^(up - x) X, P as 2^(-2 x) P and Q as 2^-q Q, with x and q a step's exponents such that the singular values
+// of X are below 2^x and those of Q below 2^q.  X_0 has singular values up to |G| / (|G| + eps) <= 1; the host follows the
+// largest that the polynomial makes of (0, 1] (`x`, `q`).  A G below eps begins at 2^-shift, which only the device knows, and grows
+// by 2^q a step until it meets the host's bound.  2^up, around sqrt(m n), puts the elements of X, not the singular values, around 1.
+struct Exponents {
+    short x[MAX_STEPS + 1], q[MAX_STEPS];
+    short a, b, c;  // |a| < 2^a and so on; far below everything where the coefficient is zero
+    short up;
+};
+constexpr int FAR_BELOW = -8000;
+struct StepExponents {
+    int x, q, next;  // x of the step and of the one after it
+};
+__device__ __forceinline__ void begin(const Exponents& e, int shift, StepExponents& s) { s.next = min((int) e.x[0], -shift); }
+__device__ __forceinline__ void advance(const Exponents& e, int q, int next, StepExponents& s) {
+    s.x = s.next;
+    const int b = e.b + 2 * s.x, c = e.c + 4 * s.x;  // |a| + |b| 4^x + |c| 16^x
+    const int bound = max((int) e.a, max(b, c)) + (e.a >= max(b, c) + 2 ? 1 : 2);
+    s.q = min(q, bound);
+    s.next = min(next, s.x + s.q);
+}
+__device__ __forceinline__ StepExponents exponents_of(const Exponents& e, int shift, int step) {
+    StepExponents s;
+    begin(e, shift, s);
+    for (int i = 0; i <= step; i++) advance(e, e.q[i], e.x[i + 1], s);
+    return s;
+}
+// k 2^e for e between -252 and 254; beyond, zero and infinity
+__device__ __forceinline__ float times_power(float k, int e) {
+    auto power = [](int e) { return __int_as_float(e < -126 ? 0 : e > 127 ? 0x7f800000 : (e + 127) << 23); };
+    return k * power(e >> 1) * power(e - (e >> 1));
+}
+__device__ __forceinline__ double power_of_two(int e) { return __hiloint2double((e + 1023) << 20, 0); }
+// The factor that makes 2^(up + shift) X_0 of a matrix of that norm: 2^-shift is the first power of two at or above norm / (norm + eps).
+__device__ __forceinline__ double first_factor(double norm, double eps, int up, int& shift) {
+    const double inverse = 1.0 / (norm + eps), r = norm * inverse;
+    shift = r > 0 && r < 1 ? min(1022 - (__double2hiint(r) >> 20), 100) : 0;  // no finite norm, or none at all: 0
+    return inverse * power_of_two(up + shift);
+}
+
 // K blocks of 64 between folds of the main accumulator, whatever the result's type.  4096 x 4096 FP32 with folds every 64 / 128 / 256 /
 // 1024 of K: errors against 64 bits 1.2e-6, 1.6e-6, 3.1e-6, 1.1e-5 (a plain FP32 evaluation: 4.8e-6), 3.36 / 3.16 / 3.05 / 2.97 ms.  With
 // folds every 1024 a BF16 result of 1024 x 4096 differs from the correctly rounded one by 1.7e-4, with these by 9e-5.
@@ -140,10 +183,10 @@ norm_kernel(const Source<T> s, double* __restrict__ partial) {
     }
 }
 
-// Planes of `up` X_0, which is the transpose of the source where that is `tall`; a warp does one 32 x 32 block.
+// Planes of 2^(up + shift) X_0, which is the transpose of the source where that is `tall`; a warp does one 32 x 32 block.
 template <typename T>
 __global__ void __launch_bounds__(256)
-split_kernel(const Source<T> s, const double* __restrict__ partial, int partials, float eps, double up, bool tall, const Planes x, unsigned* arrived) {
+split_kernel(const Source<T> s, double* partial, int partials, float eps, int up, bool tall, const Planes x, unsigned* arrived) {
     __shared__ float patches[8][plane::PATCH_FLOATS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = blockIdx.z;
     const int row0 = blockIdx.y * 32, col0 = (blockIdx.x * 8 + warp) * 32;
@@ -154,7 +197,9 @@ split_kernel(const Source<T> s, const double* __restrict__ partial, int partials
     for (int i = lane; i < partials; i += 32) sum += partial[batch * NORM_BLOCKS + i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double inverse = up / (sqrt(sum) + (double) eps);
+    int shift;
+    const double inverse = first_factor(sqrt(sum), eps, up, shift);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) partial[batch * NORM_BLOCKS + SHIFT_AT] = shift;
     float* patch = patches[warp];
 #pragma unroll
     for (int q = 0; q < 4; q++) {
@@ -198,7 +243,6 @@ struct ResultEpilogue {
     struct Args {
         Matrix<T> out;
         int rows, cols;
-        float f;
     };
     // one value of the block's row r, in the lane's column of it
     struct Writer {
@@ -210,18 +254,18 @@ struct ResultEpilogue {
             if (r < rows) put(p + r * ld, f * x);
         }
     };
-    static __device__ __forceinline__ Writer writer(const Args& a, const TileAt& at, int lane) {
-        return {a.out.base + at.batch * a.out.stride + at.row * a.out.ld + at.col + lane, a.out.ld, at.col + lane < a.cols ? a.rows - at.row : 0, a.f};
+    static __device__ __forceinline__ Writer writer(const Args& a, const TileAt& at, int lane, float f) {
+        return {a.out.base + at.batch * a.out.stride + at.row * a.out.ld + at.col + lane, a.out.ld, at.col + lane < a.cols ? a.rows - at.row : 0, f};
     }
 };
 
-// W <- keep W - step X
+// W <- keep W - step X, the last X f times the product
 template <typename T>
 struct StepEpilogue {
     struct Args {
         Matrix<T> w;
         int rows, cols;
-        float f, keep, step;
+        float keep, step;
     };
     struct Writer {
         T* p;
@@ -232,8 +276,8 @@ struct StepEpilogue {
             if (r < rows) put(p + r * ld, keep * get(p + r * ld) - step * (f * x));
         }
     };
-    static __device__ __forceinline__ Writer writer(const Args& a, const TileAt& at, int lane) {
-        return {a.w.base + at.row * a.w.ld + at.col + lane, a.w.ld, at.col + lane < a.cols ? a.rows - at.row : 0, a.f, a.keep, a.step};
+    static __device__ __forceinline__ Writer writer(const Args& a, const TileAt& at, int lane, float f) {
+        return {a.w.base + at.row * a.w.ld + at.col + lane, a.w.ld, at.col + lane < a.cols ? a.rows - at.row : 0, f, a.keep, a.step};
     }
 };
 
@@ -253,8 +297,9 @@ struct Chain {
     Planes x[2], p, q;           // step s reads x[s % 2] and writes the other
     Product gram, poly, apply, last;
     int batch, steps;
-    float f0;                    // X_0 is held 1 / f0 times itself
     float ka, kb, kc;
+    Exponents exponents;
+    const double* shifts;        // per matrix, at SHIFT_AT of its NORM_BLOCKS
     float* parts;                // of cut tiles: [slot][32 x 32 block][1024]
     unsigned* arrived;           // CTAs that have come to the barriers so far
     int* status_word;
@@ -363,12 +408,22 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
             if (barriers) meet();
             constexpr int WIDE = C::BN / 32, PER_TILE = (C::TILE_M / 32) * WIDE;  // 32 x 32 blocks of a tile, row by row
             const Planes& out = kind == 0 ? c.p : kind == 1 ? c.q : c.x[(i / 3 + 1) & 1];
-            const float f = kind == 1 ? c.kc : i == 0 ? c.f0 * c.f0 : i == 2 ? c.f0 : 1.f;
+            int of = -1;  // the matrix whose factors these are: of the product, and of P and I in Q
+            float f = 0, kb = 0, ka = 0;
+            auto factors = [&](int batch) {
+                if (batch == of) return;
+                of = batch;
+                const StepExponents s = exponents_of(c.exponents, (int) __ldcg(c.shifts + batch * NORM_BLOCKS), i / 3);
+                f = kind == 1 ? c.kc : 1.f;
+                f = times_power(f, kind == 0 ? -2 * c.exponents.up : kind == 1 ? 4 * s.x - s.q : s.q + s.x - (kind == 2 ? s.next : c.exponents.up));
+                kb = times_power(c.kb, 2 * s.x - s.q);
+                ka = times_power(c.ka, -s.q);
+            };
             // one body for all products, so that its code is fetched once
             auto finish = [&](const TileAt& at, const float* v) {
                 if (at.row >= g.rows || at.col >= g.cols) return;
                 if (kind == 3) {
-                    plane::by_rows(v, (uint32_t*) e.patch, e.lane, Last::writer(last, at, e.lane));
+                    plane::by_rows(v, (uint32_t*) e.patch, e.lane, Last::writer(last, at, e.lane, f));
                     return;
                 }
                 plane::by_eights(v, (uint32_t*) e.patch, e.lane, [&](int r, int col, float* u) {
@@ -381,16 +436,17 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                         float old[8];
                         plane::load8<Fp16Planes>(c.p, at.batch, r, col, old);
 #pragma unroll
-                        for (int j = 0; j < 8; j++) u[j] += c.kb * old[j] + (r == col + j ? c.ka : 0.f);
+                        for (int j = 0; j < 8; j++) u[j] += kb * old[j] + (r == col + j ? ka : 0.f);
                     }
                     plane::store8<Fp16Planes, TERMS>(out, at.batch, r, col, u);
                 });
             };
             for (int k = 0; ok && item_at(g, k, unit, units, w); k++) {
-                ok = e.collect(w.kb0, w.kb1, FOLD, g.K, kind < 2 ? EVEN_GROWTH : 0.f, sum);
-                if (!ok) break;
                 TileAt at;
                 place(g, w.tile, at.batch, tm, tn);
+                factors(at.batch);  // while the tile is multiplied
+                ok = e.collect(w.kb0, w.kb1, FOLD, g.K, kind < 2 ? EVEN_GROWTH : 0.f, sum);
+                if (!ok) break;
                 const int row = (int) e.rank * plane::BM + e.quarter() * 32;
                 at.row = tm * C::TILE_M + row;
                 e.blocks(sum, [&](int column, const float* v) {
@@ -410,6 +466,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                     at.row = tm * C::TILE_M + b % PER_TILE / WIDE * 32;
                     at.col = tn * C::BN + b % WIDE * 32;
                     if (at.row >= g.rows || at.col >= g.cols) continue;
+                    factors(at.batch);
                     float v[32];
                     plane::join_parts(c.parts, b, total, g.splits, v, e.lane);
                     finish(at, v);
@@ -440,14 +497,14 @@ constexpr int SMALL_THREADS = 512, SMALL_ROWS = 128, SMALL_COLUMNS = 256, SMALL_
 constexpr int SUB_BYTES = 128 * 128;          // 128 rows of 64 values, 128-byte swizzled
 constexpr int SQUARE_BYTES = 2 * TERMS * SUB_BYTES;  // planes of 128 x 128 values: [plane][64 columns]
 constexpr int HALF_PATCH = 16 * 128;          // 16 rows of 32 FP32
-constexpr int SMALL_SMEM = 1024 + 2 * SQUARE_BYTES + SQUARE_BYTES + 16 * HALF_PATCH + 512;
+constexpr int SMALL_SMEM = 1024 + 2 * SQUARE_BYTES + SQUARE_BYTES + 16 * HALF_PATCH + MAX_STEPS * 16 + 512;
 static_assert(SMALL_SMEM <= plane::MAX_SMEM, "X, P and the patches fit");
 static_assert(SQUARE_BYTES + 16 * HALF_PATCH >= 16 * plane::PATCH_FLOATS * 4, "the patches of the result lie where P and the others were");
 
 struct Small {
     int m, n, tall, batch, steps, cluster, slice;  // slice: columns of X per CTA
-    float eps, f0, ka, kb, kc;
-    double up;
+    float eps, ka, kb, kc;
+    Exponents exponents;
     int* status_word;
 };
 
@@ -484,9 +541,9 @@ __device__ __forceinline__ void get_row(const uint8_t* square, int r, int c0, fl
     }
 }
 
-// D(main) + D(main2) = A B, D(cross) (+)= its two smaller products: squares a and b, b along its rows or down its columns; n columns of
-// the result, `depth` of K, both multiples of 32.  main2 takes the second half of K, or is main.
-__device__ __forceinline__ void square_product(uint32_t main, uint32_t main2, uint32_t cross, uint32_t a, uint32_t b, bool down, bool more, int n, int depth) {
+// D(main) = A B, D(cross) (+)= its two smaller products: squares a and b, b along its rows or down its columns; n columns of
+// the result, `depth` of K, both multiples of 32
+__device__ __forceinline__ void square_product(uint32_t main, uint32_t cross, uint32_t a, uint32_t b, bool down, bool more, int n, int depth) {
     const uint32_t idesc = plane::idesc_16(Fp16Planes::FORMAT, 128, n) | (down ? 1u << 16 : 0u);
     // down: 64 columns further is a sub-tile (leading offset), 16 rows of K are 2048 bytes; along: 16 of K are 32 bytes, 64 a sub-tile
     const uint64_t da = ptx::make_kmajor_sw128_desc(a), db = ptx::make_kmajor_sw128_desc(b) + (down ? (uint64_t) ((SUB_BYTES >> 4) - 1) << 16 : 0);
@@ -496,8 +553,7 @@ __device__ __forceinline__ void square_product(uint32_t main, uint32_t main2, ui
         const uint32_t plane = 2 * SUB_BYTES >> 4, first = more || k > 0;
         plane::umma<false>(cross, da + plane + ka, db + kb, idesc, first);
         plane::umma<false>(cross, da + ka, db + plane + kb, idesc, 1u);
-        const bool second = main2 != main && k >= depth / 32;
-        plane::umma<false>(second ? main2 : main, da + ka, db + kb, idesc, k > (second ? depth / 32 : 0));
+        plane::umma<false>(main, da + ka, db + kb, idesc, k > 0);
     }
 }
 
@@ -514,7 +570,8 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
     uint8_t* x = (uint8_t*) (((uintptr_t) smem_raw + 1023) & ~(uintptr_t) 1023);  // one or two squares
     uint8_t* square = x + 2 * SQUARE_BYTES;                                     // P, Q, and the parts of P
     uint8_t* patches = square + SQUARE_BYTES;
-    double* sums = (double*) (patches + 16 * HALF_PATCH);                       // per warp, then per CTA
+    float4* factors = (float4*) (patches + 16 * HALF_PATCH);                    // of every step: of P P, P and I in Q, and of Q X
+    double* sums = (double*) (factors + MAX_STEPS);                             // per warp, then per CTA
     uint64_t* bar = (uint64_t*) (sums + 32);
     uint32_t* tmem_slot = (uint32_t*) (bar + 1);
     volatile int* abort_flag = (volatile int*) (tmem_slot + 1);
@@ -533,6 +590,10 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) ptx::tmem_alloc<false>(ptx::smem_u32(tmem_slot), 512);
+    if (threadIdx.x >= SMALL_THREADS - MAX_STEPS) {  // fetched while G is: the bounds that the steps' factors are made of
+        const int step = threadIdx.x - (SMALL_THREADS - MAX_STEPS);
+        factors[step] = make_float4(0.f, (float) p.exponents.q[step], (float) p.exponents.x[step + 1], 0.f);
+    }
     // the source: X's columns [c0, c0 + columns) are eights along rows of G, or rows of G where X is its transpose
     const int lines = p.tall ? columns : p.m, eights = ((p.tall ? p.m : columns) + 7) / 8, row0 = p.tall ? c0 : 0, col0 = p.tall ? 0 : c0;
     double sum = 0;
@@ -560,8 +621,19 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
     meet();
     sum = 0;
     for (int k = 0; k < p.cluster; k++) sum += sums[16 + k];
-    const double inverse = p.up / (sqrt(sum) + (double) p.eps);
+    int shift;
+    const double inverse = first_factor(sqrt(sum), p.eps, p.exponents.up, shift);
     const uint32_t tmem = *tmem_slot;
+    if (threadIdx.x == SMALL_THREADS - 1) {  // there before the first product ends
+        StepExponents e;
+        begin(p.exponents, shift, e);
+        for (int step = 0; step < p.steps; step++) {
+            const float4 bounds = factors[step];
+            advance(p.exponents, (int) bounds.y, (int) bounds.z, e);
+            factors[step] = make_float4(times_power(p.kc, 4 * e.x - e.q), times_power(p.kb, 2 * e.x - e.q), times_power(p.ka, -e.q),
+                                        times_power(1.f, e.q + e.x - (step + 1 < p.steps ? e.next : p.exponents.up)));
+        }
+    }
 
     for (int i = threadIdx.x; i < lines * eights; i += SMALL_THREADS) {
         const int r = i / eights, c = (i - r * eights) * 8;
@@ -602,8 +674,8 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
     // room for the parts: the second square of X if there is none, else the place of P and Q, which then needs two more meetings
     const bool apart = squares == 1;
     uint8_t* parts = apart ? x + SQUARE_BYTES : square;
-    // what makes up for truncation in a square's main sums over `depth` values, `padded` with zeros
-    auto grown = [&](int depth, int padded) { return 1.f + EVEN_GROWTH * (float) (min((depth + 15) / 16, padded / (apart ? 32 : 16)) + 1); };
+    // what makes up for truncation in a square's main sums over `depth` values
+    auto grown = [&](int depth) { return 1.f + EVEN_GROWTH * (float) ((min(depth, 128) + 15) / 16 + 1); };
     uint32_t phase = 0;
     // shared memory that this thread wrote is there for the MMAs of all; then one thread issues them and all wait
     auto multiply = [&](auto issue) {
@@ -625,38 +697,28 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         ptx::tmem_ld_wait();
     };
 
-    // with one square of X there is tensor memory to add up the two halves of K apart: half as many truncated additions each
-    const uint32_t second = apart ? 256 : 0;
-    auto read_main = [&](uint32_t column, float* v, float* u) {
-        read(column, v);
-        if (!apart) return;
-        read(column + 256, u);
-#pragma unroll
-        for (int j = 0; j < 32; j++) v[j] += u[j];
-    };
-
+    const float f = times_power(1.f, -2 * p.exponents.up);
     for (int step = 0; step < p.steps; step++) {
-        const float f = step == 0 ? p.f0 : 1.f;
         float v[32], u[32];
         // ---- P: main sums of the squares in columns 0 and 256, both squares' smaller products in 128
         multiply([&]() {
             for (int q = 0; q < squares; q++) {
                 const uint32_t at = ptx::smem_u32(x + q * SQUARE_BYTES);
-                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * (apart ? 1 : q), tmem + 128, at, at, false, q > 0, m32, width(q));
+                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 128, at, at, false, q > 0, m32, width(q));
             }
         });
         if (in_square) {
             read(0, v);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] *= grown(columns, width(0));
-            if (apart || width(1) > 0) {
+            for (int j = 0; j < 32; j++) v[j] *= grown(columns);
+            if (squares == 2 && width(1) > 0) {
                 read(256, u);
 #pragma unroll
-                for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], apart ? grown(columns, width(0)) : grown(columns - 128, width(1)), v[j]);
+                for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], grown(columns - 128), v[j]);
             }
             read(128, u);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = f * f * fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);
+            for (int j = 0; j < 32; j++) v[j] = f * fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);
             if (p.cluster == 1) put_row(square, row, wide, v);
         }
         if (p.cluster > 1) {
@@ -715,31 +777,33 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         }
         // ---- Q, in place of P
         const uint32_t sq = ptx::smem_u32(square);
-        multiply([&]() { square_product(tmem, tmem + second, tmem + 128, sq, sq, false, false, m32, m32); });
+        multiply([&]() { square_product(tmem, tmem + 128, sq, sq, false, false, m32, m32); });
         if (in_square) {
-            read_main(0, v, u);
+            read(0, v);
             read(128, u);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j] * grown(p.m, m32));
+            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j] * grown(p.m));
             get_row(square, row, wide, u);
+            const float4 k = factors[step];
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = p.kc * v[j] + p.kb * u[j] + (row == wide + j && row < p.m ? p.ka : 0.f);
+            for (int j = 0; j < 32; j++) v[j] = k.x * v[j] + k.y * u[j] + (row == wide + j && row < p.m ? k.z : 0.f);
             put_row(square, row, wide, v);
         }
         // ---- X
         multiply([&]() {
             for (int q = 0; q < squares; q++)
-                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * q + second, tmem + 256 * q + 128, sq, ptx::smem_u32(x + q * SQUARE_BYTES), true, false, width(q), m32);
+                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * q + 128, sq, ptx::smem_u32(x + q * SQUARE_BYTES), true, false, width(q), m32);
         });
+        const float apply = factors[step].w;
         for (int q = 0; q < squares; q++) {
             if (quarter * 32 >= m32 || wide >= width(q)) continue;
-            read_main(256 * q, v, u);
+            read(256 * q, v);
             read(256 * q + 128, u);
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);
             if (step + 1 < p.steps) {
 #pragma unroll
-                for (int j = 0; j < 32; j++) v[j] *= f;
+                for (int j = 0; j < 32; j++) v[j] *= apply;
                 put_row(x + q * SQUARE_BYTES, row, wide, v);
             } else {
                 const int column = c0 + q * 128 + wide;
@@ -749,12 +813,12 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
                 at.col = p.tall ? quarter * 32 : column;
                 const int end = c0 + columns;  // the columns after them are another CTA's
                 if (p.tall) {
-                    const auto write = Last::writer(last, at, lane);
+                    const auto write = Last::writer(last, at, lane, apply);
 #pragma unroll
                     for (int j = 0; j < 32; j++)
                         if (column + j < end) write(j, v[j]);
                 } else {
-                    auto write = Last::writer(last, at, lane);
+                    auto write = Last::writer(last, at, lane, apply);
                     if (column + lane >= end) write.rows = 0;
                     plane::by_rows(v, (uint32_t*) square + warp * plane::PATCH_FLOATS, lane, write);
                     __syncwarp();
@@ -777,7 +841,7 @@ int bad(const char* who, const char* what) {
     return CAKEB200_ERR_ARG;
 }
 
-constexpr int MAX_SIDE = 1 << 20, MAX_BATCH = 65535, MAX_STEPS = 64;
+constexpr int MAX_SIDE = 1 << 20, MAX_BATCH = 65535;
 
 struct Layout {
     Planes x[2], p, q;
@@ -860,9 +924,53 @@ struct Coefficients {
     float a, b, c, eps;
 };
 
+// the exponent e of the first power of two at or above v >= 0
+short exponent_above(double v) {
+    if (!(v > 0)) return FAR_BELOW;
+    if (!std::isfinite(v)) return -FAR_BELOW;
+    return (short) std::ceil(std::log2(v) - 1e-6);  // a bound that its own rounding put above a power of two is that power
+}
+// An X whose singular values are all about 1 / sqrt(m) has elements around 1 as it is held, and 2^-12 of that is the least that FP16 pairs
+// hold with all their bits.  So coefficients may let a singular value of 1 grow 2^12 times as far as small ones, which grow by |a| a step;
+// where it would run away further the bounds are those of singular values up to 2, and larger ones come out infinite.
+Exponents exponents_for(const Coefficients& k, int up, bool runaway = false) {
+    Exponents e = {};
+    double small = 1;
+    e.up = (short) up;
+    const double a = k.a, b = k.b, c = k.c;
+    e.a = exponent_above(std::fabs(a)); e.b = exponent_above(std::fabs(b)); e.c = exponent_above(std::fabs(c));
+    double u = 1;  // the largest singular value so far
+    for (int s = 0; s < k.steps; s++) {
+        const double y = u * u;
+        auto quotient = [&](double t2) { return std::fabs(a + b * t2 + c * t2 * t2); };
+        // their extremes over [0, u]: the ends, and where the derivative is zero (of b t^2 + c t^4; of a t + b t^3 + c t^5)
+        double q = std::max(quotient(0), quotient(y)), x = u * quotient(y);
+        if (c != 0) {
+            const double t2 = -b / (2 * c), d = 9 * b * b - 20 * a * c;
+            if (t2 > 0 && t2 < y) q = std::max(q, quotient(t2));
+            if (d >= 0)
+                for (double root : {std::sqrt(d), -std::sqrt(d)}) {
+                    const double r2 = (root - 3 * b) / (10 * c);
+                    if (r2 > 0 && r2 < y) x = std::max(x, std::sqrt(r2) * quotient(r2));
+                }
+        } else if (b != 0) {
+            const double r2 = -a / (3 * b);
+            if (r2 > 0 && r2 < y) x = std::max(x, std::sqrt(r2) * quotient(r2));
+        }
+        e.x[s] = exponent_above(u);
+        e.q[s] = exponent_above(q);
+        if (!runaway && u > 4096 * small) return exponents_for(k, up, true);
+        u = runaway ? std::min(x, 2.0) : x;
+        small *= std::fabs(a);
+    }
+    e.x[k.steps] = exponent_above(u);
+    return e;
+}
+
 int check_coefficients(const char* who, const Coefficients& k) {
     if (k.steps < 1 || k.steps > MAX_STEPS) return bad(who, "1 to 64 steps");
     if (!(k.eps >= 0.f)) return bad(who, "eps is a number that is not negative");
+    if (!std::isfinite(k.a) || !std::isfinite(k.b) || !std::isfinite(k.c)) return bad(who, "the coefficients are finite numbers");
     return CAKEB200_OK;
 }
 
@@ -996,16 +1104,15 @@ int run(const Source<T>& src, int batch, bool early, const Coefficients& k, void
     const int rows = src.rows, cols = src.cols;
     const bool tall = rows > cols;
     const int m = tall ? cols : rows, n = tall ? rows : cols;
-    // X_0 is held 2^up times itself: around sqrt(m n), below the 2^16 at which its largest possible element would overflow
+    // around sqrt(m n), below the 2^16 at which the largest possible element of X would overflow
     const int up = std::min(15, (int) (0.5 * std::log2((double) m * n)));
-    const float down = std::ldexp(1.f, -up);
-    last.f = k.steps == 1 ? down : 1.f;
+    const Exponents exponents = exponents_for(k, up);
     int rc, units_single = 0, units_pair = 0;
     Small small = {};
     if (early && option_get(OPT_PAIR) == 0 && option_get(OPT_K_PIECES) == 0 && fits_small(m, n, batch, st->sm_count, &small)) {  // those options are about the chain
         small.m = m; small.n = n; small.tall = tall; small.batch = batch; small.steps = k.steps;
-        small.eps = k.eps; small.f0 = down; small.ka = k.a; small.kb = k.b; small.kc = k.c;
-        small.up = std::ldexp(1.0, up);
+        small.eps = k.eps; small.ka = k.a; small.kb = k.b; small.kc = k.c;
+        small.exponents = exponents;
         small.status_word = st->status_word;
         if ((rc = launch_small<T, Last>(src, small, last, st->device, s))) return rc;
         thread_stats()->launches = 1;
@@ -1026,8 +1133,9 @@ int run(const Source<T>& src, int batch, bool early, const Coefficients& k, void
     Chain c = {};
     c.x[0] = l.x[0]; c.x[1] = l.x[1]; c.p = l.p; c.q = l.q;
     c.batch = batch; c.steps = k.steps;
-    c.f0 = down;
     c.ka = k.a; c.kb = k.b; c.kc = k.c;
+    c.exponents = exponents;
+    c.shifts = l.partial + SHIFT_AT;
     c.parts = l.parts;
     c.arrived = l.arrived;
     c.status_word = st->status_word;
@@ -1043,11 +1151,11 @@ int run(const Source<T>& src, int batch, bool early, const Coefficients& k, void
     units = std::min(units, pair ? units_pair : units_single);
 
     const long long work = (long long) rows * ((cols + 7) / 8);
-    const int partials = (int) std::max<long long>(1, std::min<long long>(NORM_BLOCKS, work / 512));
+    const int partials = (int) std::max<long long>(1, std::min<long long>(SHIFT_AT, work / 512));
     norm_kernel<T><<<dim3((unsigned) partials, (unsigned) batch), 256, 0, s>>>(src, l.partial);
     CAKE_CUDA_OK(cudaGetLastError());
     const dim3 grid((unsigned) ((cols + 255) / 256), (unsigned) ((rows + 31) / 32), (unsigned) batch);
-    if ((rc = launch_after(split_kernel<T>, grid, s, src, l.partial, partials, k.eps, std::ldexp(1.0, up), tall, l.x[0], l.arrived)))
+    if ((rc = launch_after(split_kernel<T>, grid, s, src, l.partial, partials, k.eps, up, tall, l.x[0], l.arrived)))
         return rc;
     rc = pair ? launch_chain<true, Last>(maps, c, last, units, s) : launch_chain<false, Last>(maps, c, last, units, s);
     if (!rc) thread_stats()->launches = 3;
@@ -1063,7 +1171,7 @@ int orthogonalize(const void* G, long long ldg, long long stride_g, void* out, l
     src.g = matrix((const T*) G, ldg, stride_g, rows, batch);
     src.rows = rows;
     src.cols = cols;
-    typename ResultEpilogue<T>::Args last = {matrix((T*) out, ldo, stride_o, rows, batch), rows, cols, 1.f};
+    typename ResultEpilogue<T>::Args last = {matrix((T*) out, ldo, stride_o, rows, batch), rows, cols};
     // in place is fine matrix by matrix; a result that lies across its operands has to wait for all of them
     const long long size = sizeof(T), reach_g = (rows - 1) * ldg + cols + (batch - 1) * stride_g, reach_o = (rows - 1) * ldo + cols + (batch - 1) * stride_o;
     const bool same = G == out && ldg == ldo && (batch == 1 || stride_g == stride_o);
@@ -1084,7 +1192,7 @@ int muon(void* W, long long ldw, const void* G, long long ldg, float* M, long lo
     src.nesterov = nesterov;
     src.rows = rows;
     src.cols = cols;
-    typename StepEpilogue<TW>::Args last = {matrix((TW*) W, ldw, 0, rows, 1), rows, cols, 1.f, (float) (1.0 - lr * weight_decay), (float) (lr * scale)};
+    typename StepEpilogue<TW>::Args last = {matrix((TW*) W, ldw, 0, rows, 1), rows, cols, (float) (1.0 - lr * weight_decay), (float) (lr * scale)};
     return run<TG, StepEpilogue<TW>>(src, 1, true, k, workspace, last, st, s);
 }
 

@@ -465,8 +465,11 @@ int cakeb200_q4_linear_dx(const cakeb200_q4* w, const void* dy, long long lddy, 
  *
  * _orthogonalize works on `batch` matrices `stride` elements apart, each rows x cols with leading dimension ld (elements).
  * G and out have one type, CAKEB200_F32 or CAKEB200_BF16; out may be G itself or lie across it.  All products have operands of
- * 22 bits and a sign, held in pairs of FP16, and sums in FP32; the result is rounded once.  A G that is zero gives zero; one
- * that is not finite gives NaN.
+ * 22 bits and a sign, held in pairs of FP16, and sums in FP32; the result is rounded once.  Powers of two are taken out of the
+ * operands, as |G| / (|G| + eps) and the coefficients ask for: a G far below eps loses nothing, and the elements resolve 2^-36 of the
+ * largest singular value that the coefficients can make of 1 in as many steps.  Coefficients are any finite numbers; under ones that
+ * make values near 1 grow more than 2^12 times as far as small ones, X may come out infinite or NaN once a singular value passes 2.
+ * A G that is zero gives zero; one that is not finite gives NaN.
  *
  * _muon_step is one optimiser step on one matrix, in place:
  *     M <- momentum M + (1 - momentum) G
