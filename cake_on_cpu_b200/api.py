@@ -143,6 +143,7 @@ _SIGNATURES["cakeb200_q4_workspace"] = (_sz, [_pq4, _i, _i, _i])
 _SIGNATURES["cakeb200_q4_linear"] = (_i, [_pq4, _vp, _ll, _vp, _vp, _ll, _i, _i, _vp, _sz, _vp])
 _SIGNATURES["cakeb200_q4_linear_dx"] = (_i, [_pq4, _vp, _ll, _vp, _ll, _i, _i, _vp, _sz, _vp])
 _f, _d = ctypes.c_float, ctypes.c_double
+_SIGNATURES["cakeb200_selftest_orthogonalize_wait"] = (_i, [_vp, _vp, _vp, _i, _i, _vp, _sz, _vp])
 _SIGNATURES["cakeb200_orthogonalize_workspace"] = (_sz, [_i, _i, _i, _i])
 _SIGNATURES["cakeb200_orthogonalize"] = (_i, [_vp, _ll, _ll, _vp, _ll, _ll] + [_i] * 5 + [_f] * 4 + [_vp, _sz, _vp])
 _SIGNATURES["cakeb200_muon_step"] = (_i, [_vp, _ll, _i, _vp, _ll, _i, _vp, _ll, _i, _i, _d, _d, _i, _d, _d, _i, _f, _f, _f, _f, _vp, _sz, _vp])

@@ -180,6 +180,10 @@ int check_status_word(DeviceState* st, cudaStream_t s) {
     return CAKEB200_OK;
 }
 
+}  // namespace
+int wait_and_check(DeviceState* st, cudaStream_t s) { return check_status_word(st, s); }
+namespace {
+
 // Queried once per device: the property calls cost milliseconds, far too much per product.
 void b200_cntx(DeviceState* st, cakeb200_cntx* c) {
     static std::mutex m;

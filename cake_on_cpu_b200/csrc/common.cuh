@@ -95,6 +95,8 @@ struct DeviceState {
 };
 DeviceState* device_state();  // state of the current device (created on first use)
 int ensure_scratch(DeviceState* st, size_t bytes);
+// Waits for the stream and reports (and clears) a device-side wait that gave up (abi.cu).
+int wait_and_check(DeviceState* st, cudaStream_t s);
 
 // exact-FP32 FFMA path (sgemm_ffma.cu)
 int launch_sgemm_ffma(const GemmProblem& g, cudaStream_t stream);  // untransposed operands only

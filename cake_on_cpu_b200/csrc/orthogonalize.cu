@@ -192,7 +192,7 @@ split_kernel(const Source<T> s, double* partial, int partials, float eps, int up
     const int row0 = blockIdx.y * 32, col0 = (blockIdx.x * 8 + warp) * 32;
     if (col0 >= s.cols) return;
     plane::wait_for_previous_kernel();
-    if (blockIdx.x == 0 && blockIdx.y == 0 && batch == 0 && threadIdx.x == 0) *arrived = 0;  // for the barriers of the chain
+    if (blockIdx.x == 0 && blockIdx.y == 0 && batch == 0 && threadIdx.x == 0) arrived[0] = arrived[1] = 0;  // for the barriers of the chain
     double sum = 0;
     for (int i = lane; i < partials; i += 32) sum += partial[batch * NORM_BLOCKS + i];
 #pragma unroll
@@ -301,7 +301,8 @@ struct Chain {
     Exponents exponents;
     const double* shifts;        // per matrix, at SHIFT_AT of its NORM_BLOCKS
     float* parts;                // of cut tiles: [slot][32 x 32 block][1024]
-    unsigned* arrived;           // CTAs that have come to the barriers so far
+    unsigned* arrived;           // CTAs that have come to the barriers so far; next to it, whether one came with work undone
+    int mute;                    // self-test: the first CTA never multiplies
     int* status_word;
 };
 
@@ -373,9 +374,9 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                 }
                 barriers += g.cut ? 2 : 1;
             }
-            if (!ok) e.drain_loads();
+            if (!ok || !e.loads_done()) e.drain_loads();
         } else if (e.warp == 1 && e.lane == 0 && e.rank == 0) {
-            bool ok = true;
+            bool ok = !(c.mute && blockIdx.x == 0);
             for (int i = 0; ok && i < products; i++) {
                 const Product& g = product(i);
                 for (int k = 0; ok && item_at(g, k, unit, units, w); k++) {
@@ -387,18 +388,25 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     } else {
         plane::many_registers();
         const bool leader = threadIdx.x == 128;
-        // Once a wait has given up a warp does no more work, but comes to every barrier, so that nobody waits for it.
+        // Once a wait has given up a warp does no more work, but comes to every barrier, so that nobody waits for it; its CTA says so
+        // there, and nobody works on, or stores a result, from what it left undone.
         bool ok = true;
         // all drain warps: wait until all CTAs have come to `barriers` barriers
         auto meet = [&]() {
-            if (leader) wait_for_count(c.arrived, barriers * gridDim.x, e.abort_flag, c.status_word);
+            if (leader) {
+                wait_for_count(c.arrived, barriers * gridDim.x, e.abort_flag, c.status_word);
+                if (*(volatile unsigned*) (c.arrived + 1)) *e.abort_flag = 1;
+            }
             ptx::named_barrier_sync(1, 256);
             ok = __all_sync(0xffffffffu, ok && *e.abort_flag == 0);
         };
         auto arrive = [&]() {
             publish();
             ptx::named_barrier_sync(1, 256);
-            if (leader) count_in(c.arrived);
+            if (leader) {
+                if (*e.abort_flag) *(volatile unsigned*) (c.arrived + 1) = 1;
+                count_in(c.arrived);
+            }
             barriers++;
         };
         float sum[C::COLS];
@@ -505,6 +513,7 @@ struct Small {
     int m, n, tall, batch, steps, cluster, slice;  // slice: columns of X per CTA
     float eps, ka, kb, kc;
     Exponents exponents;
+    int mute;         // self-test: the first CTA never multiplies
     int* status_word;
 };
 
@@ -682,12 +691,14 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         ptx::fence_proxy_async_smem();
         ptx::tcgen05_fence_before();
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && !(p.mute && blockIdx.x == 0)) {
             ptx::tcgen05_fence_after();
             issue();
             ptx::umma_commit(done);
         }
-        ptx::mbar_wait(done, phase, abort_flag, p.status_word, 560);
+        if (!ptx::mbar_wait(done, phase, abort_flag, p.status_word, 560))  // all CTAs of the cluster work on, but none stores a result
+            for (int k = 0; k < p.cluster; k++)
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote(ptx::smem_u32((const void*) abort_flag), k)), "r"(1) : "memory");
         __syncwarp();
         phase ^= 1;
         ptx::tcgen05_fence_after();
@@ -795,6 +806,10 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
                 if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * q + 128, sq, ptx::smem_u32(x + q * SQUARE_BYTES), true, false, width(q), m32);
         });
         const float apply = factors[step].w;
+        if (step + 1 == p.steps) {
+            meet();
+            if (*abort_flag) break;
+        }
         for (int q = 0; q < squares; q++) {
             if (quarter * 32 >= m32 || wide >= width(q)) continue;
             read(256 * q, v);
@@ -829,6 +844,10 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
     ptx::tcgen05_fence_before();
     meet();
     if (warp == 0) {
+        if (*abort_flag) {  // products that nobody waited for come to their end
+            const unsigned long long t0 = ptx::global_ns();
+            while ((long long) (ptx::global_ns() - t0) < 20000000LL) __nanosleep(1000);
+        }
         ptx::tcgen05_fence_after();
         ptx::tmem_free<false>(tmem, 512);
     }
@@ -842,6 +861,7 @@ int bad(const char* who, const char* what) {
 }
 
 constexpr int MAX_SIDE = 1 << 20, MAX_BATCH = 65535;
+thread_local int g_mute = 0;  // in a self-test's call
 
 struct Layout {
     Planes x[2], p, q;
@@ -1113,6 +1133,7 @@ int run(const Source<T>& src, int batch, bool early, const Coefficients& k, void
         small.m = m; small.n = n; small.tall = tall; small.batch = batch; small.steps = k.steps;
         small.eps = k.eps; small.ka = k.a; small.kb = k.b; small.kc = k.c;
         small.exponents = exponents;
+        small.mute = g_mute;
         small.status_word = st->status_word;
         if ((rc = launch_small<T, Last>(src, small, last, st->device, s))) return rc;
         thread_stats()->launches = 1;
@@ -1138,6 +1159,7 @@ int run(const Source<T>& src, int batch, bool early, const Coefficients& k, void
     c.shifts = l.partial + SHIFT_AT;
     c.parts = l.parts;
     c.arrived = l.arrived;
+    c.mute = g_mute;
     c.status_word = st->status_word;
     const int forced = option_get(OPT_PAIR);  // 1: pairs, 2: single SMs, 0: the faster by the model
     Chain other = c;
@@ -1273,6 +1295,17 @@ int cakeb200_muon_step(void* W, long long ldw, int type_w, const void* G, long l
     if (type_g == CAKEB200_F32) CAKE_MUON(__nv_bfloat16, float);
     CAKE_MUON(__nv_bfloat16, __nv_bfloat16);
 #undef CAKE_MUON
+}
+
+int cakeb200_selftest_orthogonalize_wait(float* W, const float* G, float* M, int rows, int cols, void* workspace, size_t workspace_bytes,
+                                         void* stream) {
+    g_mute = 1;
+    const int rc = cakeb200_muon_step(W, cols, CAKEB200_F32, G, cols, CAKEB200_F32, M, cols, rows, cols, 1.0, 0.0, 0, 0.0, 1.0, 5, 3.4445f, -4.7750f,
+                                      2.0315f, 1e-7f, workspace, workspace_bytes, stream);
+    g_mute = 0;
+    if (rc) return rc;
+    DeviceState* st = device_state();
+    return st ? wait_and_check(st, (cudaStream_t) stream) : CAKEB200_ERR_NO_DEVICE;
 }
 
 }  // extern "C"

@@ -321,6 +321,14 @@ struct Engine {
         }
         return true;
     }
+    // TMA thread that has issued everything: waits until it has been multiplied, so that no load is on its way into a CTA that has gone.
+    __device__ __forceinline__ bool loads_done() {
+        for (int s = 0; s < STAGES; s++) {
+            if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, status_word, 505)) return false;
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        return true;
+    }
     // TMA thread that gave up: lets the loads already issued land before the CTA goes away (bounded).
     __device__ __forceinline__ void drain_loads() {
         const unsigned long long t0 = global_ns();
@@ -462,7 +470,7 @@ plane_gemm_kernel(const __grid_constant__ OperandMaps map_a, const __grid_consta
                 const Operand a = {map_a.m, tm * C::TILE_M + (int) e.rank * 128, p.a_turn}, b = {map_b.m, tn * C::BN + (int) e.rank * 128, p.b_turn};
                 ok = e.load(a, b, batch, p.batch, w.kb0, w.kb1);
             }
-            if (!ok) e.drain_loads();
+            if (!ok || !e.loads_done()) e.drain_loads();
         } else if (e.warp == 1 && e.lane == 0 && e.rank == 0) {
             for (int k = 0; item_at(p.t, k, unit, units, w); k++)
                 if (!e.multiply(p.a_turn, p.b_turn, w.kb0, w.kb1, p.chunk)) break;

@@ -280,6 +280,11 @@ int cakeb200_selftest_bounded_wait(int limit_us, void* stream);
  * an arrival its peer never sends, gives up after `limit_us` ("where 901"), and both CTAs still
  * leave through the cluster barrier that ends those kernels. */
 int cakeb200_selftest_bounded_wait_pair(int limit_us, void* stream);
+/* The same inside cakeb200_muon_step (FP32, rows dense, lr 1, no momentum, no decay): one CTA never multiplies, its waits give up after
+ * two seconds, and no CTA stores a result: the call waits, W is as it was and CAKEB200_ERR_DEVICE_TIMEOUT is returned.  M and
+ * workspace as for cakeb200_muon_step. */
+int cakeb200_selftest_orthogonalize_wait(float* W, const float* G, float* M, int rows, int cols, void* workspace,
+                                         size_t workspace_bytes, void* stream);
 
 /* ---- One product with K sharded over the GPUs of one box, one process per GPU.
  *
@@ -435,8 +440,10 @@ int cakeb200_unpack_B(float* B, const float* B_p, int K, int N, int p, const cak
  * tells how many bytes of device memory, on a 1024-byte boundary, the call needs for that (0 for few rows: workspace may then
  * be NULL); two calls that may overlap on the GPU need one each.  A row with an infinity or a NaN gives results
  * that are not finite, and does not touch other rows.  The result must not overlap the operands.  `rows` may be 0.  Device
- * pointers of the current device only; work is enqueued on `stream`.  Results do not depend on timing.  Waits inside the
- * kernels are bounded; one that gave up shows in the status of the next blocking product (cakeb200_sgemm). */
+ * pointers of the current device only; work is enqueued on `stream`.  Results do not depend on timing.  Waits for copies and
+ * products inside the kernels are bounded; one that gave up leaves the result undefined and shows in the status of the next blocking
+ * product (cakeb200_sgemm).  The CTAs of a cluster meet at the hardware's barrier, which has no limit and needs none: they are resident
+ * together, and every path comes to it. */
 typedef struct cakeb200_q4 {
     const void* packed;
     int out_features, in_features, group;
@@ -480,8 +487,9 @@ int cakeb200_q4_linear_dx(const cakeb200_q4* w, const void* dy, long long lddy, 
  * `workspace` is device memory of the caller's, 1024-byte aligned and at least _workspace(rows, cols, batch, type of the
  * result) bytes (1 for the step's batch); its content does not matter before and after the call, but calls that may overlap on the
  * GPU, captured graphs among them, need one each.  Device pointers of the current device only; work is enqueued on `stream`.  1 to
- * 64 steps, up to 2^20 rows and columns and 65535 matrices.  Waits inside the kernels are bounded; one that gave up shows in
- * the status of the next blocking product (cakeb200_sgemm). */
+ * 64 steps, up to 2^20 rows and columns and 65535 matrices.  Waits inside the kernels are bounded, the clusters' barriers apart (as
+ * above); one that gave up shows in the status of the next blocking product (cakeb200_sgemm), and out or W are not written if it did so
+ * before the last product (M has been by then). */
 size_t cakeb200_orthogonalize_workspace(int rows, int cols, int batch, int type);
 int cakeb200_orthogonalize(const void* G, long long ldg, long long stride_g, void* out, long long ldo, long long stride_o, int rows,
                            int cols, int batch, int type, int steps, float a, float b, float c, float eps, void* workspace,
