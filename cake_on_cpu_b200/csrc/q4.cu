@@ -99,14 +99,16 @@ __device__ __forceinline__ void join(const float* red, int rank, int cluster, F 
     }
 }
 
-// Whether the kernels below take a product, or the weights are expanded and multiplied on tcgen05 (q4_gemm.cu).  Beyond 64
-// rows these read the codes again for every 32 (gradient: 16) rows, the others pay for three launches, a workspace and the expanded
-// weights whatever the number of rows.  us of a call here / there: 4096 x 4096 BF16, 128 rows 51 / 45; 2048 x 2048 BF16, 128 rows 31 /
-// 43 and 512 rows 54 / 47; 1024 x 1024 FP32, 128 rows 24 / 41 and 1000 rows 65 / 50; gradients 2048 x 2048 BF16, 65 rows 35 / 35,
-// 1024 x 1024, 192 rows 30 / 33.
-bool few_rows(const Q4View& w, int rows, bool dx) {
+// Whether the kernels below take a product, or the weights are expanded and multiplied on tcgen05 (q4_gemm.cu).  These read the codes
+// again for every 32 (gradient: 16) rows, the others pay for three launches, a workspace and the expanded weights whatever the
+// number of rows.  us here / there: y of 16-bit types, 128 rows, 4096 x 4096 41 / 41, 8192 x 4096 66 / 68, 16384 x 8192 184 / 248 (192
+// rows 270 / 264), 2048 x 2048 20 / 25 (256 rows 29 / 27); 512 rows, 1024 x 1024 23 / 23.  FP32 takes three MMAs here: 65 rows, 4096 x
+// 4096 59 / 53, 16384 x 8192 326 / 348, 128 rows 434 / 348; 1024 x 1024, 384 rows 29 / 29.  Gradients, 65 rows, 4096 x 4096 BF16 53 / 41,
+// 2048 x 2048 25 / 25, 1024 x 1024, 192 rows 20 / 23, 256 rows 27 / 20.
+bool few_rows(const Q4View& w, int rows, int type, bool dx) {
     if (rows <= 64) return true;
     if (rows > 1024 || option_get(OPT_PAIR) || option_get(OPT_K_PIECES)) return false;  // those options are about tcgen05 tiles
+    if (rows <= 128 && type != CAKEB200_F32 && !dx) return true;
     return (long long) rows * w.N * w.K <= (dx ? 1LL << 28 : 1LL << 29);
 }
 
@@ -805,7 +807,7 @@ int product(const char* who, const cakeb200_q4* w, const void* in, long long ld_
     p.ld_in = ld_in; p.ld_out = ld_out; p.rows = rows;
     p.vec = (uintptr_t) in % 16 == 0 && (rows == 1 || (ld_in * (long long) size) % 16 == 0);
     cudaStream_t s = (cudaStream_t) stream;
-    if (!few_rows(p.w, rows, dx)) {
+    if (!few_rows(p.w, rows, type, dx)) {
         if (!workspace || (uintptr_t) workspace % 1024) return bad(who, "this many rows need a workspace on a 1024-byte boundary");
         if (workspace_bytes < q4_gemm_workspace(p.w, rows, type, dx)) return bad(who, "the workspace is too small");
         if (!on_current_device(workspace)) return bad(who, "operands must be device pointers of the current device");
@@ -949,7 +951,7 @@ int cakeb200_q4_dequantize(const cakeb200_q4* w, void* W, long long ldw, int typ
 
 size_t cakeb200_q4_workspace(const cakeb200_q4* w, int rows, int type, int dx) {
     Q4View v;
-    if (q4_view(w, "cakeb200_q4_workspace", &v) || !known_type(type) || few_rows(v, rows, dx != 0)) return 0;
+    if (q4_view(w, "cakeb200_q4_workspace", &v) || !known_type(type) || few_rows(v, rows, type, dx != 0)) return 0;
     return q4_gemm_workspace(v, rows, type, dx != 0);
 }
 

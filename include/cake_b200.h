@@ -434,7 +434,7 @@ int cakeb200_unpack_B(float* B, const float* B_p, int K, int N, int p, const cak
  *     _linear_dx:  dx[r, k] = sum_n dy[r, n] w[n, k],              the gradient of _linear for its input
  *
  * x, bias, y, dy and dx share one type, CAKEB200_F32, _F16 or _BF16; leading dimensions are in elements; sums are FP32.  Few rows
- * (up to 64, or up to 1024 of small weights) are multiplied with the weights as they are, the scales applied in FP32; for more the
+ * (up to 64, up to 128 of 16-bit types in _linear, up to 1024 of small weights) are multiplied with the weights as they are, the scales applied in FP32; for more the
  * weights are expanded first, a slab at a time, into pairs of BF16 that hold them exactly.  Either way a result of 16 bits is rounded
  * once, from FP32 (for FP16 and more rows less than 2^-14 of the products' sizes is left out before).  _workspace
  * tells how many bytes of device memory, on a 1024-byte boundary, the call needs for that (0 for few rows: workspace may then

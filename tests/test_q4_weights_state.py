@@ -81,3 +81,13 @@ def test_state_of_the_same_geometry(cake):
     with pytest.raises(RuntimeError):
         model.load_state_dict(state)
     model.load_state_dict(state, strict=False)
+
+
+def test_which_products_need_a_workspace(cake):
+    """Up to 64 rows none; up to 128 none for y in 16 bits; beyond, by the sizes."""
+    L = cake.lib()
+    W = _weights(cake, 40, 100)
+    W._c.out_features, W._c.in_features = 16384, 8192  # only looked at
+    for t, rows, dx, none in ((2, 64, 0, True), (2, 65, 0, True), (1, 128, 0, True), (2, 129, 0, False), (0, 64, 0, True), (0, 65, 0, False), (2, 64, 1, True),
+                              (2, 65, 1, False)):
+        assert (L.cakeb200_q4_workspace(W._ref, rows, t, dx) == 0) == none, (t, rows, dx)
