@@ -73,10 +73,11 @@ __device__ __forceinline__ double first_factor(double norm, double eps, int up, 
     return inverse * power_of_two(up + shift);
 }
 
-// K blocks of 64 between folds of the main accumulator, whatever the result's type.  4096 x 4096 FP32 with folds every 64 / 128 / 256 /
-// 1024 of K: errors against 64 bits 1.2e-6, 1.6e-6, 3.1e-6, 1.1e-5 (a plain FP32 evaluation: 4.8e-6), 3.36 / 3.16 / 3.05 / 2.97 ms.  With
-// folds every 1024 a BF16 result of 1024 x 4096 differs from the correctly rounded one by 1.7e-4, with these by 9e-5.
-constexpr int FOLD = 2;
+// K blocks of 64 between folds of the main accumulator, whatever the result's type: one, or two where X has more than 512 rows.
+// Errors of FP32 with folds every 64 / 128 of K (and of a plain FP32 evaluation): 137 x 900 1.9e-6 / 3.1e-6 (1.5e-6), 300 x 400 1.1e-6 /
+// 1.7e-6 (2.1e-6), 700 x 800 1.0e-6 / 1.5e-6 (2.8e-6), 4096 x 4096 1.2e-6 / 1.6e-6 (4.8e-6; folds every 256 and 1024: 3.1e-6 and
+// 1.1e-5); times 300 x 400 199 / 197 us, 2048 x 2048 613 / 577, 4096 x 4096 3.39 / 3.16 ms.
+inline int fold_for(int m) { return m > 512 ? 2 : 1; }
 // The tensor core truncates the sum that it adds to.  n additions that grow it evenly, as squares do on the diagonals of X X^T and
 // of its square, lose half a unit in the last place each, on average over the mantissas 0.36 2^-23 of the sum so far, which is (n + 1) / 2
 // times the last one's: that part has a sign, and is put back into those two products.  Not into Q X, whose sums are of either sign
@@ -296,7 +297,7 @@ struct Product : plane::Tiling {
 struct Chain {
     Planes x[2], p, q;           // step s reads x[s % 2] and writes the other
     Product gram, poly, apply, last;
-    int batch, steps;
+    int batch, steps, fold;
     float ka, kb, kc;
     Exponents exponents;
     const double* shifts;        // per matrix, at SHIFT_AT of its NORM_BLOCKS
@@ -381,7 +382,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                 const Product& g = product(i);
                 for (int k = 0; ok && item_at(g, k, unit, units, w); k++) {
                     place(g, w.tile, batch, tm, tn);
-                    ok = e.multiply(turn(g.a, tm), turn(g.b, tn), w.kb0, w.kb1, FOLD);
+                    ok = e.multiply(turn(g.a, tm), turn(g.b, tn), w.kb0, w.kb1, c.fold);
                 }
             }
         }
@@ -453,7 +454,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                 TileAt at;
                 place(g, w.tile, at.batch, tm, tn);
                 factors(at.batch);  // while the tile is multiplied
-                ok = e.collect(w.kb0, w.kb1, FOLD, g.K, kind < 2 ? EVEN_GROWTH : 0.f, sum);
+                ok = e.collect(w.kb0, w.kb1, c.fold, g.K, kind < 2 ? EVEN_GROWTH : 0.f, sum);
                 if (!ok) break;
                 const int row = (int) e.rank * plane::BM + e.quarter() * 32;
                 at.row = tm * C::TILE_M + row;
@@ -550,19 +551,25 @@ __device__ __forceinline__ void get_row(const uint8_t* square, int r, int c0, fl
     }
 }
 
-// D(main) = A B, D(cross) (+)= its two smaller products: squares a and b, b along its rows or down its columns; n columns of
-// the result, `depth` of K, both multiples of 32
-__device__ __forceinline__ void square_product(uint32_t main, uint32_t cross, uint32_t a, uint32_t b, bool down, bool more, int n, int depth) {
+// D(main) + D(main2) = A B, D(cross) (+)= its two smaller products: squares a and b, b along its rows or down its columns; n columns of
+// the result, `depth` of K, both multiples of 32.  main2 takes what is beyond the first 64 of K, or is main.
+__device__ __forceinline__ void square_product(uint32_t main, uint32_t main2, uint32_t cross, uint32_t a, uint32_t b, bool down, bool more, int n, int depth) {
     const uint32_t idesc = plane::idesc_16(Fp16Planes::FORMAT, 128, n) | (down ? 1u << 16 : 0u);
     // down: 64 columns further is a sub-tile (leading offset), 16 rows of K are 2048 bytes; along: 16 of K are 32 bytes, 64 a sub-tile
     const uint64_t da = ptx::make_kmajor_sw128_desc(a), db = ptx::make_kmajor_sw128_desc(b) + (down ? (uint64_t) ((SUB_BYTES >> 4) - 1) << 16 : 0);
+    uint32_t again = 0;
 #pragma unroll 1
     for (int k = 0; k < depth / 16; k++) {
         const uint32_t ka = (uint32_t) ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4, kb = down ? (uint32_t) (k * 2048) >> 4 : ka;
         const uint32_t plane = 2 * SUB_BYTES >> 4, first = more || k > 0;
         plane::umma<false>(cross, da + plane + ka, db + kb, idesc, first);
         plane::umma<false>(cross, da + ka, db + plane + kb, idesc, 1u);
-        plane::umma<false>(main, da + ka, db + kb, idesc, k > 0);
+        plane::umma<false>(main, da + ka, db + kb, idesc, again);
+        again = 1;
+        if (k == 3 && main2 != main) {
+            main = main2;
+            again = 0;
+        }
     }
 }
 
@@ -683,8 +690,6 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
     // room for the parts: the second square of X if there is none, else the place of P and Q, which then needs two more meetings
     const bool apart = squares == 1;
     uint8_t* parts = apart ? x + SQUARE_BYTES : square;
-    // what makes up for truncation in a square's main sums over `depth` values
-    auto grown = [&](int depth) { return 1.f + EVEN_GROWTH * (float) ((min(depth, 128) + 15) / 16 + 1); };
     uint32_t phase = 0;
     // shared memory that this thread wrote is there for the MMAs of all; then one thread issues them and all wait
     auto multiply = [&](auto issue) {
@@ -708,6 +713,19 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         ptx::tmem_ld_wait();
     };
 
+    // What is beyond 64 of K is added up apart, in columns 256 and on, for four truncated additions each; not in the sum of two squares
+    // of X, which take 128 of K each there.
+    auto read_two = [&](uint32_t column, bool two, float up, float up2, float* v, float* u) {
+        read(column, v);
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] *= up;
+        if (!two) return;
+        read(column + 256, u);
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], up2, v[j]);
+    };
+    auto grown = [&](int depth) { return 1.f + EVEN_GROWTH * (float) ((depth + 15) / 16 + 1); };
+    const int first = apart ? 64 : 128;  // columns of X whose squares are summed first
     const float f = times_power(1.f, -2 * p.exponents.up);
     for (int step = 0; step < p.steps; step++) {
         float v[32], u[32];
@@ -715,18 +733,11 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         multiply([&]() {
             for (int q = 0; q < squares; q++) {
                 const uint32_t at = ptx::smem_u32(x + q * SQUARE_BYTES);
-                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 128, at, at, false, q > 0, m32, width(q));
+                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * (apart ? 1 : q), tmem + 128, at, at, false, q > 0, m32, width(q));
             }
         });
         if (in_square) {
-            read(0, v);
-#pragma unroll
-            for (int j = 0; j < 32; j++) v[j] *= grown(columns);
-            if (squares == 2 && width(1) > 0) {
-                read(256, u);
-#pragma unroll
-                for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], grown(columns - 128), v[j]);
-            }
+            read_two(0, columns > first, grown(min(columns, first)), grown(columns - first), v, u);
             read(128, u);
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = f * fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);
@@ -788,32 +799,37 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         }
         // ---- Q, in place of P
         const uint32_t sq = ptx::smem_u32(square);
-        multiply([&]() { square_product(tmem, tmem + 128, sq, sq, false, false, m32, m32); });
+        multiply([&]() { square_product(tmem, tmem + 256, tmem + 128, sq, sq, false, false, m32, m32); });
         if (in_square) {
-            read(0, v);
+            read_two(0, m32 > 64, grown(min(p.m, 64)), grown(p.m - 64), v, u);
             read(128, u);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j] * grown(p.m));
+            for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);
             get_row(square, row, wide, u);
             const float4 k = factors[step];
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = k.x * v[j] + k.y * u[j] + (row == wide + j && row < p.m ? k.z : 0.f);
             put_row(square, row, wide, v);
         }
-        // ---- X
-        multiply([&]() {
-            for (int q = 0; q < squares; q++)
-                if (width(q) > 0) square_product(tmem + 256 * q, tmem + 256 * q + 128, sq, ptx::smem_u32(x + q * SQUARE_BYTES), true, false, width(q), m32);
-        });
+        // ---- X, a square at a time; in the last step at once, as the patches of the result lie where Q is
         const float apply = factors[step].w;
-        if (step + 1 == p.steps) {
-            meet();
-            if (*abort_flag) break;
-        }
+        const bool at_once = squares == 2 && step + 1 == p.steps;
         for (int q = 0; q < squares; q++) {
+            const uint32_t to = at_once ? 256 * q : 0;
+            if (q == 0 || !at_once)
+                multiply([&]() {
+                    for (int i = q; i < (at_once ? 2 : q + 1); i++)
+                        if (width(i) > 0)
+                            square_product(tmem + (at_once ? 256 * i : 0), tmem + (at_once ? 256 * i : 256), tmem + (at_once ? 256 * i : 0) + 128, sq,
+                                           ptx::smem_u32(x + i * SQUARE_BYTES), true, false, width(i), m32);
+                });
+            if (q == 0 && step + 1 == p.steps) {
+                meet();
+                if (*abort_flag) break;
+            }
             if (quarter * 32 >= m32 || wide >= width(q)) continue;
-            read(256 * q, v);
-            read(256 * q + 128, u);
+            read_two(to, !at_once && m32 > 64, 1.f, 1.f, v, u);
+            read(to + 128, u);
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);
             if (step + 1 < p.steps) {
@@ -1153,7 +1169,7 @@ int run(const Source<T>& src, int batch, bool early, const Coefficients& k, void
 
     Chain c = {};
     c.x[0] = l.x[0]; c.x[1] = l.x[1]; c.p = l.p; c.q = l.q;
-    c.batch = batch; c.steps = k.steps;
+    c.batch = batch; c.steps = k.steps; c.fold = fold_for(m);
     c.ka = k.a; c.kb = k.b; c.kc = k.c;
     c.exponents = exponents;
     c.shifts = l.partial + SHIFT_AT;
