@@ -493,7 +493,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
 // X of at most 128 rows and 256 columns per CTA of a cluster stays in shared memory from the first step to the last, as planes
 // in the layout that the MMAs read; one launch does a whole batch, a cluster per matrix, and memory is touched to read G and
 // to write the result.  The grid-wide barriers, stores and loads between products are what small matrices spend their time
-// on otherwise (five steps, FP32: 12 x 96 x 960 188 us in the chain above, 64 here; 1 x 64 x 64 133 and 29).
+// on otherwise (five steps, FP32: 12 x 96 x 960 188 us in the chain above, 70 here; 1 x 64 x 64 119 and 33).
 //
 // A step of CTA k, which holds the columns X_k:
 //     X_k X_k^T on its own; the parts of P are exchanged: every CTA adds up 128 / cluster rows of all parts, in order of the
@@ -1102,8 +1102,8 @@ bool fits_small(int m, int n, int batch, int sm_count, Small* p) {
     while (c * SMALL_COLUMNS < n) c *= 2;
     // half as many columns per CTA make a step shorter as long as all clusters are resident together
     while (c < SMALL_CLUSTER && n > 128 * c && (long long) batch * 2 * c <= sm_count * 3 / 4) c *= 2;
-    // One CTA per matrix is faster than the chain for any batch (2000 of 64 x 128: 0.60 ms, 1.09 in the chain).  Clusters are
-    // as long as few wait for others: of 8 CTAs, 128 x 2048, 32 matrices 298 us (chain 320), 64 matrices 497 (474).
+    // One CTA per matrix is faster than the chain for any batch (2000 of 64 x 128: 0.47 ms, 1.19 in the chain).  Clusters are
+    // as long as few wait for others: of 8 CTAs, 128 x 2048, 32 matrices 326 us (chain 326), 48 434 (405), 64 x 1000, 64 matrices 145 (280).
     if (c > 1 && (long long) batch * c > 3ll * sm_count) return false;
     p->cluster = c;  // n > 64 c, so that slices rounded up to 8 leave every CTA some columns
     p->slice = ((n + c - 1) / c + 7) / 8 * 8;

@@ -608,8 +608,9 @@ struct Costs {
 };
 // A K block: the MMAs (64 and 128 clocks each) or the shared-memory traffic (16 KB per plane written, 8 KB per MMA read, 128 bytes
 // a clock), whichever is longer, at 1.85 GHz and with the 10 % that both lose in practice (three products of two planes:
-// 0.75 and 0.93 measured); or its way from L2, 47 bytes a clock at best (one product of one plane: 0.44 in either form, with
-// four stages as with six; 500 x 4096 x 4096 in BF16 takes 34.3 us in parts on pairs, 41.7 whole on single SMs).
+// 0.75 and 0.93 measured); or its way from L2, 47 bytes a clock at best (measured on products of one plane, four stages as well as six),
+// which decides for one plane against two on single SMs.  500 x 4096 x 4096 in BF16 takes 51 us on pairs, 59 on single SMs; 65 x 4096
+// x 4096 41 and 37; in every shape of 65 to 2000 rows and 2048^2 to 16384 x 8192 weights that was timed the faster form is chosen.
 inline Costs costs_of(int ta, int tb, int products, double between) {
     const double load = (ta + tb) * 16384.0 / 47.0 / 1.1, smem = std::max(load, ((ta + tb) * 16384.0 + products * 4 * 8192.0) / 128.0);
     Costs c;
