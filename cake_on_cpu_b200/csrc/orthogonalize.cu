@@ -60,10 +60,10 @@ __device__ __forceinline__ StepExponents exponents_of(const Exponents& e, int sh
     for (int i = 0; i <= step; i++) advance(e, e.q[i], e.x[i + 1], s);
     return s;
 }
-// k 2^e for e between -252 and 254; beyond, zero and infinity
+// k 2^e for e between -252 and 254; beyond, zero and infinity (but a coefficient of zero stays zero)
 __device__ __forceinline__ float times_power(float k, int e) {
     auto power = [](int e) { return __int_as_float(e < -126 ? 0 : e > 127 ? 0x7f800000 : (e + 127) << 23); };
-    return k * power(e >> 1) * power(e - (e >> 1));
+    return k == 0.f ? 0.f : k * power(e >> 1) * power(e - (e >> 1));
 }
 __device__ __forceinline__ double power_of_two(int e) { return __hiloint2double((e + 1023) << 20, 0); }
 // The factor that makes 2^(up + shift) X_0 of a matrix of that norm: 2^-shift is the first power of two at or above norm / (norm + eps).

@@ -102,6 +102,18 @@ def test_coefficients_that_shrink_or_grow(cake, shape):
             cake.cake_muon_step(d.clone(), d, torch.zeros_like(d), 0.1, steps=steps, coeffs=coeffs)
 
 
+@pytest.mark.parametrize("shape", [(20, 30), (150, 210)], ids=str)
+def test_a_large_result_that_fp32_holds(cake, shape):
+    """X grows to 1e35, and its square, which nothing needs, is beyond FP32: coefficients of zero stay zero."""
+    import torch
+    rng = np.random.default_rng(shape[0])
+    g = rng.standard_normal(shape).astype(np.float32)
+    got = cake.cake_orthogonalize(torch.from_numpy(g).cuda(), steps=18, coeffs=(100.0, 0.0, 0.0)).double().cpu().numpy()
+    want = g.astype(np.float64) / (np.linalg.norm(g.astype(np.float64)) + np.float64(np.float32(EPS))) * 1e36
+    # 18 roundings of X to 22 bits and a sign, and of 100, which 22 bits hold
+    assert np.all(np.abs(got - want) <= 18 * 2.0 ** -22 * np.abs(want))
+
+
 @pytest.mark.parametrize("shape", [(1, 1), (1, 7), (9, 1), (5, 5), (16, 16), (12, 40), (150, 150)], ids=str)
 def test_matrices_with_one_entry_a_row(cake, shape):
     """Every sum is one product, so nothing is truncated and nothing may be put back: what is left are the roundings of
