@@ -74,15 +74,22 @@ __device__ __forceinline__ double first_factor(double norm, double eps, int up, 
 }
 
 // K blocks of 64 between folds of the main accumulator, whatever the result's type: one, or two where X has more than 512 rows.
-// Errors of FP32 with folds every 64 / 128 of K (and of a plain FP32 evaluation): 137 x 900 1.9e-6 / 3.1e-6 (1.5e-6), 300 x 400 1.1e-6 /
-// 1.7e-6 (2.1e-6), 700 x 800 1.0e-6 / 1.5e-6 (2.8e-6), 4096 x 4096 1.2e-6 / 1.6e-6 (4.8e-6; folds every 256 and 1024: 3.1e-6 and
-// 1.1e-5); times 300 x 400 199 / 197 us, 2048 x 2048 613 / 577, 4096 x 4096 3.39 / 3.16 ms.
+// Errors of FP32 with folds every 64 / 128 of K (and of a plain FP32 evaluation): 137 x 900 1.3e-6 / 2.3e-6 (1.5e-6), 300 x 400 0.9e-6 /
+// 1.3e-6 (2.0e-6), 700 x 800 0.9e-6 / 1.3e-6 (2.5e-6), 4096 x 4096 1.1e-6 / 1.4e-6 (4.8e-6); times 300 x 400 206 / 201 us, 2048 x 2048
+// 624 / 580, 4096 x 4096 3.39 / 3.12 ms.
 inline int fold_for(int m) { return m > 512 ? 2 : 1; }
-// The tensor core truncates the sum that it adds to.  n additions that grow it evenly, as squares do on the diagonals of X X^T and
-// of its square, lose half a unit in the last place each, on average over the mantissas 0.36 2^-23 of the sum so far, which is (n + 1) / 2
-// times the last one's: that part has a sign, and is put back into those two products.  Not into Q X, whose sums are of either sign
-// and, while X is small, of a single term.
-constexpr float EVEN_GROWTH = 0.18f * 1.1920929e-7f;
+// The tensor core truncates the sum that it adds to, which has a sign where sums do not: it is put back into the two products whose
+// sums are of squares, by the additions that they really had, as measured in 2^-24 of the sum.
+//   X X^T: sums that grow evenly lose 2.2, 3.0, 3.9 and 7.9 in 2, 3, 4 and 8 additions (rows of 32 to 256 random values).
+//   P P: the largest product of a sum on the diagonal is there from some addition on, and all later ones take from the whole: 1.8 for
+//   each but one in folds of 64 (5.5 in four, from the bias of single steps), 1.2 in folds of 128 (errors of 2048 x 2048 1.25e-6,
+//   with 1.8 1.5e-6).
+// A sum of a single addition is left alone, and so is Q X, whose sums are of either sign and, while X is small, of a single term.
+// Errors over those of a plain FP32 evaluation, gradients of 32 to 128 rows and up to 2048 columns: median 0.90, 90 % below 1.22; with
+// 0.36 (n + 1) in both products instead 1.31 and 1.94.  Matrices with one entry a row have nothing to put back and pay for it: 2e-6.
+__device__ __forceinline__ plane::Loss gram_loss() { return {0.96f * 5.9604645e-8f, 0}; }
+__device__ __forceinline__ plane::Loss square_loss(int fold) { return {(fold > 1 ? 1.2f : 1.8f) * 5.9604645e-8f, 1}; }
+__device__ __forceinline__ plane::Loss no_loss() { return {0.f, 0}; }
 
 // eight consecutive elements; `vec`: all eight exist and the address is 16-byte aligned
 __device__ __forceinline__ void get8(const float* p, int n, bool vec, float* v) {
@@ -454,7 +461,7 @@ newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
                 TileAt at;
                 place(g, w.tile, at.batch, tm, tn);
                 factors(at.batch);  // while the tile is multiplied
-                ok = e.collect(w.kb0, w.kb1, c.fold, g.K, kind < 2 ? EVEN_GROWTH : 0.f, sum);
+                ok = e.collect(w.kb0, w.kb1, c.fold, g.K, kind == 0 ? gram_loss() : kind == 1 ? square_loss(c.fold) : no_loss(), sum);
                 if (!ok) break;
                 const int row = (int) e.rank * plane::BM + e.quarter() * 32;
                 at.row = tm * C::TILE_M + row;
@@ -724,7 +731,6 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
 #pragma unroll
         for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], up2, v[j]);
     };
-    auto grown = [&](int depth) { return 1.f + EVEN_GROWTH * (float) ((depth + 15) / 16 + 1); };
     const int first = apart ? 64 : 128;  // columns of X whose squares are summed first
     const float f = times_power(1.f, -2 * p.exponents.up);
     for (int step = 0; step < p.steps; step++) {
@@ -737,7 +743,7 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
             }
         });
         if (in_square) {
-            read_two(0, columns > first, grown(min(columns, first)), grown(columns - first), v, u);
+            read_two(0, columns > first, gram_loss().factor(min(columns, first)), gram_loss().factor(columns - first), v, u);
             read(128, u);
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = f * fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);
@@ -801,7 +807,7 @@ small_kernel(const Source<T> s, const Small p, const typename Last::Args last) {
         const uint32_t sq = ptx::smem_u32(square);
         multiply([&]() { square_product(tmem, tmem + 256, tmem + 128, sq, sq, false, false, m32, m32); });
         if (in_square) {
-            read_two(0, m32 > 64, grown(min(p.m, 64)), grown(p.m - 64), v, u);
+            read_two(0, m32 > 64, square_loss(1).factor(min(p.m, 64)), square_loss(1).factor(p.m - 64), v, u);
             read(128, u);
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = fmaf(u[j], 1.f / Fp16Planes::TERM, v[j]);

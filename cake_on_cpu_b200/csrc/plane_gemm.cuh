@@ -235,6 +235,14 @@ __device__ __forceinline__ void join_parts(const float* parts, int b, int total,
     }
 }
 
+// What truncation takes from a sum, where that has a sign: `each` of it for every addition but the first `but`.
+struct Loss {
+    float each;
+    int but;
+    // what makes up for it in a sum over `depth` values
+    __device__ __forceinline__ float factor(int depth) const { return 1.f + each * (float) ((depth + UMMA_K - 1) / UMMA_K - but); }
+};
+
 // What a CTA's roles share.  Every role walks the same sequence of (tile, K range) items and keeps its own place in it.
 template <class Format, int TA, int TB, bool PAIR>
 struct Engine {
@@ -395,7 +403,7 @@ struct Engine {
     // [32 * (warp % 4), +32) of tensor memory, so two warps share a quarter of the rows and take half of the columns each.
     __device__ __forceinline__ int quarter() const { return warp & 3; }
     __device__ __forceinline__ int half() const { return (warp - 4) >> 2; }
-    __device__ __forceinline__ bool collect(int kb0, int kb1, int chunk, int K, float growth, float (&sum)[COLS]) {
+    __device__ __forceinline__ bool collect(int kb0, int kb1, int chunk, int K, const Loss& loss, float (&sum)[COLS]) {
         const uint32_t at = ((uint32_t) (quarter() * 32) << 16) + (uint32_t) (half() * COLS);
         float v[64];
 #pragma unroll
@@ -405,8 +413,7 @@ struct Engine {
             if (!__all_sync(0xffffffffu, ok)) return false;  // the tensor-memory loads below need the whole warp
             fold_phase ^= 1;
             tcgen05_fence_after();
-            // sums that grow evenly: `growth` of what is read for each addition that had something to add, and one more
-            const float up = 1.f + growth * (float) (min(min(chunk, kb1 - kb) * (BK / UMMA_K), (K - kb * BK + UMMA_K - 1) / UMMA_K) + 1);
+            const float up = loss.factor(min(min(chunk, kb1 - kb) * BK, K - kb * BK));
 #pragma unroll
             for (int c = 0; c < COLS; c += 64) {
                 tmem_ld64(tmem_main + at + (uint32_t) c, v);
@@ -479,7 +486,7 @@ plane_gemm_kernel(const __grid_constant__ OperandMaps map_a, const __grid_consta
         many_registers();
         float sum[C::COLS];
         for (int k = 0; item_at(p.t, k, unit, units, w); k++) {
-            if (!e.collect(w.kb0, w.kb1, p.chunk, p.t.K, 0.f, sum)) break;
+            if (!e.collect(w.kb0, w.kb1, p.chunk, p.t.K, Loss{0.f, 0}, sum)) break;
             TileAt at;
             place(p.t, w.tile, at.batch, tm, tn);
             const int row = (int) e.rank * BM + e.quarter() * 32;
