@@ -397,8 +397,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 
 // A CTA computes one k block (64 input features) x 8 NT rows; its warps share out the block rows of the CTA, the CTAs
 // of a cluster those of the product.  The reduction runs over output features, whose scales differ, so the scale goes
-// into the other operand: dy[r, n] s[n, g], formed in FP32 and split into TERMS bf16 terms (two for 16-bit types: 2^-16
-// relative, far below their own rounding; three for FP32).  Sums of one block row (16 n) leave the MMA for an FP32 total.
+// into the other operand: dy[r, n] s[n, g], formed in FP32 and split into TERMS bf16 terms (two for 16-bit types, each rounded
+// to nearest: 2^-17 relative and of either sign, far below their own rounding; three for FP32, exactly).  Sums of one block row (16 n) leave the MMA for an FP32 total.
 template <typename T, int NT, int GROUPS, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
 q4_linear_dx_kernel(const Q4Args p) {
@@ -474,8 +474,13 @@ q4_linear_dx_kernel(const Q4Args p) {
             uint32_t b[NT][2][TERMS];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                split_pair<TERMS>(v[nt][0] * s[0], v[nt][1] * s[1], b[nt][0]);
-                split_pair<TERMS>(v[nt][2] * s[2], v[nt][3] * s[3], b[nt][1]);
+                if constexpr (TERMS == 2) {
+                    round_pair(v[nt][0] * s[0], v[nt][1] * s[1], b[nt][0]);
+                    round_pair(v[nt][2] * s[2], v[nt][3] * s[3], b[nt][1]);
+                } else {
+                    split_pair<TERMS>(v[nt][0] * s[0], v[nt][1] * s[1], b[nt][0]);
+                    split_pair<TERMS>(v[nt][2] * s[2], v[nt][3] * s[3], b[nt][1]);
+                }
             }
             const uint32_t sub_lo = zero_pair<M>(now.zeros[m] & 15u), sub_hi = zero_pair<M>((now.zeros[m] >> 8) & 15u);
 #pragma unroll

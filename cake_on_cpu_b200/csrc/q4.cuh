@@ -77,6 +77,17 @@ __device__ __forceinline__ void split_pair(float v0, float v1, uint32_t* out) {
     }
 }
 
+// The same in two terms, each rounded to nearest: within 2^-17 of v, on either side of it.
+__device__ __forceinline__ void round_pair(float v0, float v1, uint32_t* out) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v0, v1);
+        out[t] = *reinterpret_cast<const uint32_t*>(&h);
+        v0 -= __uint_as_float(out[t] << 16);
+        v1 -= __uint_as_float(out[t] & 0xffff0000u);
+    }
+}
+
 __device__ __forceinline__ float q4_scale(uint16_t bits, int is_bf16) {
     return is_bf16 ? __uint_as_float((uint32_t) bits << 16) : __half2float(__ushort_as_half(bits));
 }

@@ -113,3 +113,22 @@ def test_ends_of_the_range_of_fp32(cake, rows, expanded):
     x[0, 3], x[1, 5], x[2, 0] = torch.finfo(torch.float32).max, 1.1754944e-38 * 65536, 1 + 2.0 ** -23
     y = cake.cake_q4_linear(x, W4)
     assert torch.equal(y, x.sum(1, keepdim=True).expand(rows, 16))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("rows", [1, 8, 30])
+def test_gradients_of_few_rows_are_cut_on_either_side(cake, rows, dtype):
+    """dy s goes into the product as two terms within 2^-17 of it.  With 16 output features a sum is one multiplication of 16 pairs, twice: four
+    roundings of 2^-23 at most.  So a result is the correctly rounded one unless a border between two of them lies as near as that."""
+    import torch
+    rng = np.random.default_rng(rows)
+    N, K = 16, 4000
+    z = np.zeros((N, K // 32), dtype=np.uint8)
+    W4, w = _make(cake, rng, N, K, 32, z, torch.float16)
+    t = getattr(torch, dtype)
+    dy = torch.from_numpy(np.abs(rng.standard_normal((rows, N))).astype(np.float32)).to(t)
+    want = dy.double().numpy() @ w  # of positive terms
+    got = cake.cake_q4_linear_dx(dy.cuda(), W4).double().cpu().numpy()
+    _, e = np.frexp(want)
+    ulp = np.ldexp(torch.finfo(t).eps, e - 1)
+    assert np.all(np.abs(got - want) <= ulp / 2 + want * (2.0 ** -17 + 4 * 2.0 ** -23))
